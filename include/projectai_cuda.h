@@ -236,6 +236,57 @@ pai_status pai_sdpa_decode(pai_ctx* ctx, const pai_tensor* q, const pai_tensor* 
 pai_status pai_linear_fused(pai_ctx* ctx, const pai_tensor* x, const pai_tensor* norm_weight, float eps,
                             const pai_tensor* weights, int32_t n_weights, int32_t mode, const pai_tensor* residual,
                             pai_tensor* out);
+/* ==== Paged KV cache: requests of different lengths in one step (no counterpart in the reference) ====
+ * The decode-step ops above hold a batch whose rows all stand at one position. A server's requests join and end at
+ * different steps and have different lengths, so their keys and values live in pages: caches [pages, KVH, P, D] (P
+ * positions a page, unit head-dim stride, both caches of one layout), and table [N, max_pages], whose row i names
+ * request i's pages in order. Position j of request i sits at offset j % P of page table[i, j / P]; its slot is
+ * page * P + j % P. Rows of a step's q, k and v [rows, heads, D] are the requests' new tokens one request after the
+ * other: request i's are rows q_start[i] .. q_start[i+1]-1. Ids, lengths, positions and slots are integral F32 values
+ * read on the device, so a step can be captured (pai_graph_begin) and replayed: pages * P, max_pages * P and the
+ * number of rows may be at most 2^24, up to which F32 holds every integer. Device values that are out of range, not
+ * integral or contradict one another set the device error flag (pai_check_device_error), and what they concern is
+ * skipped as described at each op; nothing outside the given views is read or written for them. */
+/* Plans a step: which pages its new tokens take, and each token's slot and position. lengths [N]: tokens in the cache;
+ * new_tokens [N]: tokens this step adds, 0 = none, -1 = the request has ended. ring [R] holds free page ids from
+ * element state[0] on (modulo R), state[1] of them; R is the number of pages that exist, and ids are in [0, R).
+ * Requests take their pages from the ring in request order, page order within a request: request i takes
+ * ceil((lengths[i] + new_tokens[i]) / P) - ceil(lengths[i] / P), written into its row of table (in place; entries of
+ * pages it held stay). The pages of ended requests go back behind the ring's last free one (in place), to be taken by
+ * later steps; their rows of table stay as they are, no longer valid. Results, all newly allocated: q_start [N+1],
+ * kv_len [N] (lengths[i] + new_tokens[i], 0 for an ended request: the next step's lengths), slots [rows] and
+ * positions [rows] of the new tokens (rows behind the last token: slot -1, position 0) and the ring's next state [2].
+ * The inputs lengths, new_tokens and state are not changed, so a step can be planned again. Tokens of a page that table
+ * or ring names wrongly (an id outside [0, R)) get slot -1 and set the error flag. When a value is invalid, a request
+ * needs more than max_pages pages, the tokens exceed rows or the ring is short of pages, the error flag is set and no
+ * request gets anything: table and ring stay as they are, q_start is 0 everywhere, every slot -1, kv_len = lengths
+ * (0 where that is invalid) and the state is the one given. table, ring and the inputs must not overlap. */
+pai_status pai_paged_plan(pai_ctx* ctx, const pai_tensor* lengths, const pai_tensor* new_tokens, const pai_tensor* table,
+                          const pai_tensor* ring, const pai_tensor* state, int32_t page_size, int32_t rows,
+                          pai_tensor* q_start, pai_tensor* kv_len, pai_tensor* slots, pai_tensor* positions,
+                          pai_tensor* next_state);
+/* pai_rope_append over pages: q [rows, H, D] and k [rows, KVH, D] are rotated with the table rows `positions` [rows] of
+ * full [T, D] tables (RotaryEmbedding's values); q goes to the new tensor q_out [rows, H, D], and k, with v copied, to
+ * `slots` [rows] of the caches. Rows of slot -1 write nothing to the caches (their q is still rotated). A slot outside
+ * [-1, pages * P) sets the error flag and writes nothing; a position outside the tables too, and its row of q_out is
+ * 0. Slots other than -1 must differ from one another (pai_paged_plan's do): of two rows with one slot, each element
+ * that the cache ends up with is one of theirs. q, k and v rows may be strided (unit head-dim stride). */
+pai_status pai_paged_rope_append(pai_ctx* ctx, const pai_tensor* q, const pai_tensor* k, const pai_tensor* v,
+                                 const pai_tensor* cos_table, const pai_tensor* sin_table, const pai_tensor* positions,
+                                 const pai_tensor* slots, const pai_tensor* k_cache, const pai_tensor* v_cache,
+                                 pai_tensor* q_out);
+/* Causal attention of a step's new tokens over their requests' pages, the values of pai_sdpa_fwd per request: row r of
+ * request i stands at position p = kv_len[i] - (q_start[i+1] - q_start[i]) + (r - q_start[i]) and attends positions
+ * 0 .. p of table's row i. q [rows, H, D] (any strides, unit along D), H % KVH == 0, D <= 128; out [rows, H, D]. Rows
+ * without a key (p < 0) and rows that belong to no request are 0. max_new bounds the new tokens of one request (0: rows
+ * is taken); it is a host value because the kernels and their launch sizes are chosen by it. One long chunk and many
+ * single tokens may share a call. Cache positions that a row does not attend may hold anything, NaN and infinities
+ * included. A q_start that does not rise or leaves [0, rows], a kv_len outside [0, max_pages * P] or a request of more
+ * than max_new tokens sets the error flag and the request is skipped (its rows of out are unspecified); a page id
+ * outside the caches sets it too, and its positions are not attended. */
+pai_status pai_sdpa_paged(pai_ctx* ctx, const pai_tensor* q, const pai_tensor* k_cache, const pai_tensor* v_cache,
+                          const pai_tensor* table, const pai_tensor* q_start, const pai_tensor* kv_len, float scale,
+                          int32_t max_new, pai_tensor* out);
 /* Captures every op issued on the context between begin and end into one CUDA graph; no host upload or
  * synchronising call may come in between. The device memory the captured ops use stays reserved for the graph
  * until pai_graph_destroy, so tensors created during the capture hold each replay's results. */

@@ -14,6 +14,7 @@
 // output element keeps its sequential accumulation order, and cross-row sums (the cross-entropy total) are
 // reduced in row order afterwards, so results are bit-identical for every thread count.
 #include "projectai_cuda.h"
+#include "paged_args.h"
 
 #include <cerrno>
 #include <cmath>
@@ -59,6 +60,7 @@ struct pai_ctx {
   std::vector<uint8_t> ds_bytes;
   int ds_elem = 0, ds_seq = 0;
   int64_t ds_blocks = 0;
+  int error_flag = 0;  // what the CUDA library's kernels record for device values out of range
   // the last checkpoint read by oracle_ckpt_load
   std::string ck_meta;
   std::vector<std::string> ck_names;
@@ -1021,5 +1023,189 @@ ORC_API pai_status oracle_dataset_close(pai_ctx* c) {
   std::vector<uint8_t>().swap(c->ds_bytes);
   c->ds_elem = c->ds_seq = 0;
   c->ds_blocks = 0;
+  return PAI_OK;
+}
+
+// ---------------------------------------------------------------- paged KV cache (no counterpart in the reference)
+// The definitions of pai_paged_plan, pai_paged_rope_append and pai_sdpa_paged (include/projectai_cuda.h), request by
+// request. A wrong device value sets the context's error flag, as the CUDA kernels do.
+namespace {
+
+// An integral F32 value in [lo, hi].
+bool integral(float f, int64_t lo, int64_t hi, int64_t* out) {
+  if (!(f >= (float)lo && f <= (float)hi) || f != floorf(f)) return false;
+  *out = (int64_t)f;
+  return true;
+}
+
+float& at1(const pai_tensor& t, int64_t i) { return buf(t)[t.offset + i * t.strides[0]]; }
+float& at2(const pai_tensor& t, int64_t i, int64_t j) { return buf(t)[t.offset + i * t.strides[0] + j * t.strides[1]]; }
+float* at3(const pai_tensor& t, int64_t i, int64_t j, int64_t k) {
+  return buf(t) + t.offset + i * t.strides[0] + j * t.strides[1] + k * t.strides[2];
+}
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+}  // namespace
+
+ORC_API pai_status oracle_check_device_error(pai_ctx* c, int32_t* code) {
+  CHECK_CTX(c);
+  const int e = c->error_flag;
+  c->error_flag = 0;
+  if (code) *code = e;
+  return e ? fail(PAI_ERR_TIMEOUT, "a kernel reported device error %d", e) : PAI_OK;
+}
+
+ORC_API pai_status oracle_paged_plan(pai_ctx* c, const pai_tensor* lengths, const pai_tensor* new_tokens,
+                                     const pai_tensor* table, const pai_tensor* ring, const pai_tensor* state,
+                                     int32_t page_size, int32_t rows, pai_tensor* q_start, pai_tensor* kv_len,
+                                     pai_tensor* slots, pai_tensor* positions, pai_tensor* next_state) {
+  CHECK_CTX(c);
+  const pai_tensor* ins[5] = {lengths, new_tokens, table, ring, state};
+  const char* names[5] = {"lengths", "new_tokens", "table", "ring", "state"};
+  for (int i = 0; i < 5; i++) TRY(check_desc(c, ins[i], names[i]));
+  TRY(pai_paged::check_plan(fail, lengths, new_tokens, table, ring, state, page_size, rows));
+  const int n = lengths->dims[0];
+  const int64_t P = page_size, R = ring->dims[0], MB = table->dims[1];
+  int32_t d1 = n + 1, dn = n, dr = rows, d2 = 2;
+  pai_tensor qs, kl, sl, ps, ns;
+  TRY(alloc(c, 1, &d1, PAI_F32, &qs));
+  TRY(alloc(c, 1, &dn, PAI_F32, &kl));
+  TRY(alloc(c, 1, &dr, PAI_F32, &sl));
+  TRY(alloc(c, 1, &dr, PAI_F32, &ps));
+  TRY(alloc(c, 1, &d2, PAI_F32, &ns));
+  for (int t = 0; t < rows; t++) buf(sl)[t] = -1.0f;
+  std::vector<int64_t> len((size_t)n), add((size_t)n), have((size_t)n), need((size_t)n), back((size_t)n);
+  int64_t head = 0, count = 0, tokens = 0, taken = 0, freed = 0;
+  bool ok = integral(at1(*state, 0), 0, R > 0 ? R - 1 : 0, &head) && integral(at1(*state, 1), 0, R, &count);
+  for (int i = 0; i < n; i++) {
+    const size_t u = (size_t)i;
+    int64_t l = 0, a = 0;
+    const bool lok = integral(at1(*lengths, i), 0, MB * P, &l), aok = integral(at1(*new_tokens, i), -1, rows, &a);
+    buf(kl)[i] = lok ? (float)l : 0.0f;
+    if (!lok || !aok || l + (a > 0 ? a : 0) > MB * P) ok = false;
+    len[u] = l;
+    add[u] = a > 0 ? a : 0;
+    have[u] = ceil_div(l, P);
+    need[u] = a < 0 ? 0 : ceil_div(l + add[u], P) - have[u];
+    back[u] = a < 0 ? have[u] : 0;
+    tokens += add[u];
+    taken += need[u];
+    freed += back[u];
+  }
+  if (tokens > rows || taken > count || count + freed > R) ok = false;
+  if (!ok) {
+    c->error_flag = 70;
+    buf(ns)[0] = at1(*state, 0);
+    buf(ns)[1] = at1(*state, 1);
+  } else {
+    int64_t t = 0, k = 0, b = 0;
+    for (int i = 0; i < n; i++) {
+      const size_t u = (size_t)i;
+      for (int64_t j = 0; j < back[u]; j++) at1(*ring, (head + count + b++) % R) = at2(*table, i, j);
+      for (int64_t j = 0; j < need[u]; j++) at2(*table, i, have[u] + j) = at1(*ring, (head + k++) % R);
+      for (int64_t j = 0; j < add[u]; j++, t++) {
+        const int64_t pos = len[u] + j;
+        int64_t page = 0;
+        buf(ps)[t] = (float)pos;
+        if (integral(at2(*table, i, pos / P), 0, R - 1, &page)) buf(sl)[t] = (float)(page * P + pos % P);
+        else c->error_flag = 71;
+      }
+      buf(qs)[i + 1] = (float)t;
+      buf(kl)[i] = at1(*new_tokens, i) < 0.0f ? 0.0f : (float)(len[u] + add[u]);
+    }
+    buf(ns)[0] = R > 0 ? (float)((head + taken) % R) : 0.0f;
+    buf(ns)[1] = (float)(count - taken + freed);
+  }
+  *q_start = qs; *kv_len = kl; *slots = sl; *positions = ps; *next_state = ns;
+  return PAI_OK;
+}
+
+ORC_API pai_status oracle_paged_rope_append(pai_ctx* c, const pai_tensor* q, const pai_tensor* k, const pai_tensor* v,
+                                            const pai_tensor* cos_table, const pai_tensor* sin_table,
+                                            const pai_tensor* positions, const pai_tensor* slots,
+                                            const pai_tensor* k_cache, const pai_tensor* v_cache, pai_tensor* q_out) {
+  CHECK_CTX(c);
+  const pai_tensor* ins[9] = {q, k, v, cos_table, sin_table, positions, slots, k_cache, v_cache};
+  const char* names[9] = {"q", "k", "v", "cos", "sin", "positions", "slots", "k_cache", "v_cache"};
+  for (int i = 0; i < 9; i++) TRY(check_desc(c, ins[i], names[i]));
+  TRY(pai_paged::check_append(fail, q, k, v, cos_table, sin_table, positions, slots, k_cache, v_cache));
+  const int rows = q->dims[0], H = q->dims[1], KVH = k->dims[1], D = q->dims[2], half = D / 2;
+  const int64_t P = k_cache->dims[2];
+  pai_tensor r;
+  TRY(alloc(c, 3, q->dims, PAI_F32, &r));
+  for (int t = 0; t < rows; t++) {
+    int64_t pos = 0, slot = 0;
+    if (!integral(at1(*positions, t), 0, (int64_t)cos_table->dims[0] - 1, &pos)) { c->error_flag = 72; continue; }
+    const float* cr = &at2(*cos_table, pos, 0);
+    const float* sr = &at2(*sin_table, pos, 0);
+    auto rotate = [&](const float* x, float* y) {
+      for (int j = 0; j < half; j++) {
+        const float x0 = x[j], x1 = x[j + half];
+        y[j] = x0 * cr[j] + -x1 * sr[j];
+        y[j + half] = x1 * cr[j + half] + x0 * sr[j + half];
+      }
+    };
+    for (int h = 0; h < H; h++) rotate(at3(*q, t, h, 0), buf(r) + ((int64_t)t * H + h) * D);
+    if (at1(*slots, t) == -1.0f) continue;
+    if (!integral(at1(*slots, t), 0, k_cache->dims[0] * P - 1, &slot)) { c->error_flag = 73; continue; }
+    for (int h = 0; h < KVH; h++) {
+      rotate(at3(*k, t, h, 0), at3(*k_cache, slot / P, h, slot % P));
+      memcpy(at3(*v_cache, slot / P, h, slot % P), at3(*v, t, h, 0), (size_t)D * 4);
+    }
+  }
+  *q_out = r;
+  return PAI_OK;
+}
+
+ORC_API pai_status oracle_sdpa_paged(pai_ctx* c, const pai_tensor* q, const pai_tensor* k_cache, const pai_tensor* v_cache,
+                                     const pai_tensor* table, const pai_tensor* q_start, const pai_tensor* kv_len,
+                                     float scale, int32_t max_new, pai_tensor* out) {
+  CHECK_CTX(c);
+  const pai_tensor* ins[6] = {q, k_cache, v_cache, table, q_start, kv_len};
+  const char* names[6] = {"q", "k_cache", "v_cache", "table", "q_start", "kv_len"};
+  for (int i = 0; i < 6; i++) TRY(check_desc(c, ins[i], names[i]));
+  TRY(pai_paged::check_sdpa(fail, q, k_cache, v_cache, table, q_start, kv_len, max_new));
+  const int rows = q->dims[0], H = q->dims[1], D = q->dims[2], n = table->dims[0], KVH = k_cache->dims[1], g = H / KVH;
+  const int64_t P = k_cache->dims[2], cap = table->dims[1] * P;
+  const int64_t most = max_new > 0 ? max_new : rows;
+  pai_tensor r;
+  TRY(alloc(c, 3, q->dims, PAI_F32, &r));
+  for (int i = 0; i < n; i++) {
+    int64_t a = 0, b = 0, len = 0;
+    if (!integral(at1(*q_start, i), 0, rows, &a) || !integral(at1(*q_start, i + 1), 0, rows, &b) ||
+        !integral(at1(*kv_len, i), 0, cap, &len) || b < a || b - a > most) {
+      c->error_flag = 74;
+      continue;
+    }
+    std::vector<int64_t> page((size_t)ceil_div(len, P));
+    for (size_t j = 0; a < b && j < page.size(); j++)
+      if (!integral(at2(*table, i, (int64_t)j), 0, (int64_t)k_cache->dims[0] - 1, &page[j])) { c->error_flag = 75; page[j] = -1; }
+    for (int64_t t = a; t < b; t++) {
+      const int64_t pos = len - (b - a) + (t - a);
+      for (int h = 0; h < H; h++) {
+        const float* x = at3(*q, t, h, 0);
+        std::vector<double> s, acc((size_t)D, 0.0);
+        std::vector<int64_t> key;
+        double top = -INFINITY, total = 0.0;
+        for (int64_t j = 0; j <= pos; j++) {
+          if (page[(size_t)(j / P)] < 0) continue;
+          const float* y = at3(*k_cache, page[(size_t)(j / P)], h / g, j % P);
+          double dot = 0.0;
+          for (int e = 0; e < D; e++) dot += (double)x[e] * (double)y[e];
+          s.push_back(dot * (double)scale);
+          key.push_back(j);
+          if (s.back() > top || s.back() != s.back()) top = s.back();
+        }
+        for (size_t m = 0; m < s.size(); m++) {
+          const double w = exp(s[m] - top);
+          const float* y = at3(*v_cache, page[(size_t)(key[m] / P)], h / g, key[m] % P);
+          total += w;
+          for (int e = 0; e < D; e++) acc[(size_t)e] += w * (double)y[e];
+        }
+        for (int e = 0; e < D; e++) buf(r)[(t * H + h) * D + e] = s.empty() ? 0.0f : (float)(acc[(size_t)e] / total);
+      }
+    }
+  }
+  *out = r;
   return PAI_OK;
 }

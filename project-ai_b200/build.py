@@ -63,7 +63,7 @@ def build_cuda(verbose: bool = False) -> Path:
     BUILD.mkdir(exist_ok=True)
     LIB.mkdir(exist_ok=True)
     sources = sorted(CSRC.glob("*.cu"))
-    headers = sorted(CSRC.glob("*.cuh")) + [INCLUDE / "projectai_cuda.h"]
+    headers = sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + [INCLUDE / "projectai_cuda.h"]
     jobs = []
     for src in sources:
         obj = BUILD / (src.stem + ".o")

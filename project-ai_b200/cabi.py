@@ -154,6 +154,14 @@ _SIGS = {
     "dataset_batch": [c_void_p, POINTER(c_int64), c_int32, T, T],
     "dataset_close": [c_void_p],
     "rmsnorm_bwd_noalloc": [c_void_p, T, T, T, c_float, T, T],
+    "write": [c_void_p, POINTER(c_float), c_int64, T],
+    "paged_plan": [c_void_p, T, T, T, T, T, c_int32, c_int32, T, T, T, T, T],
+    "paged_rope_append": [c_void_p, T, T, T, T, T, T, T, T, T, T],
+    "sdpa_paged": [c_void_p, T, T, T, T, T, T, c_float, c_int32, T],
+    "graph_begin": [c_void_p],
+    "graph_end": [c_void_p, POINTER(c_void_p)],
+    "graph_launch": [c_void_p, c_void_p],
+    "graph_destroy": [c_void_p, c_void_p],
     "timer_start": [c_void_p],
     "timer_stop": [c_void_p, POINTER(c_float)],
     "launch_count": [c_void_p, POINTER(c_int64)],
@@ -361,6 +369,49 @@ class NativeBackend:
     def adamw_step(self, p, g, m, v, lr, beta1, beta2, eps, weight_decay, t, grad_scale=1.0):
         self._c("adamw_step", ctypes.byref(p), ctypes.byref(g), ctypes.byref(m), ctypes.byref(v), c_float(lr),
                 c_float(beta1), c_float(beta2), c_float(eps), c_float(weight_decay), int(t), c_float(grad_scale))
+
+    # --- paged KV cache: requests of different lengths in one step
+    def paged_plan(self, lengths, new_tokens, table, ring, state, page_size: int, rows: int) -> tuple:
+        """Pages, slots and positions of a step's new tokens: (q_start, kv_len, slots, positions, next_state). Writes the
+        pages taken into `table` and those that ended requests return into `ring`."""
+        out = [PaiTensor() for _ in range(5)]
+        self._c("paged_plan", ctypes.byref(lengths), ctypes.byref(new_tokens), ctypes.byref(table), ctypes.byref(ring),
+                ctypes.byref(state), page_size, rows, *map(ctypes.byref, out))
+        return tuple(out)
+
+    def paged_rope_append(self, q, k, v, cos_table, sin_table, positions, slots, k_cache, v_cache) -> PaiTensor:
+        """Rotates q (returned) and k at `positions` and writes k and v into `slots` of the paged caches."""
+        out = PaiTensor()
+        self._c("paged_rope_append", ctypes.byref(q), ctypes.byref(k), ctypes.byref(v), ctypes.byref(cos_table),
+                ctypes.byref(sin_table), ctypes.byref(positions), ctypes.byref(slots), ctypes.byref(k_cache),
+                ctypes.byref(v_cache), ctypes.byref(out))
+        return out
+
+    def sdpa_paged(self, q, k_cache, v_cache, table, q_start, kv_len, scale: float, max_new: int = 0) -> PaiTensor:
+        """Causal attention of each request's new tokens over its pages: [rows, H, D]."""
+        out = PaiTensor()
+        self._c("sdpa_paged", ctypes.byref(q), ctypes.byref(k_cache), ctypes.byref(v_cache), ctypes.byref(table),
+                ctypes.byref(q_start), ctypes.byref(kv_len), scale, max_new, ctypes.byref(out))
+        return out
+
+    # --- CUDA graphs (pai_graph_*) and uploads into existing tensors
+    def write(self, data, dst: PaiTensor) -> None:
+        a = np.ascontiguousarray(np.asarray(data, dtype=np.float32))
+        self._c("write", a.ctypes.data_as(POINTER(c_float)), a.size, ctypes.byref(dst))
+
+    def graph_begin(self) -> None:
+        self._c("graph_begin")
+
+    def graph_end(self) -> c_void_p:
+        g = c_void_p()
+        self._c("graph_end", ctypes.byref(g))
+        return g
+
+    def graph_launch(self, graph: c_void_p) -> None:
+        self._c("graph_launch", graph)
+
+    def graph_destroy(self, graph: c_void_p) -> None:
+        self._c("graph_destroy", graph)
 
     def timer_start(self) -> None:
         self._c("timer_start")

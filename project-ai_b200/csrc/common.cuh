@@ -45,6 +45,8 @@ struct BlockInfo {
   int scope;         // index of the owning open scope, or -1
 };
 
+constexpr int kTickets = 4096;  // counters in pai_ctx::d_tickets
+
 struct NcclState;  // defined in dp.cu
 struct IoState;    // defined in io.cu
 
@@ -76,6 +78,9 @@ struct pai_ctx {
   int64_t in_use = 0, peak = 0, reserved = 0;
   // device flag the kernels with bounded waits report into (0 = ok)
   int* d_error_flag = nullptr;
+  // arrival counters of the paged attention's split work (attention_paged.cu): zero between launches, which reset what
+  // they used; launches of one context run one after another on its stream, replayed graphs' included
+  unsigned* d_tickets = nullptr;
   pai::NcclState* nccl = nullptr;
   pai::IoState* io = nullptr;  // checkpoint streaming and the open packed dataset (io.cu)
   char name[128] = {0};

@@ -401,11 +401,15 @@ PAI_API pai_status pai_ctx_create(int device, pai_ctx** out) {
   cudaError_t e1 = cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking);
   cudaError_t e2 = cudaStreamCreateWithFlags(&c->comm_stream, cudaStreamNonBlocking);
   cudaError_t e3 = cudaMalloc(&c->d_error_flag, 64);
-  if (e1 != cudaSuccess || e2 != cudaSuccess || e3 != cudaSuccess) {
+  cudaError_t e4 = cudaMalloc(&c->d_tickets, kTickets * sizeof(unsigned));
+  if (e1 != cudaSuccess || e2 != cudaSuccess || e3 != cudaSuccess || e4 != cudaSuccess) {
     delete c;
     return set_error(PAI_ERR_CUDA, "failed to create streams for device %d", device);
   }
+  // both clears are ordered before the first kernel: the compute stream does not wait for the default stream by itself
   cudaMemset(c->d_error_flag, 0, 64);
+  cudaMemset(c->d_tickets, 0, kTickets * sizeof(unsigned));
+  cudaDeviceSynchronize();
   *out = c;
   return PAI_OK;
 }
@@ -426,6 +430,7 @@ PAI_API pai_status pai_ctx_destroy(pai_ctx* ctx) {
   for (auto& kv : ctx->graph_owner)  // blocks parked by graphs the caller did not destroy
     if (!ctx->live.count(kv.first)) cudaFree(kv.first);
   cudaFree(ctx->d_error_flag);
+  cudaFree(ctx->d_tickets);
   if (ctx->pinned) {
     cudaFreeHost(ctx->pinned);
     for (int i = 0; i < pai::kPinnedChunks; i++) cudaEventDestroy(ctx->pinned_ev[i]);

@@ -1,0 +1,53 @@
+// Device helpers shared by the paged KV cache kernels (paged.cu, attention_paged.cu).
+#pragma once
+
+#include "common.cuh"
+#include "paged_args.h"
+
+namespace pai {
+namespace paged {
+
+// An integral F32 value in [lo, hi] (hi <= 2^24, which F32 holds exactly).
+__device__ __forceinline__ bool integral(float f, int lo, int hi, int& out) {
+  if (!(f >= (float)lo && f <= (float)hi) || f != floorf(f)) return false;
+  out = (int)f;
+  return true;
+}
+
+// Division by a page size: a shift for powers of two (shift >= 0), else a plain division.
+struct PageDiv {
+  int size, shift;
+  __device__ __forceinline__ int div(int x) const { return shift >= 0 ? x >> shift : x / size; }
+};
+inline PageDiv page_div(int size) {
+  int s = 0;
+  while (s < 24 && (1 << s) < size) s++;
+  return PageDiv{size, (1 << s) == size ? s : -1};
+}
+
+// Exclusive prefix sum of one value per thread over the block, in thread order; total in every thread. `tmp` holds one
+// value per warp.
+template <int THREADS>
+__device__ __forceinline__ int64_t block_prefix(int64_t v, int64_t* tmp, int64_t& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();  // tmp may still be read from an earlier call
+  if (lane == 31) tmp[warp] = x;
+  __syncthreads();
+  int64_t before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; w++) {
+    if (w < warp) before += tmp[w];
+    total += tmp[w];
+  }
+  return before + x - v;
+}
+
+}  // namespace paged
+}  // namespace pai

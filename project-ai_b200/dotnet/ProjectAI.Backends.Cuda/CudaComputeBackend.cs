@@ -638,6 +638,67 @@ public sealed unsafe class CudaComputeBackend : IComputeBackend
         }
     }
 
+    /// <summary>Plans a step over the paged cache: which pages the new tokens take (written into table; pages of ended
+    /// requests go back to ring), their slots and positions, and the next lengths and ring state.</summary>
+    public (Tensor QStart, Tensor KvLen, Tensor Slots, Tensor Positions, Tensor NextState) PagedPlan(
+        Tensor lengths, Tensor newTokens, Tensor table, Tensor ring, Tensor state, int pageSize, int rows)
+    {
+        lock (_gate)
+        {
+            Drain();
+            var dl = Desc(lengths);
+            var dn = Desc(newTokens);
+            var dt = Desc(table);
+            var dr = Desc(ring);
+            var ds = Desc(state);
+            PaiTensor start, len, slots, positions, next;
+            Native.Check(Native.PagedPlan(Ctx, &dl, &dn, &dt, &dr, &ds, pageSize, rows, &start, &len, &slots, &positions, &next));
+            return (Wrap(start), Wrap(len), Wrap(slots), Wrap(positions), Wrap(next));
+        }
+    }
+
+    /// <summary>RoPE of q and k at their positions, then k and v written to their slots of the paged caches; returns
+    /// the rotated q.</summary>
+    public Tensor PagedRopeAppend(Tensor q, Tensor k, Tensor v, Tensor cosTable, Tensor sinTable, Tensor positions,
+                                  Tensor slots, Tensor kCache, Tensor vCache)
+    {
+        lock (_gate)
+        {
+            Drain();
+            var dq = Desc(q);
+            var dk = Desc(k);
+            var dv = Desc(v);
+            var c = Desc(cosTable);
+            var s = Desc(sinTable);
+            var p = Desc(positions);
+            var sl = Desc(slots);
+            var kc = Desc(kCache);
+            var vc = Desc(vCache);
+            PaiTensor o;
+            Native.Check(Native.PagedRopeAppend(Ctx, &dq, &dk, &dv, &c, &s, &p, &sl, &kc, &vc, &o));
+            return Wrap(o);
+        }
+    }
+
+    /// <summary>Causal attention of each request's new tokens over its pages (0 for maxNew: no bound but the rows).</summary>
+    public Tensor SdpaPaged(Tensor q, Tensor kCache, Tensor vCache, Tensor table, Tensor qStart, Tensor kvLen, float scale,
+                            int maxNew)
+    {
+        lock (_gate)
+        {
+            Drain();
+            var dq = Desc(q);
+            var kc = Desc(kCache);
+            var vc = Desc(vCache);
+            var t = Desc(table);
+            var s = Desc(qStart);
+            var l = Desc(kvLen);
+            PaiTensor o;
+            Native.Check(Native.SdpaPaged(Ctx, &dq, &kc, &vc, &t, &s, &l, scale, maxNew, &o));
+            return Wrap(o);
+        }
+    }
+
     /// <summary>RoPE, cache append and decode attention in one launch (the values of RopeAppend + SdpaDecode).</summary>
     public Tensor AttentionDecodeStep(Tensor q, Tensor k, Tensor v, Tensor cosTable, Tensor sinTable, Tensor kCache,
                                       Tensor vCache, Tensor position, float scale)

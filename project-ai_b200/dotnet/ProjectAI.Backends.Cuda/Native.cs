@@ -95,6 +95,9 @@ internal static unsafe partial class Native
     [LibraryImport(Lib, EntryPoint = "pai_rope_append")] internal static partial int RopeAppend(IntPtr ctx, PaiTensor* q, PaiTensor* k, PaiTensor* v, PaiTensor* cosTable, PaiTensor* sinTable, PaiTensor* kCache, PaiTensor* vCache, PaiTensor* pos, PaiTensor* qOut);
     [LibraryImport(Lib, EntryPoint = "pai_attn_decode_step")] internal static partial int AttnDecodeStep(IntPtr ctx, PaiTensor* q, PaiTensor* k, PaiTensor* v, PaiTensor* cosTable, PaiTensor* sinTable, PaiTensor* kCache, PaiTensor* vCache, PaiTensor* pos, float scale, PaiTensor* @out);
     [LibraryImport(Lib, EntryPoint = "pai_sdpa_decode")] internal static partial int SdpaDecode(IntPtr ctx, PaiTensor* q, PaiTensor* kCache, PaiTensor* vCache, PaiTensor* pos, float scale, PaiTensor* @out);
+    [LibraryImport(Lib, EntryPoint = "pai_paged_plan")] internal static partial int PagedPlan(IntPtr ctx, PaiTensor* lengths, PaiTensor* newTokens, PaiTensor* table, PaiTensor* ring, PaiTensor* state, int pageSize, int rows, PaiTensor* qStart, PaiTensor* kvLen, PaiTensor* slots, PaiTensor* positions, PaiTensor* nextState);
+    [LibraryImport(Lib, EntryPoint = "pai_paged_rope_append")] internal static partial int PagedRopeAppend(IntPtr ctx, PaiTensor* q, PaiTensor* k, PaiTensor* v, PaiTensor* cosTable, PaiTensor* sinTable, PaiTensor* positions, PaiTensor* slots, PaiTensor* kCache, PaiTensor* vCache, PaiTensor* qOut);
+    [LibraryImport(Lib, EntryPoint = "pai_sdpa_paged")] internal static partial int SdpaPaged(IntPtr ctx, PaiTensor* q, PaiTensor* kCache, PaiTensor* vCache, PaiTensor* table, PaiTensor* qStart, PaiTensor* kvLen, float scale, int maxNew, PaiTensor* @out);
     [LibraryImport(Lib, EntryPoint = "pai_linear_fused")] internal static partial int LinearFused(IntPtr ctx, PaiTensor* x, PaiTensor* normWeight, float eps, PaiTensor* weights, int nWeights, int mode, PaiTensor* residual, PaiTensor* @out);
     [LibraryImport(Lib, EntryPoint = "pai_graph_begin")] internal static partial int GraphBegin(IntPtr ctx);
     [LibraryImport(Lib, EntryPoint = "pai_graph_end")] internal static partial int GraphEnd(IntPtr ctx, IntPtr* graph);

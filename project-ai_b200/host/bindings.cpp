@@ -159,6 +159,11 @@ PYBIND11_MODULE(_paihost, m) {
            py::arg("residual") = nullptr, py::arg("norm_weight") = nullptr, py::arg("eps") = 0.0f)
       .def("rope_append", &NativeBackend::rope_append)
       .def("attn_decode_step", &NativeBackend::attn_decode_step)
+      .def("paged_plan", &NativeBackend::paged_plan, py::arg("lengths"), py::arg("new_tokens"), py::arg("table"),
+           py::arg("ring"), py::arg("state"), py::arg("page_size"), py::arg("rows"))
+      .def("paged_rope_append", &NativeBackend::paged_rope_append)
+      .def("sdpa_paged", &NativeBackend::sdpa_paged, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"), py::arg("table"),
+           py::arg("q_start"), py::arg("kv_len"), py::arg("scale"), py::arg("max_new") = 0)
       .def("sdpa_fwd", [](NativeBackend& be, const Tensor& q, const Tensor& k, const Tensor& v, float scale, bool causal,
                           int pos) { return be.sdpa_fwd(q, k, v, scale, causal, pos); })
       .def("sdpa_bwd", &NativeBackend::sdpa_bwd)

@@ -195,6 +195,14 @@ class NativeBackend {
                      const Tensor& k_cache, const Tensor& v_cache, const Tensor& pos);
   Tensor attn_decode_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cos_table, const Tensor& sin_table,
                           const Tensor& k_cache, const Tensor& v_cache, const Tensor& pos, float scale);
+  // paged KV cache (requests of different lengths): q_start, kv_len, slots, positions, next_state of a step; rotate and
+  // append into slots (returns the rotated q); attention of the new tokens over their requests' pages
+  std::vector<Tensor> paged_plan(const Tensor& lengths, const Tensor& new_tokens, const Tensor& table, const Tensor& ring,
+                                 const Tensor& state, int page_size, int rows);
+  Tensor paged_rope_append(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cos_table, const Tensor& sin_table,
+                           const Tensor& positions, const Tensor& slots, const Tensor& k_cache, const Tensor& v_cache);
+  Tensor sdpa_paged(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table, const Tensor& q_start,
+                    const Tensor& kv_len, float scale, int max_new);
   void graph_begin();
   pai_graph* graph_end();
   void graph_launch(pai_graph* g);

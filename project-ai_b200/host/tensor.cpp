@@ -289,6 +289,14 @@ void TensorImpl::backward(const Tensor& seed) {
   X(attn_decode_step, int (*)(pai_ctx*, const pai_tensor*, const pai_tensor*, const pai_tensor*, const pai_tensor*,      \
                               const pai_tensor*, const pai_tensor*, const pai_tensor*, const pai_tensor*, float,         \
                               pai_tensor*))                                                                              \
+  X(paged_plan, int (*)(pai_ctx*, const pai_tensor*, const pai_tensor*, const pai_tensor*, const pai_tensor*,            \
+                        const pai_tensor*, int32_t, int32_t, pai_tensor*, pai_tensor*, pai_tensor*, pai_tensor*,         \
+                        pai_tensor*))                                                                                    \
+  X(paged_rope_append, int (*)(pai_ctx*, const pai_tensor*, const pai_tensor*, const pai_tensor*, const pai_tensor*,     \
+                               const pai_tensor*, const pai_tensor*, const pai_tensor*, const pai_tensor*,               \
+                               const pai_tensor*, pai_tensor*))                                                          \
+  X(sdpa_paged, int (*)(pai_ctx*, const pai_tensor*, const pai_tensor*, const pai_tensor*, const pai_tensor*,            \
+                        const pai_tensor*, const pai_tensor*, float, int32_t, pai_tensor*))                              \
   X(graph_begin, int (*)(pai_ctx*))                                                                                      \
   X(graph_end, int (*)(pai_ctx*, pai_graph**))                                                                           \
   X(graph_launch, int (*)(pai_ctx*, pai_graph*))                                                                         \
@@ -864,6 +872,39 @@ Tensor NativeBackend::attn_decode_step(const Tensor& q, const Tensor& k, const T
   check(fn_->attn_decode_step(ctx_, &dq, &dk, &dv, &dc, &ds, &dkc, &dvc, &dp, scale, &o));
   invalidate_shadow(k_cache);
   invalidate_shadow(v_cache);
+  return wrap(o);
+}
+
+std::vector<Tensor> NativeBackend::paged_plan(const Tensor& lengths, const Tensor& new_tokens, const Tensor& table,
+                                              const Tensor& ring, const Tensor& state, int page_size, int rows) {
+  need((void*)fn_->paged_plan, "paged_plan");
+  pai_tensor dl = lengths->desc(), dn = new_tokens->desc(), dt = table->desc(), dr = ring->desc(), ds = state->desc(), o[5];
+  check(fn_->paged_plan(ctx_, &dl, &dn, &dt, &dr, &ds, page_size, rows, &o[0], &o[1], &o[2], &o[3], &o[4]));
+  invalidate_shadow(table);
+  invalidate_shadow(ring);
+  std::vector<Tensor> r;
+  for (const pai_tensor& d : o) r.push_back(wrap(d));
+  return r;
+}
+
+Tensor NativeBackend::paged_rope_append(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cos_table,
+                                        const Tensor& sin_table, const Tensor& positions, const Tensor& slots,
+                                        const Tensor& k_cache, const Tensor& v_cache) {
+  need((void*)fn_->paged_rope_append, "paged_rope_append");
+  pai_tensor dq = q->desc(), dk = k->desc(), dv = v->desc(), dc = cos_table->desc(), ds = sin_table->desc(),
+             dp = positions->desc(), dsl = slots->desc(), dkc = k_cache->desc(), dvc = v_cache->desc(), o;
+  check(fn_->paged_rope_append(ctx_, &dq, &dk, &dv, &dc, &ds, &dp, &dsl, &dkc, &dvc, &o));
+  invalidate_shadow(k_cache);
+  invalidate_shadow(v_cache);
+  return wrap(o);
+}
+
+Tensor NativeBackend::sdpa_paged(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table,
+                                 const Tensor& q_start, const Tensor& kv_len, float scale, int max_new) {
+  need((void*)fn_->sdpa_paged, "sdpa_paged");
+  pai_tensor dq = q->desc(), dk = k_cache->desc(), dv = v_cache->desc(), dt = table->desc(), ds = q_start->desc(),
+             dl = kv_len->desc(), o;
+  check(fn_->sdpa_paged(ctx_, &dq, &dk, &dv, &dt, &ds, &dl, scale, max_new, &o));
   return wrap(o);
 }
 
