@@ -10,7 +10,7 @@
 
 #include <algorithm>
 
-#include "paged.cuh"
+#include "attention_paged.cuh"
 
 namespace pai {
 namespace paged {
@@ -19,54 +19,6 @@ constexpr int kRowsThreads = 256;
 constexpr int kRowsWarps = kRowsThreads / 32;
 constexpr int kRowsPerSm = 2;  // resident blocks (registers)
 constexpr int kUnit = 64;      // keys per unit of the work split
-
-struct AttnArgs {
-  const float* q; int64_t q0, q1;          // row, head strides
-  const float* k;
-  const float* v;
-  int64_t c0, c1, c2;                      // page, head, position strides of both caches
-  const float* table; int64_t t0, t1;
-  const float* start; int64_t start_s;     // q_start [n + 1]
-  const float* len; int64_t len_s;         // kv_len [n]
-  float* out;                              // [rows, H, D]
-  int n, rows, H, KVH, g, D, max_pages, pages, max_new;
-  PageDiv page;
-  double scale2;                           // scale * log2(e): scores are kept in powers of two
-  int vec;                                 // cache rows may be read as float4
-  float* part;                             // partial results, two slots per block
-  unsigned* tickets;                       // arrivals, one counter per block (all zero between launches)
-  int* error_flag;
-};
-
-// 2^x with the library's range handling; 2^-inf = 0.
-__device__ __forceinline__ float pow2(float x) { return exp2f(x); }
-
-struct Req {
-  int first, n, len;  // first row, new tokens, keys
-};
-
-// Request i; false when its values are invalid (sets the error flag), n = 0 when it has no new token.
-__device__ __forceinline__ bool load_req(const AttnArgs& a, int i, Req& r) {
-  int end = 0;
-  r.first = r.n = r.len = 0;
-  if (!integral(a.start[i * a.start_s], 0, a.rows, r.first) || !integral(a.start[(i + 1) * a.start_s], 0, a.rows, end) ||
-      !integral(a.len[i * a.len_s], 0, a.max_pages * a.page.size, r.len) || end < r.first || end - r.first > a.max_new) {
-    return false;
-  }
-  r.n = end - r.first;
-  return true;
-}
-
-// Rows of out that belong to no request are zero.
-__device__ __forceinline__ void zero_rest(const AttnArgs& a) {
-  int lo, hi;
-  if (!integral(a.start[0], 0, a.rows, lo) || !integral(a.start[a.n * a.start_s], 0, a.rows, hi) || hi < lo) return;
-  const int per = a.H * a.D, rest = lo + (a.rows - hi);
-  for (int r = blockIdx.x; r < rest; r += gridDim.x) {
-    float* o = a.out + (int64_t)(r < lo ? r : hi + (r - lo)) * per;
-    for (int e = threadIdx.x; e < per; e += blockDim.x) o[e] = 0.0f;
-  }
-}
 
 // V values per lane, summed over the L lanes of a group: each lane is left with max(1, V / L) of the sums, value
 // index base(lane) + i. Each step halves the values a lane keeps and sends the other half to its partner.
@@ -438,27 +390,33 @@ PAI_API pai_status pai_sdpa_paged(pai_ctx* ctx, const pai_tensor* q, const pai_t
   if (numel(r) > 0) {
     auto aligned = [](const pai_tensor& t) {
       if (reinterpret_cast<uintptr_t>(fptr(t)) % 16) return false;
-      for (int i = 0; i < 3; i++)
+      for (int i = 0; i + 1 < t.rank; i++)
         if (t.dims[i] > 1 && t.strides[i] % 4) return false;
       return true;
     };
     a.vec = a.D % 4 == 0 && aligned(*k_cache) && aligned(*v_cache);
+    a.q_vec = a.D % 4 == 0 && aligned(*q);
     const int64_t most = (int64_t)a.max_new * a.g;  // rows of one kv head
+    const bool tc = most > 8 && paged::tc_fits(a);
     const int R = most <= 1 ? 1 : most <= 2 ? 2 : most <= 4 ? 4 : 8;
     // no more blocks than units there can be
     const int64_t groups = (most + R - 1) / R, tiles = std::max<int64_t>(1, ((int64_t)a.max_pages * a.page.size + 63) / 64);
     const int64_t units = std::max<int64_t>(1, (int64_t)a.n * a.KVH) * groups * tiles;
     const int grid = (int)std::min<int64_t>(std::min(ctx->sm_count * paged::kRowsPerSm, kTickets), units);
-    Scratch part;
     const int lanes = a.D <= 16 ? 4 : a.D <= 32 ? 8 : a.D <= 64 ? 16 : 32;
-    PAI_TRY(scratch(ctx, (size_t)grid * 2 * R * (4 * lanes + 2) * 4, &part));
+    Scratch part;
+    PAI_TRY(scratch(ctx, tc ? paged::tc_part_bytes(ctx) : (size_t)grid * 2 * R * (4 * lanes + 2) * 4, &part));
     a.part = static_cast<float*>(part.p);
     KernelTimerScope timer(ctx, "attn_paged", 0.0);
-    cudaError_t e = lanes == 4    ? paged::launch_rows<4>(a, R, dim3(grid), ctx->stream)
-                    : lanes == 8  ? paged::launch_rows<8>(a, R, dim3(grid), ctx->stream)
-                    : lanes == 16 ? paged::launch_rows<16>(a, R, dim3(grid), ctx->stream)
-                                  : paged::launch_rows<32>(a, R, dim3(grid), ctx->stream);
-    PAI_PDL_LAUNCH(e, "paged attention");
+    if (tc) {
+      PAI_TRY(paged::tc_launch(ctx, a));
+    } else {
+      cudaError_t e = lanes == 4    ? paged::launch_rows<4>(a, R, dim3(grid), ctx->stream)
+                      : lanes == 8  ? paged::launch_rows<8>(a, R, dim3(grid), ctx->stream)
+                      : lanes == 16 ? paged::launch_rows<16>(a, R, dim3(grid), ctx->stream)
+                                    : paged::launch_rows<32>(a, R, dim3(grid), ctx->stream);
+      PAI_PDL_LAUNCH(e, "paged attention");
+    }
   }
   *out = r;
   return PAI_OK;

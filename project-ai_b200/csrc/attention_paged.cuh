@@ -1,0 +1,66 @@
+// What the paged attention kernels share: their arguments and the reading of a request's row range and length.
+#pragma once
+
+#include <math.h>
+
+#include "paged.cuh"
+
+namespace pai {
+namespace paged {
+
+struct AttnArgs {
+  const float* q; int64_t q0, q1;          // row, head strides
+  const float* k;
+  const float* v;
+  int64_t c0, c1, c2;                      // page, head, position strides of both caches
+  const float* table; int64_t t0, t1;
+  const float* start; int64_t start_s;     // q_start [n + 1]
+  const float* len; int64_t len_s;         // kv_len [n]
+  float* out;                              // [rows, H, D]
+  int n, rows, H, KVH, g, D, max_pages, pages, max_new;
+  PageDiv page;
+  double scale2;                           // scale * log2(e): scores are kept in powers of two
+  int vec, q_vec;                          // cache rows, rows of q may be read as float4
+  float* part;                             // partial results, two slots per block
+  unsigned* tickets;                       // arrivals, one counter per block (all zero between launches)
+  int* error_flag;
+};
+
+// 2^x with the library's range handling; 2^-inf = 0.
+__device__ __forceinline__ float pow2(float x) { return exp2f(x); }
+
+struct Req {
+  int first, n, len;  // first row, new tokens, keys
+};
+
+// Request i; false when its values are invalid (sets the error flag), n = 0 when it has no new token.
+__device__ __forceinline__ bool load_req(const AttnArgs& a, int i, Req& r) {
+  int end = 0;
+  r.first = r.n = r.len = 0;
+  if (!integral(a.start[i * a.start_s], 0, a.rows, r.first) || !integral(a.start[(i + 1) * a.start_s], 0, a.rows, end) ||
+      !integral(a.len[i * a.len_s], 0, a.max_pages * a.page.size, r.len) || end < r.first || end - r.first > a.max_new) {
+    return false;
+  }
+  r.n = end - r.first;
+  return true;
+}
+
+// Rows of out that belong to no request are zero.
+__device__ __forceinline__ void zero_rest(const AttnArgs& a) {
+  int lo, hi;
+  if (!integral(a.start[0], 0, a.rows, lo) || !integral(a.start[a.n * a.start_s], 0, a.rows, hi) || hi < lo) return;
+  const int per = a.H * a.D, rest = lo + (a.rows - hi);
+  for (int r = blockIdx.x; r < rest; r += gridDim.x) {
+    float* o = a.out + (int64_t)(r < lo ? r : hi + (r - lo)) * per;
+    for (int e = threadIdx.x; e < per; e += blockDim.x) o[e] = 0.0f;
+  }
+}
+
+// The tensor-core kernel (attention_paged_tc.cu): whether it takes this call, the device memory for its partial
+// results, and its launch.
+bool tc_fits(const AttnArgs& a);
+size_t tc_part_bytes(const pai_ctx* ctx);
+pai_status tc_launch(pai_ctx* ctx, const AttnArgs& a);
+
+}  // namespace paged
+}  // namespace pai
