@@ -6,25 +6,30 @@
 // fp16 holds 2^-24 .. 65504, so operands are first scaled by powers of two (exact) that bring the largest magnitude of
 // a query row, or of a tile of 128 keys or values, to [2^13, 2^14); numbers far below that lose relative precision
 // only under 2^-39 of the largest. The scales come out again in a factor that the softmax and the sum over tiles
-// multiply by anyway. Weights are scaled by 2^14 for the same reason, in numerator and denominator alike. This is half
+// multiply by anyway. Weights exp(s - m) are taken against a reference m that follows the row maximum only when that has
+// risen by 2^9, so that sums need a rescale rarely, and carry a factor 2^6 in numerator and denominator: they stay under
+// 2^15, and their remainders lose nothing above 2^-31 of a typical largest one. This is half
 // the tensor time of three TF32 products and half the shared memory. Per tile of keys the product P·V goes to its own
-// accumulator and is added to fp32 registers with the running rescale, so the tensor cores' sums stay short (24 steps).
+// accumulator and is added to fp32 registers, so the tensor cores' sums stay short (24 steps).
 //
 // One persistent CTA per SM works on an item: 256 query rows (two tiles of 128, row = token * g + head of the group) of
 // one (request, kv head) against a run of key tiles:
-//   warps 0-3, 4-7  one softmax warpgroup per query tile, a thread per row: writes Q (split) to TMEM; per key tile takes
-//                   the row maximum of S, exponentiates, writes P (split) over S in TMEM, and adds the last P·V to its
-//                   64 registers of output while the tensor cores compute the next S;
+//   warps 0-3, 4-7  softmax of one query tile each, a thread per row: write Q (split) to TMEM; per key tile take the row
+//                   maximum of S, exponentiate, write P (split) over S in TMEM, and add the last P·V to their 64 registers
+//                   of output while the tensor cores compute the next S; the two take turns at this;
 //   warps 8-11      split K and V: read a raw fp32 tile from shared memory, write hi and lo (SWIZZLE_128B rows of 64)
 //                   over it;
 //   warp 12         copies raw K and V rows from their pages with bulk copies, up to three tiles ahead;
-//   warps 13, 14    one thread each issues S = Q·Kᵀ and P·V of one query tile; while one tile is in its softmax the
-//                   other's products run.
-// Both query tiles use each converted K and V tile, which halves conversion and shared-memory writes per product.
+//   warps 13, 14    issue S = Q·Kᵀ and P·V of one query tile each;
+//   warp 15         walks the CTA's share of the work and hands the items to the others.
+// Both query tiles use each converted K and V tile, which halves conversion and shared-memory writes per product. Up to
+// 128 rows there is one query tile: both softmax groups then work on it, each on every second key tile; the second hands
+// its result to the first through TMEM.
 //
 // Work split: as in k_paged_rows, the (item, key tile) units of all requests in one line, divided evenly over the CTAs;
 // an item that crosses CTAs leaves fp32 partial results that the last of them to finish joins in CTA order.
 // Every wait is bounded; a timeout sets the context's error flag and the CTA drains and exits.
+#include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include "attention_paged.cuh"
@@ -52,12 +57,17 @@ constexpr int kTcKeys = 128;                 // keys of one tile
 constexpr int kTcDim = 64;                   // padded head dim
 constexpr int kTcStages = 3;                 // K and V tiles in shared memory
 constexpr int kTcRing = 8;                   // scales of the last tiles (more than the tiles in flight between two readers)
-constexpr int kTcThreads = 512;              // four warpgroups; the last warp is idle
-constexpr int kConvWarp = 8, kLoadWarp = 12, kIssueWarp = 13;
-// Registers per thread of the softmax, conversion and loading/issuing warpgroups: 2·168 + 104 + 64 = 504 of the
-// 4·128 = 512 that the CTA is launched with.
-constexpr int kSoftmaxRegs = 168, kConvRegs = 104, kMiscRegs = 64;
-static_assert(2 * kSoftmaxRegs + kConvRegs + kMiscRegs <= 4 * 128, "more registers than the launch holds");
+constexpr int kSoftmaxWarps = 4;             // per query tile
+constexpr int kConvWarps = 4;
+constexpr int kConvWarp = 2 * kSoftmaxWarps, kLoadWarp = kConvWarp + kConvWarps, kIssueWarp = kLoadWarp + 1;
+constexpr int kWalkWarp = kIssueWarp + 2;
+constexpr int kTcThreads = 32 * (kWalkWarp + 1);  // four warpgroups
+constexpr int kItems = 4;                         // items handed out ahead
+// Registers per thread of the softmax, conversion and loading/issuing warpgroups: 2·176 + 96 + 64 = 512, what the CTA is
+// launched with (4·128).
+constexpr int kLaunchRegs = 128, kSoftmaxRegs = 176, kConvRegs = 96, kMiscRegs = 64;
+static_assert(2 * kSoftmaxRegs + kConvRegs + kMiscRegs <= 4 * kLaunchRegs, "more registers than the launch holds");
+static_assert(kTcThreads == 4 * 128 && kTcThreads * kLaunchRegs <= 65536, "one CTA's registers");
 constexpr uint32_t kHalfTile = kTcKeys * 128;      // hi or lo: 128 rows of 64 fp16
 constexpr uint32_t kTile = 2 * kHalfTile;          // 32 KB, the size of the raw fp32 tile as well
 constexpr int kTcPart = 2 * kTcRows * (kTcDim + 2);  // floats of one partial result
@@ -66,16 +76,28 @@ __host__ __device__ constexpr uint32_t col_s(int t) { return 128u * (uint32_t)t;
 __host__ __device__ constexpr uint32_t col_pv(int t) { return 256u + 64u * (uint32_t)t; }
 __host__ __device__ constexpr uint32_t col_q(int t) { return 384u + 64u * (uint32_t)t; }
 
+// One run of key tiles [t0, t1) of 256 query rows of a (request, kv head).
+struct Item {
+  int req, first, shift, len;  // first row of the request, position of its first new token, keys
+  int kvh, row0, rows;         // first query row of the item, query rows of the kv head
+  int t0, t1, end[2];          // key tiles, and where they end for each query tile (causality; t0 if it has no rows)
+  int split;                   // one query tile, whose key tiles the two softmax groups share out
+  int whole, c0, c1;           // 1 if these are all key tiles of the rows; the CTAs that share them
+  int stop;                    // no further item
+};
+
 struct TcShared {
   uint64_t raw[2][kTcStages];    // [K, V]: the raw tile has landed
   uint64_t conv[2][kTcStages];   // it is split
   uint64_t empty[2][kTcStages];  // both query tiles' products have read it
-  uint64_t s_full[2], p_full[2], pv_full[2], q_full[2], done[2], drained[2];  // per query tile
+  uint64_t s_full[2], pv_full[2], drained[2];  // per query tile
+  uint64_t item_full[kItems], item_free[kItems];
+  Item items[kItems];
   int64_t tmp[kTcThreads / 32];
-  int64_t off, total;
-  uint32_t seen[kTcRing][4];     // keys of a tile that exist (bit per key)
-  uint32_t max_bits[2][4];       // converter warps' largest magnitudes
-  uint32_t odd[2][4];            // ... and whether a value is not finite
+  int64_t off;
+  alignas(16) uint32_t seen[kTcRing][4];  // keys of a tile that exist (bit per key)
+  alignas(16) uint32_t max_bits[2][kConvWarps];  // converter warps' largest magnitudes; top bit: one is not finite
+  float join_m[kTcRows], join_l[kTcRows];        // split items: the second group's maxima and sums
   float scale[2][kTcRing];       // what a product with the tile is multiplied by to undo the tile's scale
   int v_odd[kTcRing];            // a V tile held values that are not finite
   int req;
@@ -90,40 +112,80 @@ __host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool b_mn) {
   return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
-// D (TMEM) (+)= A (TMEM, two fp16 per column) · B (shared)
-__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// D (TMEM) (+)= A (TMEM, two fp16 per column) · B (shared), issued by the lane whose `leader` is set. The whole warp runs
+// the surrounding code, so addresses and descriptors stay in uniform registers (from a branch of one lane each product
+// took about 100 cycles to issue).
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t leader) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc));
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(leader));
+}
+__device__ __forceinline__ void commit_if(uint64_t* bar, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+      "r"(leader)
+      : "memory");
 }
 
-// Bounded wait that also gives up once another role of the CTA has.
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, const volatile int* abort) {
+// 32 TMEM columns of this warp's lanes into registers, without waiting; tmem_ready() waits for every load so far and
+// hands the registers on.
+__device__ __forceinline__ void tmem_get(uint32_t addr, float (&x)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7]), "=f"(x[8]),
+        "=f"(x[9]), "=f"(x[10]), "=f"(x[11]), "=f"(x[12]), "=f"(x[13]), "=f"(x[14]), "=f"(x[15]), "=f"(x[16]),
+        "=f"(x[17]), "=f"(x[18]), "=f"(x[19]), "=f"(x[20]), "=f"(x[21]), "=f"(x[22]), "=f"(x[23]), "=f"(x[24]),
+        "=f"(x[25]), "=f"(x[26]), "=f"(x[27]), "=f"(x[28]), "=f"(x[29]), "=f"(x[30]), "=f"(x[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_ready(float (&x)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(x[0]), "+f"(x[1]), "+f"(x[2]), "+f"(x[3]), "+f"(x[4]), "+f"(x[5]), "+f"(x[6]), "+f"(x[7]),
+                 "+f"(x[8]), "+f"(x[9]), "+f"(x[10]), "+f"(x[11]), "+f"(x[12]), "+f"(x[13]), "+f"(x[14]), "+f"(x[15]),
+                 "+f"(x[16]), "+f"(x[17]), "+f"(x[18]), "+f"(x[19]), "+f"(x[20]), "+f"(x[21]), "+f"(x[22]),
+                 "+f"(x[23]), "+f"(x[24]), "+f"(x[25]), "+f"(x[26]), "+f"(x[27]), "+f"(x[28]), "+f"(x[29]),
+                 "+f"(x[30]), "+f"(x[31])
+               :
+               : "memory");
+}
+
+// Bounded wait that also gives up once another role of the CTA has (abort may be null). Each try suspends the thread up
+// to kSuspendNs or until the phase completes: without the hint a try returned at once so often that the waiting warps'
+// polls were half of all instructions issued.
+constexpr uint32_t kSuspendNs = 20000, kTries = 1u << 18;
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort) {
   const uint32_t addr = smem_u32(bar);
-  for (uint32_t i = 0; i < tc::kWaitLimit; i++) {
+  for (uint32_t i = 0; i < kTries; i++) {
     uint32_t done;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(done)
-        : "r"(addr), "r"(parity)
+        : "r"(addr), "r"(parity), "r"(kSuspendNs)
         : "memory");
     if (done) return true;
-    if ((i & 255u) == 255u && *abort) return false;
+    if (abort && *abort) return false;
   }
+  if (abort) *abort = 1;
   return false;
 }
-// Lane 0 polls, the warp follows its result.
-__device__ __forceinline__ bool warp_wait_bar(uint64_t* bar, uint32_t parity, const volatile int* abort) {
-  int ok = 0;
-  if ((threadIdx.x & 31) == 0) ok = wait_bar(bar, parity, abort) ? 1 : 0;
-  return __shfl_sync(0xffffffffu, ok, 0) != 0;
+// The whole warp polls (a poll by one lane and a shuffle take twice the 150 cycles of this).
+__device__ __forceinline__ bool warp_wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  const bool ok = wait_bar(bar, parity, abort);
+  return __all_sync(0xffffffffu, ok);
 }
 __device__ __forceinline__ void bar_named(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ void bar_signal(int id, int threads) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
 // The power of two that brings a magnitude (bits of a finite fp32, sign cleared) to [2^13, 2^14), and its inverse.
@@ -137,11 +199,11 @@ __device__ __forceinline__ bool finite_bits(uint32_t bits) { return bits < 0x7f8
 
 __device__ __forceinline__ uint32_t pack2(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 // Two fp32 numbers as fp16 hi parts and fp16 remainders (first number in the low half).
-__device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
-  const __half2 h = __floats2half2_rn(x0, x1);
+__device__ __forceinline__ void split2(float2 x, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __float22half2_rn(x);
   const float2 f = __half22float2(h);
   hi = pack2(h);
-  lo = pack2(__floats2half2_rn(x0 - f.x, x1 - f.y));
+  lo = pack2(__float22half2_rn(__ffma2_rn(f, make_float2(-1.0f, -1.0f), x)));
 }
 
 // A request's units: per kv head, groups of 256 rows, each with the key tiles that its last row attends.
@@ -163,21 +225,17 @@ __device__ __forceinline__ Shape shape_of(const AttnArgs& a, const Req& r) {
   return s;
 }
 
-// One run of key tiles [t0, t1) of a row group; `tiles` are all of the group's.
-struct Item {
-  Req r;
-  int req, kvh, row0, rows, t0, t1, tiles;
-  int64_t unit;  // of tile 0, in the line of all units
-};
-
-// Walks the CTA's share of the units; every role walks it alike.
-struct Walk {
-  int req;
-  int64_t off, u, u1;
-  __device__ __forceinline__ bool next(const AttnArgs& a, Item& it) {
+// Hands out the CTA's share of the units, [u, u1) from unit `off` of request `req` on, as items.
+__device__ __forceinline__ void walk_role(const AttnArgs& a, TcShared& sh, int req, int64_t off, int64_t u, int64_t u1,
+                                          int64_t total) {
+  const int64_t G = min((int64_t)gridDim.x, total);
+  for (int i = 0;; i++) {
+    Item it{};
+    it.stop = 1;
     while (u < u1) {
-      load_req(a, req, it.r);
-      const Shape s = shape_of(a, it.r);
+      Req r;
+      load_req(a, req, r);
+      const Shape s = shape_of(a, r);
       if (off >= s.units * a.KVH) {
         req++;
         off = 0;
@@ -185,256 +243,367 @@ struct Walk {
       }
       it.kvh = (int)(off / s.units);
       int64_t rest = off - it.kvh * s.units;
-      int group = 0;
+      int group = 0, tiles;
       for (;; group++) {
-        it.tiles = group_tiles(a, it.r, s.rows, group);
-        if (rest < it.tiles) break;
-        rest -= it.tiles;
+        tiles = group_tiles(a, r, s.rows, group);
+        if (rest < tiles) break;
+        rest -= tiles;
       }
       it.req = req;
+      it.first = r.first;
+      it.shift = r.len - r.n;
+      it.len = r.len;
       it.row0 = group * 2 * kTcRows;
       it.rows = s.rows;
       it.t0 = (int)rest;
-      it.t1 = (int)min((int64_t)it.tiles, rest + (u1 - u));
-      it.unit = u - rest;
+      it.t1 = (int)min((int64_t)tiles, rest + (u1 - u));
+      it.whole = it.t0 == 0 && it.t1 == tiles;
+      it.c0 = (int)(((u - rest + 1) * G - 1) / total);
+      it.c1 = (int)(((u - rest + tiles) * G - 1) / total);
+      for (int t = 0; t < 2; t++) {
+        const int row0 = it.row0 + t * kTcRows, last = min(s.rows, row0 + kTcRows) - 1;
+        const int keys = it.shift + last / a.g + 1;  // that the tile's last row attends
+        it.end[t] = row0 < s.rows ? max(it.t0, min(it.t1, (keys + kTcKeys - 1) / kTcKeys)) : it.t0;
+      }
+      it.split = it.row0 + kTcRows >= s.rows && it.end[0] - it.t0 >= 2;
+      if (it.split) it.end[1] = it.end[0];
+      it.stop = 0;
       u += it.t1 - it.t0;
       off += it.t1 - it.t0;
-      return true;
+      break;
     }
-    return false;
+    const int slot = i % kItems;
+    if (!wait_bar(&sh.item_free[slot], ((i / kItems) & 1) ^ 1, &sh.abort)) {
+      atomicExch(a.error_flag, 80);
+      sh.abort = 1;
+      return;
+    }
+    sh.items[slot] = it;
+    mbar_arrive(&sh.item_full[slot]);
+    if (it.stop) return;
   }
-};
+}
 
-// Key tiles of the item that query tile t (its first row `row0`) attends: [t0, result).
-__device__ __forceinline__ int tile_end(const AttnArgs& a, const Item& it, int row0) {
-  const int last = min(it.rows, row0 + kTcRows) - 1;
-  const int keys = it.r.len - it.r.n + last / a.g + 1;
-  return max(it.t0, min(it.t1, (keys + kTcKeys - 1) / kTcKeys));
+// Item i for a whole warp (all of it copied, so the slot is free again); false when there is none. Waits the whole time
+// limit whether another role gave up or not: the warps that meet at named barriers must all see an item or none.
+__device__ __forceinline__ bool take_item(TcShared& sh, int i, Item& it) {
+  const int slot = i % kItems;
+  it.stop = 0;
+  if (!warp_wait_bar(&sh.item_full[slot], (i / kItems) & 1, nullptr)) return false;
+  it = sh.items[slot];
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.item_free[slot]);
+  return it.stop == 0;
 }
 
 // ---------------------------------------------------------------- roles
-// Softmax warpgroup of query tile `tile`.
-template <int tile>
-__device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, Walk walk, uint32_t tmem) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = warp & 3;
+// Softmax of query tile `tile`.
+__device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, uint32_t tmem) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = warp & 3, tile = warp >> 2;
   const int row = quad * 32 + lane;
   const uint32_t base = tmem + ((uint32_t)(quad * 32) << 16);
   const uint32_t cs = base + col_s(tile), cpv = base + col_pv(tile), cq = base + col_q(tile);
-  const int64_t G = min((int64_t)gridDim.x, sh.total);
   bool ok = true;
   int J = 0, C = 0;  // key tiles of the CTA and of this query tile so far
   Item it;
-  while (walk.next(a, it)) {
-    const int first = it.row0 + tile * kTcRows;
+  for (int i = 0; take_item(sh, i, it); i++) {
+    const int first = it.row0 + (it.split ? 0 : tile * kTcRows);
     if (first >= it.rows) {
       J += it.t1 - it.t0;
+      continue;
+    }
+    const int step = it.split ? 2 : 1, t0 = it.t0 + (it.split ? tile : 0);
+    const int end = t0 + (max(0, (tile == 0 ? it.end[0] : it.end[1]) - t0) + step - 1) / step * step;
+    const int warps = min(4, (it.rows - first + 31) >> 5);  // of this group that have rows
+    // The groups take turns at the softmax, so that each runs beside the other's products: the x-th of the first group,
+    // the x-th of the second, the x+1-th of the first, as far as the two have key tiles. Left alone they fall into step,
+    // wait for the tensor cores together and then compute together.
+    const int first1 = it.row0 + (it.split ? 0 : kTcRows), both = 32 * (min(4, (it.rows - it.row0 + 31) >> 5) + max(0, min(4, (it.rows - first1 + 31) >> 5)));
+    const int other = first1 >= it.rows ? 0 : it.split ? (it.end[0] - it.t0 + (tile ^ 1 ? 0 : 1)) >> 1 : (tile ? it.end[0] : it.end[1]) - it.t0;
+    if (quad >= warps) {
+      // None of this warp's rows exists. What is left in its rows of TMEM goes into no other row.
+      J += it.t1 - it.t0;
+      C += (end - t0) / step;
+      bar_named(7 + tile, 128 + 32);
+      if (it.split) {
+        bar_named(4, 256);
+        bar_named(4, 256);
+      }
+      if (!it.whole && !(it.split && tile == 1)) {
+        bar_named(2 + tile, 128);
+        bar_named(2 + tile, 128);
+      }
       continue;
     }
     const int r = first + row;
     const bool live = r < it.rows;
     const int s = r / a.g, h = it.kvh * a.g + (r - s * a.g);
-    const int limit = live ? it.r.len - it.r.n + s : -1;  // the last key this row attends
-    const int first_limit = it.r.len - it.r.n + first / a.g;
-    const int end = tile_end(a, it, first);
+    const int limit = live ? it.shift + s : -1;  // the last key this row attends
+    const int first_limit = it.shift + first / a.g;
     float qdown;  // undoes the row's scale
     {
-      float x[64];
-      uint32_t big = 0;
-      const float* p = a.q + (int64_t)(it.r.first + s) * a.q0 + (int64_t)h * a.q1;
-      if (a.q_vec) {
+      const float* p = a.q + (int64_t)(it.first + s) * a.q0 + (int64_t)h * a.q1;
+      auto get = [&](int d) {  // four elements, as scores in powers of two want them; rounded once from 64 bits
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (live && d < a.D) {
+          if (a.q_vec) {
+            const float4 f = *reinterpret_cast<const float4*>(p + d);
+            v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+          } else {
 #pragma unroll
-        for (int d = 0; d < 64; d += 4) {
-          const float4 v = live && d < a.D ? *reinterpret_cast<const float4*>(p + d) : make_float4(0.f, 0.f, 0.f, 0.f);
-          x[d] = v.x; x[d + 1] = v.y; x[d + 2] = v.z; x[d + 3] = v.w;
+            for (int e = 0; e < 4; e++) v[e] = p[d + e];  // the head dim is a multiple of 4
+          }
         }
-      } else {
+        return make_float4((float)((double)v[0] * a.scale2), (float)((double)v[1] * a.scale2),
+                           (float)((double)v[2] * a.scale2), (float)((double)v[3] * a.scale2));
+      };
+      uint32_t big = 0;
+#pragma unroll 4
+      for (int d = 0; d < 64; d += 4) {
+        const float4 f = get(d);
+        const float v[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
-        for (int d = 0; d < 64; d++) x[d] = live && d < a.D ? p[d] : 0.0f;
-      }
-#pragma unroll
-      for (int d = 0; d < 64; d++) {
-        x[d] = (float)((double)x[d] * a.scale2);  // scores in powers of two; rounded once from 64 bits
-        const uint32_t b = __float_as_uint(x[d]) & 0x7fffffffu;
-        if (finite_bits(b)) big = max(big, b);
+        for (int e = 0; e < 4; e++) {
+          const uint32_t b = __float_as_uint(v[e]) & 0x7fffffffu;
+          if (finite_bits(b)) big = max(big, b);
+        }
       }
       float up;
       tile_scale(big, up, qdown);
-      float lo[32];
+#pragma unroll 1
+      for (int c = 0; c < 4; c++) {  // 16 elements: 8 columns of hi, 8 of lo
+        float hi[8], lo[8];
 #pragma unroll
-      for (int d = 0; d < 32; d++) {
-        uint32_t hi, l;
-        split2(x[2 * d] * up, x[2 * d + 1] * up, hi, l);
-        x[d] = __uint_as_float(hi);
-        lo[d] = __uint_as_float(l);
-      }
-      if (ok) {
-        tmem_st32(cq, x);
-        tmem_st32(cq + 32, lo);
-        tmem_st_wait();
-        fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.q_full[tile]);
-      }
-    }
-    float o[64];
-#pragma unroll
-    for (int d = 0; d < 64; d++) o[d] = 0.0f;
-    float m = -INFINITY, l = 0.0f, alpha = 1.0f;
-    int odd = 0;
-    auto fold = [&](int slot) {  // o = o * alpha + (P·V of the last tile)
-      const float f = sh.scale[1][slot];
-      odd |= sh.v_odd[slot];
-#pragma unroll
-      for (int c = 0; c < 2; c++) {
-        float pv[32];
-        tmem_ld32(cpv + 32 * c, pv);
-#pragma unroll
-        for (int d = 0; d < 32; d++) o[32 * c + d] = fmaf(pv[d], f, o[32 * c + d] * alpha);
-      }
-    };
-    for (int t = it.t0; t < end; t++) {
-      const int slot = (J + t - it.t0) % kTcRing;
-      if (t > it.t0) {
-        if (ok && !warp_wait_bar(&sh.pv_full[tile], (C - 1) & 1, &sh.abort)) ok = false;
-        if (ok) {
-          fence_after();
-          fold((slot + kTcRing - 1) % kTcRing);
+        for (int d = 0; d < 4; d++) {
+          const float4 f = get(16 * c + 4 * d);
+          uint32_t h0, l0, h1, l1;
+          split2(make_float2(f.x * up, f.y * up), h0, l0);
+          split2(make_float2(f.z * up, f.w * up), h1, l1);
+          hi[2 * d] = __uint_as_float(h0); hi[2 * d + 1] = __uint_as_float(h1);
+          lo[2 * d] = __uint_as_float(l0); lo[2 * d + 1] = __uint_as_float(l1);
         }
+        tc::tmem_st8(cq + 8 * c, hi);
+        tc::tmem_st8(cq + 32 + 8 * c, lo);
       }
+      tmem_st_wait();
+      fence_before();
+      bar_signal(5 + tile, 32 * warps + 32);  // to the issuing warp
+    }
+    float2 o[32];
+#pragma unroll
+    for (int d = 0; d < 32; d++) o[d] = make_float2(0.0f, 0.0f);
+    float m = -INFINITY, l = 0.0f;  // reference and sum of the weights
+    int odd = 0;
+    float x[32], y[32];
+    // After a timed-out wait `ok` stays false: no further TMEM or barrier-object work, but the named barriers are met.
+#pragma unroll 1
+    for (int t = t0; t < end; t += step) {
+      const int j = J + t - it.t0, slot = j % kTcRing, turn = (t - t0) / step;
       if (ok && !warp_wait_bar(&sh.s_full[tile], C & 1, &sh.abort)) ok = false;
-      if (!ok) break;
+      if (tile == 0 ? turn > 0 && turn <= other : turn < other) bar_named(9 + tile, both);
       fence_after();
       // kept finite and above 0: a score of 0 or -inf times it stays one
       const float c = fminf(fmaxf(qdown * sh.scale[0][slot], 1.1754944e-38f), 3.4028235e38f);
       const int k0 = t * kTcKeys;
-      uint32_t vis[4];
-      bool masked = k0 + kTcKeys - 1 > first_limit;
+      const uint4 seen = *reinterpret_cast<const uint4*>(sh.seen[slot]);
+      if (k0 + kTcKeys - 1 > first_limit || (seen.x & seen.y & seen.z & seen.w) != 0xffffffffu) {
+        // scores of keys that do not exist or that the row does not attend become -inf in place
+#pragma unroll 1
+        for (int g = 0; g < 4; g++) {
+          const int n = limit - (k0 + 32 * g) + 1;
+          const uint32_t vis = sh.seen[slot][g] & (n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u);
+          tmem_get(cs + 32 * g, x);
+          tmem_ready(x);
 #pragma unroll
-      for (int g = 0; g < 4; g++) {
-        const int n = limit - (k0 + 32 * g) + 1;  // keys of the chunk up to the row's last
-        const uint32_t upto = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
-        vis[g] = sh.seen[slot][g];
-        masked = masked || vis[g] != 0xffffffffu;
-        vis[g] &= upto;
-      }
-      float mx = -INFINITY;
-#pragma unroll
-      for (int g = 0; g < 4; g++) {
-        float x[32];
-        tmem_ld32(cs + 32 * g, x);
-        if (masked) {
-#pragma unroll
-          for (int i = 0; i < 32; i++) mx = fmaxf(mx, (vis[g] >> i) & 1u ? x[i] : -INFINITY);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; i++) mx = fmaxf(mx, x[i]);
+          for (int e = 0; e < 32; e++) x[e] = (vis >> e) & 1u ? x[e] : -INFINITY;
+          tmem_st32(cs + 32 * g, x);
         }
+        tmem_st_wait();
       }
-      const float mn = fmaxf(m, mx * c);
-      alpha = mn == m ? 1.0f : ex2_sfu(m - mn);
-      const float ref = (mn == -INFINITY ? 0.0f : mn) - 14.0f;
-      m = mn;
-      float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      auto largest = [&](const float (&v)[32]) {
 #pragma unroll
-      for (int g = 0; g < 4; g++) {
-        float x[32], y[32];
-        tmem_ld32(cs + 32 * g, x);
-        if (masked) {
+        for (int e = 0; e < 32; e += 8)
 #pragma unroll
-          for (int i = 0; i < 32; i++) x[i] = (vis[g] >> i) & 1u ? x[i] : -INFINITY;
-        }
+          for (int k = 0; k < 4; k++) mx[k] = fmaxf(mx[k], fmaxf(v[e + 2 * k], v[e + 2 * k + 1]));
+      };
+      tmem_get(cs, x);
+      tmem_ready(x);
+      tmem_get(cs + 32, y);
+      largest(x);
+      tmem_ready(y);
+      tmem_get(cs + 64, x);
+      largest(y);
+      tmem_ready(x);
+      tmem_get(cs + 96, y);
+      largest(x);
+      tmem_ready(y);
+      tmem_get(cs, x);  // for the exponentials
+      largest(y);
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
+      const bool rise = top > m + 9.0f;  // also from -inf; never on NaN
+      const float old = m;
+      if (rise) m = top;
+      const float ref = 6.0f - (m == -INFINITY ? 0.0f : m);
+      const float2 c2 = make_float2(c, c), ref2 = make_float2(ref, ref);
+      float2 sum0 = make_float2(0.0f, 0.0f), sum1 = sum0;
+      // 32 scores to weights, over the scores: keys 16 e .. of the tile as 8 columns of hi, 8 of lo
+      auto weights = [&](float (&v)[32], uint32_t col) {
+        float w[32];
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-          const float p0 = ex2_sfu(fmaf(x[2 * i], c, -ref)), p1 = ex2_sfu(fmaf(x[2 * i + 1], c, -ref));
-          part[(2 * i) & 3] += p0;
-          part[(2 * i + 1) & 3] += p1;
+        for (int e = 0; e < 16; e++) {
+          float2 p = __ffma2_rn(make_float2(v[2 * e], v[2 * e + 1]), c2, ref2);
+          p.x = ex2_sfu(p.x);
+          p.y = ex2_sfu(p.y);
+          if (e & 1) sum1 = __fadd2_rn(sum1, p);
+          else sum0 = __fadd2_rn(sum0, p);
           uint32_t hi, lo;
-          split2(p0, p1, hi, lo);
-          y[i] = __uint_as_float(hi);
-          y[16 + i] = __uint_as_float(lo);
+          split2(p, hi, lo);
+          w[16 * (e >> 3) + (e & 7)] = __uint_as_float(hi);
+          w[16 * (e >> 3) + 8 + (e & 7)] = __uint_as_float(lo);
         }
-        tmem_st32(cs + 32 * g, y);  // over the scores just read: keys 32g.. as 16 columns of hi, 16 of lo
+        tmem_st32(col, w);
+      };
+      tmem_ready(x);
+#pragma unroll 1
+      for (int g = 0; g < 4; g += 2) {
+        tmem_get(cs + 32 * g + 32, y);
+        weights(x, cs + 32 * g);
+        tmem_ready(y);
+        if (g == 0) tmem_get(cs + 64, x);
+        weights(y, cs + 32 * g + 32);
+        if (g == 0) tmem_ready(x);
       }
-      l = l * alpha + ((part[0] + part[1]) + (part[2] + part[3]));
       tmem_st_wait();
       fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.p_full[tile]);
+      bar_signal(5 + tile, 32 * warps + 32);
+      if (tile == 0 ? turn < other : turn + 1 < other) bar_signal(10 - tile, both);
+      const float sum = (sum0.x + sum0.y) + (sum1.x + sum1.y);
+      if (__any_sync(0xffffffffu, rise)) {
+        const float alpha = rise ? ex2_sfu(old - m) : 1.0f;
+        const float2 al = make_float2(alpha, alpha);
+        l = l * alpha + sum;
+#pragma unroll
+        for (int d = 0; d < 32; d++) o[d] = __fmul2_rn(o[d], al);
+      } else {
+        l += sum;
+      }
+      if (ok && !warp_wait_bar(&sh.pv_full[tile], C & 1, &sh.abort)) ok = false;
       C++;
-    }
-    if (end > it.t0) {
-      if (ok && !warp_wait_bar(&sh.pv_full[tile], (C - 1) & 1, &sh.abort)) ok = false;
-      if (ok) {
-        fence_after();
-        fold((J + end - 1 - it.t0) % kTcRing);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.done[tile]);
+      fence_after();
+      tmem_get(cpv, x);
+      tmem_get(cpv + 32, y);
+      const float2 f = make_float2(sh.scale[1][slot], sh.scale[1][slot]);
+      odd |= sh.v_odd[slot];
+      tmem_ready(x);
+      tmem_ready(y);
+#pragma unroll
+      for (int d = 0; d < 16; d++) {
+        o[d] = __ffma2_rn(make_float2(x[2 * d], x[2 * d + 1]), f, o[d]);
+        o[16 + d] = __ffma2_rn(make_float2(y[2 * d], y[2 * d + 1]), f, o[16 + d]);
       }
     }
+    // Every warp has read the last scales before the issuing warp frees tiles that the ring's slots are reused for, and
+    // none of this group, those without rows included, gets ahead to the next item's barriers.
+    bar_named(7 + tile, 128 + 32);
     if (odd) {
       // Values that are not finite were left out of the products: add those that this row attends.
       const int k1 = min(it.t1 * kTcKeys, limit + 1);
       for (int j = it.t0 * kTcKeys; j < k1; j++) {
+        if (it.split && ((j / kTcKeys - it.t0) & 1) != tile) continue;
         const int pi = a.page.div(j);
         int page;
         if (!integral(a.table[it.req * a.t0 + pi * a.t1], 0, a.pages - 1, page)) continue;
         const float* v = a.v + (int64_t)page * a.c0 + (int64_t)it.kvh * a.c1 + (int64_t)(j - pi * a.page.size) * a.c2;
 #pragma unroll
-        for (int d = 0; d < 64; d++)
-          if (d < a.D && !finite_bits(__float_as_uint(v[d]) & 0x7fffffffu)) o[d] += v[d];
+        for (int d = 0; d < 32; d++) {
+          if (2 * d >= a.D) break;
+          const float2 f = *reinterpret_cast<const float2*>(v + 2 * d);
+          if (!finite_bits(__float_as_uint(f.x) & 0x7fffffffu)) o[d].x += f.x;
+          if (!finite_bits(__float_as_uint(f.y) & 0x7fffffffu)) o[d].y += f.y;
+        }
       }
     }
     J += it.t1 - it.t0;
-    const bool whole = it.t0 == 0 && it.t1 == it.tiles;
-    float* out = a.out + ((int64_t)(it.r.first + s) * a.H + h) * a.D;
-    auto store = [&](float sum) {
-      const float inv = 1.0f / sum;
-#pragma unroll
-      for (int d = 0; d < 64; d += 4) {
-        if (d < a.D) {
-          const float4 v = make_float4(o[d] * inv, o[d + 1] * inv, o[d + 2] * inv, o[d + 3] * inv);
-          *reinterpret_cast<float4*>(out + d) = sum == 0.0f ? make_float4(0.f, 0.f, 0.f, 0.f) : v;
-        }
+    if (it.split) {
+      // The second group's result goes to the first through the second's P·V columns (free until its next P).
+      if (tile == 1 && ok) {
+        tmem_st32(cpv, reinterpret_cast<const float*>(o));
+        tmem_st32(cpv + 32, reinterpret_cast<const float*>(o + 16));
+        tmem_st_wait();
+        fence_before();
+        sh.join_m[row] = m;
+        sh.join_l[row] = l;
       }
-    };
-    if (whole) {
-      if (ok && live) store(l);
-      continue;
-    }
-    const int c0 = (int)(((it.unit + 1) * G - 1) / sh.total), c1 = (int)(((it.unit + it.tiles) * G - 1) / sh.total);
-    auto slot_of = [&](int b) { return a.part + (size_t)(2 * b + (b == c0 ? 1 : 0)) * kTcPart; };
-    float* mine = slot_of(blockIdx.x) + (size_t)(tile * kTcRows + row) * (kTcDim + 2);
+      bar_named(4, 256);
+      if (tile == 0 && ok) {
+        fence_after();
+        const float m1 = sh.join_m[row], mn = fmaxf(m, m1);
+        const float f0 = mn == m ? 1.0f : ex2_sfu(m - mn), f1 = mn == m1 ? 1.0f : ex2_sfu(m1 - mn);
+        m = mn;
+        l = l * f0 + sh.join_l[row] * f1;
+        tmem_get(base + col_pv(1), x);
+        tmem_get(base + col_pv(1) + 32, y);
+        tmem_ready(x);
+        tmem_ready(y);
+        const float2 g0 = make_float2(f0, f0), g1 = make_float2(f1, f1);
 #pragma unroll
-    for (int d = 0; d < 64; d += 2) *reinterpret_cast<float2*>(mine + d) = make_float2(o[d], o[d + 1]);
-    *reinterpret_cast<float2*>(mine + 64) = make_float2(m, l);
-    __threadfence();
-    bar_named(2 + tile, 128);
-    if (row == 0) {
-      unsigned* ticket = &a.tickets[2 * c0 + tile];
-      sh.last[tile] = atomicAdd(ticket, 1u) == (unsigned)(c1 - c0);
-      if (sh.last[tile]) *ticket = 0;
+        for (int d = 0; d < 16; d++) {
+          o[d] = __ffma2_rn(make_float2(x[2 * d], x[2 * d + 1]), g1, __fmul2_rn(o[d], g0));
+          o[16 + d] = __ffma2_rn(make_float2(y[2 * d], y[2 * d + 1]), g1, __fmul2_rn(o[16 + d], g0));
+        }
+        fence_before();
+      }
+      bar_named(4, 256);
+      if (tile == 1) continue;
     }
-    bar_named(2 + tile, 128);
-    if (sh.last[tile]) {
+    bool write = it.whole != 0;
+    if (!write) {
+      const int c0 = it.c0, c1 = it.c1;
+      auto part_of = [&](int b) {
+        return a.part + (size_t)(2 * b + (b == c0 ? 1 : 0)) * kTcPart + (size_t)(tile * kTcRows + row) * (kTcDim + 2);
+      };
+      float* mine = part_of(blockIdx.x);
+#pragma unroll
+      for (int d = 0; d < 32; d++) *reinterpret_cast<float2*>(mine + 2 * d) = o[d];
+      *reinterpret_cast<float2*>(mine + 64) = make_float2(m, l);
       __threadfence();
-      float M = -INFINITY, L = 0.0f;
-      for (int b = c0; b <= c1; b++)
-        M = fmaxf(M, __ldcg(slot_of(b) + (size_t)(tile * kTcRows + row) * (kTcDim + 2) + 64));
+      bar_named(2 + tile, 128);
+      if (row == 0) {
+        unsigned* ticket = &a.tickets[2 * c0 + tile];
+        sh.last[tile] = atomicAdd(ticket, 1u) == (unsigned)(c1 - c0);
+        if (sh.last[tile]) *ticket = 0;
+      }
+      bar_named(2 + tile, 128);
+      write = sh.last[tile] != 0;
+      if (write) {
+        __threadfence();
+        float M = -INFINITY;
+        for (int b = c0; b <= c1; b++) M = fmaxf(M, __ldcg(part_of(b) + 64));
+        l = 0.0f;
 #pragma unroll
-      for (int d = 0; d < 64; d++) o[d] = 0.0f;
-      for (int b = c0; b <= c1; b++) {
-        const float* p = slot_of(b) + (size_t)(tile * kTcRows + row) * (kTcDim + 2);
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(p + 64));
-        const float f = M == -INFINITY ? 1.0f : ex2_sfu(ml.x - M);
-        L += ml.y * f;
+        for (int d = 0; d < 32; d++) o[d] = make_float2(0.0f, 0.0f);
+#pragma unroll 1
+        for (int b = c0; b <= c1; b++) {
+          const float* p = part_of(b);
+          const float2 ml = __ldcg(reinterpret_cast<const float2*>(p + 64));
+          const float f = M == -INFINITY ? 1.0f : ex2_sfu(ml.x - M);
+          l += ml.y * f;
 #pragma unroll
-        for (int d = 0; d < 64; d += 2) {
-          const float2 v = __ldcg(reinterpret_cast<const float2*>(p + d));
-          o[d] += v.x * f;
-          o[d + 1] += v.y * f;
+          for (int d = 0; d < 32; d++)
+            o[d] = __ffma2_rn(__ldcg(reinterpret_cast<const float2*>(p + 2 * d)), make_float2(f, f), o[d]);
         }
       }
-      if (ok && live) store(L);
+    }
+    if (write && ok && live) {
+      float* out = a.out + ((int64_t)(it.first + s) * a.H + h) * a.D;
+      const float inv = 1.0f / l;
+#pragma unroll
+      for (int d = 0; d < 16; d++)
+        if (4 * d < a.D)
+          *reinterpret_cast<float4*>(out + 4 * d) =
+              l == 0.0f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                        : make_float4(o[2 * d].x * inv, o[2 * d].y * inv, o[2 * d + 1].x * inv, o[2 * d + 1].y * inv);
     }
   }
   if (!ok && lane == 0) {
@@ -444,89 +613,102 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, Wa
 }
 
 // Splits the raw K and V tiles in place.
-__device__ __forceinline__ void convert_role(const AttnArgs& a, TcShared& sh, uint8_t* tiles, Walk walk) {
+__device__ __forceinline__ void convert_role(const AttnArgs& a, TcShared& sh, uint8_t* tiles) {
   const int tid = threadIdx.x - 32 * kConvWarp, warp = tid >> 5, lane = tid & 31;
   const int tr = tid >> 4, tc4 = tid & 15;  // 16 threads per row, 8 rows per pass
+  uint8_t* dst0 = tiles + tr * 128 + (((tc4 >> 1) ^ tr) << 4) + ((tc4 & 1) << 3);
   bool ok = true;
   int J = 0;
   Item it;
-  while (walk.next(a, it)) {
-    for (int t = it.t0; t < it.t1; t++, J++) {
-      const int st = J % kTcStages, slot = J % kTcRing;
-      for (int op = 0; op < 2; op++) {
-        uint8_t* tile = tiles + (op * kTcStages + st) * kTile;
-        float4 x[16];
-        uint32_t big = 0;
-        bool odd = false;
-        if (ok && !warp_wait_bar(&sh.raw[op][st], (J / kTcStages) & 1, &sh.abort)) ok = false;
-        if (ok) {
-          const float* raw = reinterpret_cast<const float*>(tile);
+  for (int i = 0; take_item(sh, i, it); i++) {
+#pragma unroll 1
+    for (int k = 2 * it.t0; k < 2 * it.t1; k++) {
+      const int op = k & 1, st = J % kTcStages, slot = J % kTcRing;
+      const uint32_t at = (uint32_t)(op * kTcStages + st) * kTile;
+      float4 x[16];
+      __nv_bfloat162 big2 = __floats2bfloat162_rn(0.0f, 0.0f);
+      uint32_t big = 0;
+      bool odd = false;
+      if (ok && !warp_wait_bar(&sh.raw[op][st], (J / kTcStages) & 1, &sh.abort)) ok = false;
+      if (ok) {
+        const float* raw = reinterpret_cast<const float*>(tiles + at) + tr * a.D + 4 * tc4;
+        const uint4 seen = *reinterpret_cast<const uint4*>(sh.seen[slot]);
+        if (a.D == kTcDim && (seen.x & seen.y & seen.z & seen.w) == 0xffffffffu) {
+#pragma unroll
+          for (int p = 0; p < 16; p++) x[p] = *reinterpret_cast<const float4*>(raw + p * 8 * kTcDim);
+        } else {
+          const uint32_t bits[4] = {seen.x, seen.y, seen.z, seen.w};
 #pragma unroll
           for (int p = 0; p < 16; p++) {
-            const int r = p * 8 + tr;
-            const bool have = ((sh.seen[slot][p >> 2] >> (r & 31)) & 1u) && 4 * tc4 < a.D;
-            x[p] = have ? *reinterpret_cast<const float4*>(raw + r * a.D + 4 * tc4) : make_float4(0.f, 0.f, 0.f, 0.f);
+            const bool have = ((bits[p >> 2] >> ((p * 8 + tr) & 31)) & 1u) && 4 * tc4 < a.D;
+            x[p] = have ? *reinterpret_cast<const float4*>(raw + p * 8 * a.D) : make_float4(0.f, 0.f, 0.f, 0.f);
           }
+        }
+        // the largest magnitude, in bf16 (only its exponent counts)
+#pragma unroll
+        for (int p = 0; p < 16; p++) {
+          big2 = __hmax2_nan(big2, __habs2(__floats2bfloat162_rn(x[p].x, x[p].y)));
+          big2 = __hmax2_nan(big2, __habs2(__floats2bfloat162_rn(x[p].z, x[p].w)));
+        }
+        const uint32_t b2 = *reinterpret_cast<const uint32_t*>(&big2);
+        big = max(b2 << 16, b2 & 0xffff0000u);
+        odd = !finite_bits(big);
+        if (odd) {  // the largest finite magnitude
+          big = 0;
 #pragma unroll
           for (int p = 0; p < 16; p++) {
             const float v[4] = {x[p].x, x[p].y, x[p].z, x[p].w};
 #pragma unroll
             for (int e = 0; e < 4; e++) {
               const uint32_t b = __float_as_uint(v[e]) & 0x7fffffffu;
-              big = max(big, b);
-            }
-          }
-          odd = !finite_bits(big);
-          if (odd) {  // the largest finite magnitude
-            big = 0;
-#pragma unroll
-            for (int p = 0; p < 16; p++) {
-              const float v[4] = {x[p].x, x[p].y, x[p].z, x[p].w};
-#pragma unroll
-              for (int e = 0; e < 4; e++) {
-                const uint32_t b = __float_as_uint(v[e]) & 0x7fffffffu;
-                if (finite_bits(b)) big = max(big, b);
-              }
+              if (finite_bits(b)) big = max(big, b);
             }
           }
         }
-        big = __reduce_max_sync(0xffffffffu, big);
-        odd = __any_sync(0xffffffffu, odd);
-        if (lane == 0) {
-          sh.max_bits[op][warp] = big;
-          sh.odd[op][warp] = odd;
+      }
+      big = __reduce_max_sync(0xffffffffu, big);
+      odd = __any_sync(0xffffffffu, odd);
+      if (lane == 0) sh.max_bits[op][warp] = big | (odd ? 0x80000000u : 0u);
+      bar_named(1, 32 * kConvWarps);  // the maxima are there, and every thread holds its part of the raw tile
+      if (ok) {
+        uint32_t any = 0;
+        big = 0;
+#pragma unroll
+        for (int w = 0; w < kConvWarps; w++) {
+          any |= sh.max_bits[op][w];
+          big = max(big, sh.max_bits[op][w] & 0x7fffffffu);
         }
-        bar_named(1, 128);  // the maxima are there, and every thread holds its part of the raw tile
-        if (!ok) continue;
-        big = max(max(sh.max_bits[op][0], sh.max_bits[op][1]), max(sh.max_bits[op][2], sh.max_bits[op][3]));
-        odd = (sh.odd[op][0] | sh.odd[op][1] | sh.odd[op][2] | sh.odd[op][3]) != 0;
+        odd = (any >> 31) != 0;
         float up, down;
         tile_scale(big, up, down);
         if (tid == 0) {
           sh.scale[op][slot] = down;
           if (op == 1) sh.v_odd[slot] = odd;
         }
+        if (odd && op == 1) {  // a value that is not finite would spoil the rows that do not attend it, too
+#pragma unroll
+          for (int p = 0; p < 16; p++) {
+            if (!isfinite(x[p].x)) x[p].x = 0.0f;
+            if (!isfinite(x[p].y)) x[p].y = 0.0f;
+            if (!isfinite(x[p].z)) x[p].z = 0.0f;
+            if (!isfinite(x[p].w)) x[p].w = 0.0f;
+          }
+        }
+        const float2 up2 = make_float2(up, up);
+        uint8_t* dst = dst0 + at;
 #pragma unroll
         for (int p = 0; p < 16; p++) {
-          const int r = p * 8 + tr;
-          float4 y = make_float4(x[p].x * up, x[p].y * up, x[p].z * up, x[p].w * up);
-          if (odd && op == 1) {  // a value that is not finite would spoil the rows that do not attend it, too
-            if (!isfinite(y.x)) y.x = 0.0f;
-            if (!isfinite(y.y)) y.y = 0.0f;
-            if (!isfinite(y.z)) y.z = 0.0f;
-            if (!isfinite(y.w)) y.w = 0.0f;
-          }
           uint2 hi, lo;
-          split2(y.x, y.y, hi.x, lo.x);
-          split2(y.z, y.w, hi.y, lo.y);
-          uint8_t* dst = tile + r * 128 + (((tc4 >> 1) ^ (r & 7)) << 4) + ((tc4 & 1) << 3);
-          *reinterpret_cast<uint2*>(dst) = hi;
-          *reinterpret_cast<uint2*>(dst + kHalfTile) = lo;
+          split2(__fmul2_rn(make_float2(x[p].x, x[p].y), up2), hi.x, lo.x);
+          split2(__fmul2_rn(make_float2(x[p].z, x[p].w), up2), hi.y, lo.y);
+          *reinterpret_cast<uint2*>(dst + p * 1024) = hi;
+          *reinterpret_cast<uint2*>(dst + p * 1024 + kHalfTile) = lo;
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.conv[op][st]);
       }
+      if (op) J++;
     }
   }
   if (!ok && lane == 0) {
@@ -536,20 +718,20 @@ __device__ __forceinline__ void convert_role(const AttnArgs& a, TcShared& sh, ui
 }
 
 // Copies the raw K and V tiles out of their pages.
-__device__ __forceinline__ void load_role(const AttnArgs& a, TcShared& sh, uint8_t* tiles, Walk walk) {
+__device__ __forceinline__ void load_role(const AttnArgs& a, TcShared& sh, uint8_t* tiles) {
   const int lane = threadIdx.x & 31;
   const int P = a.page.size;
   const uint32_t row_bytes = (uint32_t)a.D * 4;
   bool ok = true, bad = false, copied_k = false;
   int J = 0;
   Item it;
-  while (ok && walk.next(a, it)) {
+  for (int i = 0; ok && take_item(sh, i, it); i++) {
     const float* trow = a.table + (int64_t)it.req * a.t0;
     const int64_t head = (int64_t)it.kvh * a.c1;
     for (int t = it.t0; t < it.t1; t++) {
       const int st = J % kTcStages, slot = J % kTcRing;
       const uint32_t parity = ((J / kTcStages) & 1) ^ 1;
-      const int k0 = t * kTcKeys, k1 = min(k0 + kTcKeys, it.r.len);
+      const int k0 = t * kTcKeys, k1 = min(k0 + kTcKeys, it.len);
       const int p0 = a.page.div(k0), p1 = k1 > k0 ? a.page.div(k1 - 1) : p0 - 1;
       uint32_t seen[4] = {0, 0, 0, 0};
       int count = 0;
@@ -625,74 +807,84 @@ __device__ __forceinline__ void load_role(const AttnArgs& a, TcShared& sh, uint8
   }
 }
 
-// Issues the products of one query tile.
-__device__ __forceinline__ void issue_role(const AttnArgs& a, TcShared& sh, uint8_t* tiles, Walk walk, uint32_t tmem, int tile) {
+// Issues the products of query tile `tile`; the whole warp runs this. The named barriers that the softmax warps wait at are
+// met whatever fails, so `ok` only stops the work between them.
+__device__ __forceinline__ void issue_role(const AttnArgs& a, TcShared& sh, uint8_t* tiles, uint32_t tmem, int tile) {
   constexpr uint32_t is = idesc_f16(kTcRows, kTcKeys, false), ip = idesc_f16(kTcRows, kTcDim, true);
+  const int lane = threadIdx.x & 31;
+  const uint32_t leader = lane == 0, k_tiles = smem_u32(tiles), v_tiles = k_tiles + kTcStages * kTile;
   const uint32_t cs = tmem + col_s(tile), cpv = tmem + col_pv(tile), cq = tmem + col_q(tile);
-  const uint32_t k_tiles = smem_u32(tiles), v_tiles = k_tiles + kTcStages * kTile;
   bool ok = true;
-  int J = 0, C = 0, items = 0, dones = 0;
+  int J = 0, C = 0;
   Item it;
-  auto skip = [&](int op, int j) {  // a tile this query tile does not use: free it once it is converted
-    const int st = j % kTcStages;
-    if (!wait_bar(&sh.conv[op][st], (j / kTcStages) & 1, &sh.abort)) return false;
-    mbar_arrive(&sh.empty[op][st]);
-    return true;
+  auto wait_split = [&](int op, int j) {
+    return warp_wait_bar(&sh.conv[op][j % kTcStages], (j / kTcStages) & 1, &sh.abort);
   };
-  while (ok && walk.next(a, it)) {
-    const int first = it.row0 + tile * kTcRows;
-    const bool active = first < it.rows;
-    const int end = active ? tile_end(a, it, first) : it.t0;
-    if (active) {
-      if (!wait_bar(&sh.q_full[tile], items & 1, &sh.abort)) { ok = false; break; }
-      items++;
-    }
-    for (int t = it.t0; t < end; t++, J++) {
-      const int st = J % kTcStages;
-      const uint32_t parity = (J / kTcStages) & 1;
-      if (!wait_bar(&sh.conv[0][st], parity, &sh.abort) ||
-          (C > 0 && !wait_bar(&sh.pv_full[tile], (C - 1) & 1, &sh.abort))) {  // the last P has been read: S may replace it
-        ok = false;
-        break;
+  // the CTA's key tiles [j, end) that this query tile does not use: its share of freeing them, once they are split
+  auto skip = [&](int j, int end) {
+    for (; ok && j < end; j++)
+      for (int op = 0; op < 2 && ok; op++) {
+        ok = wait_split(op, j);
+        if (ok && lane == 0) mbar_arrive(&sh.empty[op][j % kTcStages]);
       }
-      fence_after();
-      const uint32_t kh = k_tiles + st * kTile, kl = kh + kHalfTile;
-#pragma unroll
-      for (int i = 0; i < 4; i++) mma_f16_ts(cs, cq + 32 + 8 * i, desc_sw128(kh + 32 * i), is, i > 0);
-#pragma unroll
-      for (int i = 0; i < 4; i++) mma_f16_ts(cs, cq + 8 * i, desc_sw128(kl + 32 * i), is, 1u);
-#pragma unroll
-      for (int i = 0; i < 4; i++) mma_f16_ts(cs, cq + 8 * i, desc_sw128(kh + 32 * i), is, 1u);
-      commit(&sh.s_full[tile]);
-      commit(&sh.empty[0][st]);
-      if (!wait_bar(&sh.p_full[tile], C & 1, &sh.abort) || !wait_bar(&sh.conv[1][st], parity, &sh.abort)) {
-        ok = false;
-        break;
-      }
-      fence_after();
-      const uint32_t vh = v_tiles + st * kTile, vl = vh + kHalfTile;
-      // 16 keys per product: columns 32 (i / 2) + 8 (i % 2) of P's hi part, 16 further of its lo part
-#pragma unroll
-      for (int i = 0; i < 8; i++) mma_f16_ts(cpv, cs + 32 * (i >> 1) + 8 * (i & 1) + 16, desc_sw128(vh + 2048 * i), ip, i > 0);
-#pragma unroll
-      for (int i = 0; i < 8; i++) mma_f16_ts(cpv, cs + 32 * (i >> 1) + 8 * (i & 1), desc_sw128(vl + 2048 * i), ip, 1u);
-#pragma unroll
-      for (int i = 0; i < 8; i++) mma_f16_ts(cpv, cs + 32 * (i >> 1) + 8 * (i & 1), desc_sw128(vh + 2048 * i), ip, 1u);
-      commit(&sh.pv_full[tile]);
-      commit(&sh.empty[1][st]);
-      C++;
+  };
+  for (int i = 0; take_item(sh, i, it); i++) {
+    const int first = it.row0 + (it.split ? 0 : tile * kTcRows), next = J + it.t1 - it.t0;
+    if (first >= it.rows) {
+      skip(J, next);
+      J = next;
+      continue;
     }
-    // The softmax has read the last scales before this thread frees tiles that the ring's slots are reused for.
-    if (ok && end > it.t0 && !wait_bar(&sh.done[tile], dones++ & 1, &sh.abort)) ok = false;
-    for (int t = end; t < it.t1 && ok; t++, J++) ok = skip(0, J) && skip(1, J);
+    const int step = it.split ? 2 : 1, t0 = it.t0 + (it.split ? tile : 0);
+    const int end = t0 + (max(0, (tile == 0 ? it.end[0] : it.end[1]) - t0) + step - 1) / step * step;
+    const int threads = 32 * min(4, (it.rows - first + 31) >> 5) + 32;
+    bar_named(5 + tile, threads);  // Q is in TMEM
+#pragma unroll 1
+    for (int t = t0; t < end; t += step, C++) {
+      const int j = J + t - it.t0, st = j % kTcStages;
+      // K is split, and the last P has been read
+      ok = ok && wait_split(0, j) && (C == 0 || warp_wait_bar(&sh.pv_full[tile], (C - 1) & 1, &sh.abort));
+      if (ok) {
+        fence_after();
+        const uint32_t kh = k_tiles + st * kTile, kl = kh + kHalfTile;
+#pragma unroll
+        for (int e = 0; e < 4; e++) mma_f16_ts(cs, cq + 32 + 8 * e, desc_sw128(kh + 32 * e), is, e > 0, leader);
+#pragma unroll
+        for (int e = 0; e < 4; e++) mma_f16_ts(cs, cq + 8 * e, desc_sw128(kl + 32 * e), is, 1u, leader);
+#pragma unroll
+        for (int e = 0; e < 4; e++) mma_f16_ts(cs, cq + 8 * e, desc_sw128(kh + 32 * e), is, 1u, leader);
+        commit_if(&sh.s_full[tile], leader);
+        commit_if(&sh.empty[0][st], leader);
+        if (it.split) commit_if(&sh.empty[0][st], leader);  // the other query tile's share as well
+        ok = wait_split(1, j);
+      }
+      bar_named(5 + tile, threads);  // P is in TMEM
+      if (ok) {
+        fence_after();
+        const uint32_t vh = v_tiles + st * kTile, vl = vh + kHalfTile;
+        // 16 keys per product: columns 16 e of P's hi part, 8 further of its lo part
+#pragma unroll
+        for (int e = 0; e < 8; e++) mma_f16_ts(cpv, cs + 16 * e + 8, desc_sw128(vh + 2048 * e), ip, e > 0, leader);
+#pragma unroll
+        for (int e = 0; e < 8; e++) mma_f16_ts(cpv, cs + 16 * e, desc_sw128(vl + 2048 * e), ip, 1u, leader);
+#pragma unroll
+        for (int e = 0; e < 8; e++) mma_f16_ts(cpv, cs + 16 * e, desc_sw128(vh + 2048 * e), ip, 1u, leader);
+        commit_if(&sh.pv_full[tile], leader);
+        commit_if(&sh.empty[1][st], leader);
+        if (it.split) commit_if(&sh.empty[1][st], leader);
+      }
+    }
+    bar_named(7 + tile, 128 + 32);
+    if (!it.split) skip(J + end - it.t0, next);
+    J = next;
   }
-  if (!ok) {
+  if (!ok && lane == 0) {
     atomicExch(a.error_flag, 79);
     sh.abort = 1;
   }
-  // every product this thread issued completes before the CTA gives its tensor memory back
-  commit(&sh.drained[tile]);
-  tc::mbar_wait(&sh.drained[tile], 0);
+  // every product issued completes before the CTA gives its tensor memory back
+  commit_if(&sh.drained[tile], leader);
+  tc::warp_wait(&sh.drained[tile], 0);
 }
 
 __global__ void __launch_bounds__(kTcThreads, 1) k_paged_tc(const AttnArgs a) {
@@ -704,15 +896,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_tc(const AttnArgs a) {
     for (int op = 0; op < 2; op++)
       for (int i = 0; i < kTcStages; i++) {
         mbar_init(&sh.raw[op][i], 1);
-        mbar_init(&sh.conv[op][i], 4);
+        mbar_init(&sh.conv[op][i], kConvWarps);
         mbar_init(&sh.empty[op][i], 2);
       }
+    for (int i = 0; i < kItems; i++) {
+      mbar_init(&sh.item_full[i], 1);
+      mbar_init(&sh.item_free[i], kWalkWarp);  // every warp before the walking one takes each item
+    }
     for (int t = 0; t < 2; t++) {
       mbar_init(&sh.s_full[t], 1);
-      mbar_init(&sh.p_full[t], 4);
       mbar_init(&sh.pv_full[t], 1);
-      mbar_init(&sh.q_full[t], 4);
-      mbar_init(&sh.done[t], 4);
       mbar_init(&sh.drained[t], 1);
     }
     sh.abort = 0;
@@ -734,24 +927,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_tc(const AttnArgs a) {
   }
   const int64_t before = block_prefix<kTcThreads>(mine, sh.tmp, total);
   const int64_t G = min((int64_t)gridDim.x, total), c = blockIdx.x;
-  Walk walk{0, 0, 0, 0};
-  if (c < G) {
-    walk.u = c * total / G;
-    walk.u1 = (c + 1) * total / G;
-    if (before <= walk.u && walk.u < before + mine) {
-      int64_t off = walk.u - before;
-      for (int i = i0; i < i1; i++) {
-        Req r;
-        load_req(a, i, r);
-        const int64_t units = shape_of(a, r).units * a.KVH;
-        if (off < units) {
-          sh.req = i;
-          sh.off = off;
-          sh.total = total;
-          break;
-        }
-        off -= units;
+  const int64_t u0 = c * total / max(G, (int64_t)1), u1 = (c + 1) * total / max(G, (int64_t)1);
+  if (c < G && before <= u0 && u0 < before + mine) {
+    int64_t off = u0 - before;
+    for (int i = i0; i < i1; i++) {
+      Req r;
+      load_req(a, i, r);
+      const int64_t units = shape_of(a, r).units * a.KVH;
+      if (off < units) {
+        sh.req = i;
+        sh.off = off;
+        break;
       }
+      off -= units;
     }
   }
   fence_before();
@@ -759,19 +947,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_tc(const AttnArgs a) {
   fence_after();
   const uint32_t tmem = sh.tmem;
   if (c < G) {
-    walk.req = sh.req;
-    walk.off = sh.off;
     if (warp < kConvWarp) {
       asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-      if (warp < 4) softmax_role<0>(a, sh, walk, tmem);
-      else softmax_role<1>(a, sh, walk, tmem);
+      softmax_role(a, sh, tmem);
     } else if (warp < kLoadWarp) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvRegs));
-      convert_role(a, sh, tiles, walk);
+      convert_role(a, sh, tiles);
     } else {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMiscRegs));
-      if (warp == kLoadWarp) load_role(a, sh, tiles, walk);
-      else if (warp < kIssueWarp + 2 && lane == 0) issue_role(a, sh, tiles, walk, tmem, warp - kIssueWarp);
+      if (warp == kLoadWarp) load_role(a, sh, tiles);
+      else if (warp < kWalkWarp) issue_role(a, sh, tiles, tmem, warp - kIssueWarp);
+      else if (lane == 0) walk_role(a, sh, sh.req, sh.off, u0, u1, total);
     }
   }
   fence_before();
