@@ -50,8 +50,10 @@ __device__ __forceinline__ void zero_rest(const AttnArgs& a) {
   int lo, hi;
   if (!integral(a.start[0], 0, a.rows, lo) || !integral(a.start[a.n * a.start_s], 0, a.rows, hi) || hi < lo) return;
   const int per = a.H * a.D, rest = lo + (a.rows - hi);
+#pragma unroll 1
   for (int r = blockIdx.x; r < rest; r += gridDim.x) {
     float* o = a.out + (int64_t)(r < lo ? r : hi + (r - lo)) * per;
+#pragma unroll 1
     for (int e = threadIdx.x; e < per; e += blockDim.x) o[e] = 0.0f;
   }
 }

@@ -14,14 +14,16 @@
 //
 // One persistent CTA per SM works on an item: 256 query rows (two tiles of 128, row = token * g + head of the group) of
 // one (request, kv head) against a run of key tiles:
-//   warps 0-3, 4-7  softmax of one query tile each, a thread per row: write Q (split) to TMEM; per key tile take the row
-//                   maximum of S, exponentiate, write P (split) over S in TMEM, and add the last P·V to their 64 registers
-//                   of output while the tensor cores compute the next S; the two take turns at this;
-//   warps 8-11      split K and V: read a raw fp32 tile from shared memory, write hi and lo (SWIZZLE_128B rows of 64)
+//   warps 0-7, 8-15 softmax of one query tile each, two threads per row (each half of the keys and half of the head
+//                   dims): write Q (split) to TMEM; per key tile take the row maximum of S, exponentiate, write P (split)
+//                   over S in TMEM, and add the last P·V to their 32 registers of output while the tensor cores compute
+//                   the next S. The two groups take turns at this. (One thread per row left each scheduler one warp at
+//                   this work, 336 cycles per 16 keys, most of it latency; two take 160 each, what the pipes need.)
+//   warps 16-23     split K and V: read a raw fp32 tile from shared memory, write hi and lo (SWIZZLE_128B rows of 64)
 //                   over it;
-//   warp 12         copies raw K and V rows from their pages with bulk copies, up to three tiles ahead;
-//   warps 13, 14    issue S = Q·Kᵀ and P·V of one query tile each;
-//   warp 15         walks the CTA's share of the work and hands the items to the others.
+//   warp 24         copies raw K and V rows from their pages with bulk copies, up to three tiles ahead;
+//   warps 25, 26    issue S = Q·Kᵀ and P·V of one query tile each;
+//   warp 27         walks the CTA's share of the work and hands the items to the others.
 // Both query tiles use each converted K and V tile, which halves conversion and shared-memory writes per product. Up to
 // 128 rows there is one query tile: both softmax groups then work on it, each on every second key tile; the second hands
 // its result to the first through TMEM.
@@ -57,17 +59,24 @@ constexpr int kTcKeys = 128;                 // keys of one tile
 constexpr int kTcDim = 64;                   // padded head dim
 constexpr int kTcStages = 3;                 // K and V tiles in shared memory
 constexpr int kTcRing = 8;                   // scales of the last tiles (more than the tiles in flight between two readers)
-constexpr int kSoftmaxWarps = 4;             // per query tile
-constexpr int kConvWarps = 4;
+constexpr int kSoftmaxWarps = 8;             // per query tile
+constexpr int kConvWarps = 8;
 constexpr int kConvWarp = 2 * kSoftmaxWarps, kLoadWarp = kConvWarp + kConvWarps, kIssueWarp = kLoadWarp + 1;
 constexpr int kWalkWarp = kIssueWarp + 2;
-constexpr int kTcThreads = 32 * (kWalkWarp + 1);  // four warpgroups
+constexpr int kTcThreads = 32 * (kWalkWarp + 1);  // seven warpgroups
 constexpr int kItems = 4;                         // items handed out ahead
-// Registers per thread of the softmax, conversion and loading/issuing warpgroups: 2·176 + 96 + 64 = 512, what the CTA is
-// launched with (4·128).
-constexpr int kLaunchRegs = 128, kSoftmaxRegs = 176, kConvRegs = 96, kMiscRegs = 64;
-static_assert(2 * kSoftmaxRegs + kConvRegs + kMiscRegs <= 4 * kLaunchRegs, "more registers than the launch holds");
-static_assert(kTcThreads == 4 * 128 && kTcThreads * kLaunchRegs <= 65536, "one CTA's registers");
+// Registers per thread of the softmax, conversion and loading/issuing warpgroups: 4·88 + 2·56 + 40 = 504, what the CTA is
+// launched with (7·72).
+constexpr int kLaunchRegs = 72, kSoftmaxRegs = 88, kConvRegs = 56, kMiscRegs = 40;
+static_assert(4 * kSoftmaxRegs + 2 * kConvRegs + kMiscRegs <= 7 * kLaunchRegs, "more registers than the launch holds");
+static_assert(kTcThreads == 7 * 128 && kTcThreads * kLaunchRegs <= 65536, "one CTA's registers");
+// Named barriers (0 is __syncthreads)
+constexpr int kBarConv = 1;    // conversion warps
+constexpr int kBarIssue = 2;   // + query tile: softmax warps with rows arrive, the issuing warp waits (Q or P is in TMEM)
+constexpr int kBarTurn = 12;   // + query tile: a group waits for its turn, the other arrives
+constexpr int kBarJoin = 4;    // both groups, at the end of split items
+constexpr int kBarEnd = 5;     // + query tile: end of an item
+constexpr int kBarPair = 8;    // + 2 query tile + quadrant / 2: the warps that share rows, of two quadrants
 constexpr uint32_t kHalfTile = kTcKeys * 128;      // hi or lo: 128 rows of 64 fp16
 constexpr uint32_t kTile = 2 * kHalfTile;          // 32 KB, the size of the raw fp32 tile as well
 constexpr int kTcPart = 2 * kTcRows * (kTcDim + 2);  // floats of one partial result
@@ -96,6 +105,7 @@ struct TcShared {
   int64_t tmp[kTcThreads / 32];
   int64_t off;
   alignas(16) uint32_t seen[kTcRing][4];  // keys of a tile that exist (bit per key)
+  float row_x[2][2][kTcRows];    // [query tile][half]: what the two threads of a row exchange
   alignas(16) uint32_t max_bits[2][kConvWarps];  // converter warps' largest magnitudes; top bit: one is not finite
   float join_m[kTcRows], join_l[kTcRows];        // split items: the second group's maxima and sums
   float scale[2][kTcRing];       // what a product with the tile is multiplied by to undo the tile's scale
@@ -132,35 +142,13 @@ __device__ __forceinline__ void commit_if(uint64_t* bar, uint32_t leader) {
       : "memory");
 }
 
-// 32 TMEM columns of this warp's lanes into registers, without waiting; tmem_ready() waits for every load so far and
-// hands the registers on.
-__device__ __forceinline__ void tmem_get(uint32_t addr, float (&x)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7]), "=f"(x[8]),
-        "=f"(x[9]), "=f"(x[10]), "=f"(x[11]), "=f"(x[12]), "=f"(x[13]), "=f"(x[14]), "=f"(x[15]), "=f"(x[16]),
-        "=f"(x[17]), "=f"(x[18]), "=f"(x[19]), "=f"(x[20]), "=f"(x[21]), "=f"(x[22]), "=f"(x[23]), "=f"(x[24]),
-        "=f"(x[25]), "=f"(x[26]), "=f"(x[27]), "=f"(x[28]), "=f"(x[29]), "=f"(x[30]), "=f"(x[31])
-      : "r"(addr));
-}
-__device__ __forceinline__ void tmem_ready(float (&x)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+f"(x[0]), "+f"(x[1]), "+f"(x[2]), "+f"(x[3]), "+f"(x[4]), "+f"(x[5]), "+f"(x[6]), "+f"(x[7]),
-                 "+f"(x[8]), "+f"(x[9]), "+f"(x[10]), "+f"(x[11]), "+f"(x[12]), "+f"(x[13]), "+f"(x[14]), "+f"(x[15]),
-                 "+f"(x[16]), "+f"(x[17]), "+f"(x[18]), "+f"(x[19]), "+f"(x[20]), "+f"(x[21]), "+f"(x[22]),
-                 "+f"(x[23]), "+f"(x[24]), "+f"(x[25]), "+f"(x[26]), "+f"(x[27]), "+f"(x[28]), "+f"(x[29]),
-                 "+f"(x[30]), "+f"(x[31])
-               :
-               : "memory");
-}
-
 // Bounded wait that also gives up once another role of the CTA has (abort may be null). Each try suspends the thread up
 // to kSuspendNs or until the phase completes: without the hint a try returned at once so often that the waiting warps'
 // polls were half of all instructions issued.
 constexpr uint32_t kSuspendNs = 20000, kTries = 1u << 18;
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort) {
   const uint32_t addr = smem_u32(bar);
+#pragma unroll 1
   for (uint32_t i = 0; i < kTries; i++) {
     uint32_t done;
     asm volatile(
@@ -181,10 +169,27 @@ __device__ __forceinline__ bool warp_wait_bar(uint64_t* bar, uint32_t parity, vo
   const bool ok = wait_bar(bar, parity, abort);
   return __all_sync(0xffffffffu, ok);
 }
+// Named barriers. A warp meets them as a whole, whatever branch one of its lanes has just taken.
 __device__ __forceinline__ void bar_named(int id, int threads) {
+  __syncwarp();
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
+// ... and whether any of the threads says so.
+__device__ __forceinline__ bool bar_any(int id, int threads, bool mine) {
+  uint32_t r;
+  __syncwarp();
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %3, 0;\n\t"
+      "bar.red.or.pred q, %1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"(threads), "r"((uint32_t)mine)
+      : "memory");
+  return r != 0;
+}
 __device__ __forceinline__ void bar_signal(int id, int threads) {
+  __syncwarp();
   asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
@@ -221,6 +226,7 @@ __device__ __forceinline__ Shape shape_of(const AttnArgs& a, const Req& r) {
   s.rows = r.n * a.g;
   s.groups = (s.rows + 2 * kTcRows - 1) / (2 * kTcRows);
   s.units = 0;
+#pragma unroll 1
   for (int i = 0; i < s.groups; i++) s.units += group_tiles(a, r, s.rows, i);
   return s;
 }
@@ -232,6 +238,7 @@ __device__ __forceinline__ void walk_role(const AttnArgs& a, TcShared& sh, int r
   for (int i = 0;; i++) {
     Item it{};
     it.stop = 1;
+#pragma unroll 1
     while (u < u1) {
       Req r;
       load_req(a, req, r);
@@ -244,6 +251,7 @@ __device__ __forceinline__ void walk_role(const AttnArgs& a, TcShared& sh, int r
       it.kvh = (int)(off / s.units);
       int64_t rest = off - it.kvh * s.units;
       int group = 0, tiles;
+#pragma unroll 1
       for (;; group++) {
         tiles = group_tiles(a, r, s.rows, group);
         if (rest < tiles) break;
@@ -297,14 +305,24 @@ __device__ __forceinline__ bool take_item(TcShared& sh, int i, Item& it) {
 }
 
 // ---------------------------------------------------------------- roles
-// Softmax of query tile `tile`.
+// Softmax of query tile `tile`. After a timed-out wait `ok` stays false: no further TMEM or barrier-object work, but the
+// named barriers are met.
 __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, uint32_t tmem) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = warp & 3, tile = warp >> 2;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = warp & 3, tile = warp >> 3, half = (warp >> 2) & 1;
   const int row = quad * 32 + lane;
   const uint32_t base = tmem + ((uint32_t)(quad * 32) << 16);
-  const uint32_t cs = base + col_s(tile), cpv = base + col_pv(tile), cq = base + col_q(tile);
+  const uint32_t cs = base + col_s(tile) + 64 * half, cpv = base + col_pv(tile) + 32 * half, cq = base + col_q(tile) + 16 * half;
+  const int pair = kBarPair + 2 * tile + (quad >> 1), end_bar = kBarEnd + tile;
   bool ok = true;
   int J = 0, C = 0;  // key tiles of the CTA and of this query tile so far
+  int pair_threads = 0;
+  // The other thread's value of this row.
+  auto exchange = [&](float v) {
+    bar_named(pair, pair_threads);  // the last value has been read
+    sh.row_x[tile][half][row] = v;
+    bar_named(pair, pair_threads);
+    return sh.row_x[tile][half ^ 1][row];
+  };
   Item it;
   for (int i = 0; take_item(sh, i, it); i++) {
     const int first = it.row0 + (it.split ? 0 : tile * kTcRows);
@@ -314,27 +332,31 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
     }
     const int step = it.split ? 2 : 1, t0 = it.t0 + (it.split ? tile : 0);
     const int end = t0 + (max(0, (tile == 0 ? it.end[0] : it.end[1]) - t0) + step - 1) / step * step;
-    const int warps = min(4, (it.rows - first + 31) >> 5);  // of this group that have rows
+    const int quads = min(4, (it.rows - first + 31) >> 5);  // quadrants of this group that have rows
     // The groups take turns at the softmax, so that each runs beside the other's products: the x-th of the first group,
-    // the x-th of the second, the x+1-th of the first, as far as the two have key tiles. Left alone they fall into step,
-    // wait for the tensor cores together and then compute together.
-    const int first1 = it.row0 + (it.split ? 0 : kTcRows), both = 32 * (min(4, (it.rows - it.row0 + 31) >> 5) + max(0, min(4, (it.rows - first1 + 31) >> 5)));
-    const int other = first1 >= it.rows ? 0 : it.split ? (it.end[0] - it.t0 + (tile ^ 1 ? 0 : 1)) >> 1 : (tile ? it.end[0] : it.end[1]) - it.t0;
-    if (quad >= warps) {
+    // the x-th of the second, the x+1-th of the first, for the `turns` that both have. Left alone they fall into step,
+    // wait for the tensor cores together and then compute together. Each signal is waited for once, the second group's
+    // last one by the first before it leaves the item, so that no group signals twice before it is heard.
+    const int first1 = it.row0 + (it.split ? 0 : kTcRows);
+    const int both = 64 * (min(4, (it.rows - it.row0 + 31) >> 5) + max(0, min(4, (it.rows - first1 + 31) >> 5)));
+    const int other = first1 >= it.rows ? 0 : it.split ? (it.end[0] - it.t0 + tile) >> 1 : (tile ? it.end[0] : it.end[1]) - it.t0;
+    const int mine = (end - t0) / step, turns = min(mine, other);
+    if (quad >= quads) {
       // None of this warp's rows exists. What is left in its rows of TMEM goes into no other row.
       J += it.t1 - it.t0;
       C += (end - t0) / step;
-      bar_named(7 + tile, 128 + 32);
+      bar_named(end_bar, 256 + 32);
       if (it.split) {
-        bar_named(4, 256);
-        bar_named(4, 256);
+        bar_named(kBarJoin, 512);
+        bar_named(kBarJoin, 512);
       }
       if (!it.whole && !(it.split && tile == 1)) {
-        bar_named(2 + tile, 128);
-        bar_named(2 + tile, 128);
+        bar_named(end_bar, 256);
+        bar_named(end_bar, 256);
       }
       continue;
     }
+    pair_threads = 64 * min(2, quads - (quad & 2));
     const int r = first + row;
     const bool live = r < it.rows;
     const int s = r / a.g, h = it.kvh * a.g + (r - s * a.g);
@@ -359,8 +381,8 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
       };
       uint32_t big = 0;
 #pragma unroll 4
-      for (int d = 0; d < 64; d += 4) {
-        const float4 f = get(d);
+      for (int d = 0; d < 32; d += 4) {
+        const float4 f = get(32 * half + d);
         const float v[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
         for (int e = 0; e < 4; e++) {
@@ -368,14 +390,15 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
           if (finite_bits(b)) big = max(big, b);
         }
       }
+      big = max(big, __float_as_uint(exchange(__uint_as_float(big))));
       float up;
       tile_scale(big, up, qdown);
 #pragma unroll 1
-      for (int c = 0; c < 4; c++) {  // 16 elements: 8 columns of hi, 8 of lo
+      for (int c = 0; c < 2; c++) {  // 16 elements: 8 columns of hi, 8 of lo
         float hi[8], lo[8];
 #pragma unroll
         for (int d = 0; d < 4; d++) {
-          const float4 f = get(16 * c + 4 * d);
+          const float4 f = get(32 * half + 16 * c + 4 * d);
           uint32_t h0, l0, h1, l1;
           split2(make_float2(f.x * up, f.y * up), h0, l0);
           split2(make_float2(f.z * up, f.w * up), h1, l1);
@@ -387,137 +410,121 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
       }
       tmem_st_wait();
       fence_before();
-      bar_signal(5 + tile, 32 * warps + 32);  // to the issuing warp
+      bar_signal(kBarIssue + tile, 64 * quads + 32);
     }
-    float2 o[32];
+    float2 o[16];
 #pragma unroll
-    for (int d = 0; d < 32; d++) o[d] = make_float2(0.0f, 0.0f);
+    for (int d = 0; d < 16; d++) o[d] = make_float2(0.0f, 0.0f);
     float m = -INFINITY, l = 0.0f;  // reference and sum of the weights
     int odd = 0;
-    float x[32], y[32];
-    // After a timed-out wait `ok` stays false: no further TMEM or barrier-object work, but the named barriers are met.
 #pragma unroll 1
     for (int t = t0; t < end; t += step) {
       const int j = J + t - it.t0, slot = j % kTcRing, turn = (t - t0) / step;
       if (ok && !warp_wait_bar(&sh.s_full[tile], C & 1, &sh.abort)) ok = false;
-      if (tile == 0 ? turn > 0 && turn <= other : turn < other) bar_named(9 + tile, both);
+      if (tile == 0 ? turn > 0 && turn <= turns : turn < turns) bar_named(kBarTurn + tile, both);
       fence_after();
       // kept finite and above 0: a score of 0 or -inf times it stays one
       const float c = fminf(fmaxf(qdown * sh.scale[0][slot], 1.1754944e-38f), 3.4028235e38f);
-      const int k0 = t * kTcKeys;
       const uint4 seen = *reinterpret_cast<const uint4*>(sh.seen[slot]);
-      if (k0 + kTcKeys - 1 > first_limit || (seen.x & seen.y & seen.z & seen.w) != 0xffffffffu) {
+      if (t * kTcKeys + kTcKeys - 1 > first_limit || (seen.x & seen.y & seen.z & seen.w) != 0xffffffffu) {
         // scores of keys that do not exist or that the row does not attend become -inf in place
 #pragma unroll 1
         for (int g = 0; g < 4; g++) {
-          const int n = limit - (k0 + 32 * g) + 1;
-          const uint32_t vis = sh.seen[slot][g] & (n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u);
-          tmem_get(cs + 32 * g, x);
-          tmem_ready(x);
+          const int k0 = 64 * half + 16 * g, n = limit - (t * kTcKeys + k0) + 1;
+          const uint32_t vis = (sh.seen[slot][k0 >> 5] >> (k0 & 31)) & (n >= 16 ? 0xffffu : n <= 0 ? 0u : (1u << n) - 1u);
+          float x[16];
+          tc::tmem_ld16(cs + 16 * g, x);
 #pragma unroll
-          for (int e = 0; e < 32; e++) x[e] = (vis >> e) & 1u ? x[e] : -INFINITY;
-          tmem_st32(cs + 32 * g, x);
+          for (int e = 0; e < 16; e++) x[e] = (vis >> e) & 1u ? x[e] : -INFINITY;
+          tc::tmem_st16(cs + 16 * g, x);
         }
         tmem_st_wait();
       }
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      auto largest = [&](const float (&v)[32]) {
+      float top = -INFINITY;
+#pragma unroll 1
+      for (int g = 0; g < 2; g++) {
+        float x[32], y = -INFINITY;
+        tmem_ld32(cs + 32 * g, x);
 #pragma unroll
-        for (int e = 0; e < 32; e += 8)
-#pragma unroll
-          for (int k = 0; k < 4; k++) mx[k] = fmaxf(mx[k], fmaxf(v[e + 2 * k], v[e + 2 * k + 1]));
-      };
-      tmem_get(cs, x);
-      tmem_ready(x);
-      tmem_get(cs + 32, y);
-      largest(x);
-      tmem_ready(y);
-      tmem_get(cs + 64, x);
-      largest(y);
-      tmem_ready(x);
-      tmem_get(cs + 96, y);
-      largest(x);
-      tmem_ready(y);
-      tmem_get(cs, x);  // for the exponentials
-      largest(y);
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
-      const bool rise = top > m + 9.0f;  // also from -inf; never on NaN
-      const float old = m;
-      if (rise) m = top;
+        for (int e = 0; e < 32; e += 4) {
+          top = fmaxf(top, fmaxf(x[e], x[e + 1]));
+          y = fmaxf(y, fmaxf(x[e + 2], x[e + 3]));
+        }
+        top = fmaxf(top, y);
+      }
+      top *= c;
+      float old = m;
+      const bool rise = bar_any(pair, pair_threads, top > m + 9.0f);  // of any row of these warps; also from -inf, never on NaN
+      if (rise) {
+        top = fmaxf(top, exchange(top));
+        if (top > m + 9.0f) m = top;
+      }
       const float ref = 6.0f - (m == -INFINITY ? 0.0f : m);
       const float2 c2 = make_float2(c, c), ref2 = make_float2(ref, ref);
       float2 sum0 = make_float2(0.0f, 0.0f), sum1 = sum0;
-      // 32 scores to weights, over the scores: keys 16 e .. of the tile as 8 columns of hi, 8 of lo
-      auto weights = [&](float (&v)[32], uint32_t col) {
-        float w[32];
+#pragma unroll 1
+      for (int g = 0; g < 4; g++) {
+        float x[16], w[16];
+        tc::tmem_ld16(cs + 16 * g, x);
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-          float2 p = __ffma2_rn(make_float2(v[2 * e], v[2 * e + 1]), c2, ref2);
+        for (int e = 0; e < 8; e++) {
+          float2 p = __ffma2_rn(make_float2(x[2 * e], x[2 * e + 1]), c2, ref2);
           p.x = ex2_sfu(p.x);
           p.y = ex2_sfu(p.y);
           if (e & 1) sum1 = __fadd2_rn(sum1, p);
           else sum0 = __fadd2_rn(sum0, p);
           uint32_t hi, lo;
           split2(p, hi, lo);
-          w[16 * (e >> 3) + (e & 7)] = __uint_as_float(hi);
-          w[16 * (e >> 3) + 8 + (e & 7)] = __uint_as_float(lo);
+          w[e] = __uint_as_float(hi);
+          w[8 + e] = __uint_as_float(lo);
         }
-        tmem_st32(col, w);
-      };
-      tmem_ready(x);
-#pragma unroll 1
-      for (int g = 0; g < 4; g += 2) {
-        tmem_get(cs + 32 * g + 32, y);
-        weights(x, cs + 32 * g);
-        tmem_ready(y);
-        if (g == 0) tmem_get(cs + 64, x);
-        weights(y, cs + 32 * g + 32);
-        if (g == 0) tmem_ready(x);
+        tc::tmem_st16(cs + 16 * g, w);  // over the scores just read: 16 keys as 8 columns of hi, 8 of lo
       }
       tmem_st_wait();
       fence_before();
-      bar_signal(5 + tile, 32 * warps + 32);
-      if (tile == 0 ? turn < other : turn + 1 < other) bar_signal(10 - tile, both);
+      bar_signal(kBarIssue + tile, 64 * quads + 32);
+      if (turn < turns) bar_signal(kBarTurn + (tile ^ 1), both);
       const float sum = (sum0.x + sum0.y) + (sum1.x + sum1.y);
-      if (__any_sync(0xffffffffu, rise)) {
-        const float alpha = rise ? ex2_sfu(old - m) : 1.0f;
+      if (rise) {
+        const float alpha = m == old ? 1.0f : ex2_sfu(old - m);
         const float2 al = make_float2(alpha, alpha);
         l = l * alpha + sum;
 #pragma unroll
-        for (int d = 0; d < 32; d++) o[d] = __fmul2_rn(o[d], al);
+        for (int d = 0; d < 16; d++) o[d] = __fmul2_rn(o[d], al);
       } else {
         l += sum;
       }
       if (ok && !warp_wait_bar(&sh.pv_full[tile], C & 1, &sh.abort)) ok = false;
       C++;
       fence_after();
-      tmem_get(cpv, x);
-      tmem_get(cpv + 32, y);
       const float2 f = make_float2(sh.scale[1][slot], sh.scale[1][slot]);
       odd |= sh.v_odd[slot];
-      tmem_ready(x);
-      tmem_ready(y);
 #pragma unroll
-      for (int d = 0; d < 16; d++) {
-        o[d] = __ffma2_rn(make_float2(x[2 * d], x[2 * d + 1]), f, o[d]);
-        o[16 + d] = __ffma2_rn(make_float2(y[2 * d], y[2 * d + 1]), f, o[16 + d]);
+      for (int c = 0; c < 2; c++) {
+        float x[16];
+        tc::tmem_ld16(cpv + 16 * c, x);
+#pragma unroll
+        for (int d = 0; d < 8; d++) o[8 * c + d] = __ffma2_rn(make_float2(x[2 * d], x[2 * d + 1]), f, o[8 * c + d]);
       }
     }
+    if (tile == 0 && turns > 0 && mine == turns) bar_named(kBarTurn, both);
+    l += exchange(l);  // before the group meets: the next item's rows may pair its warps differently
     // Every warp has read the last scales before the issuing warp frees tiles that the ring's slots are reused for, and
     // none of this group, those without rows included, gets ahead to the next item's barriers.
-    bar_named(7 + tile, 128 + 32);
+    bar_named(end_bar, 256 + 32);
     if (odd) {
       // Values that are not finite were left out of the products: add those that this row attends.
       const int k1 = min(it.t1 * kTcKeys, limit + 1);
+#pragma unroll 1
       for (int j = it.t0 * kTcKeys; j < k1; j++) {
         if (it.split && ((j / kTcKeys - it.t0) & 1) != tile) continue;
         const int pi = a.page.div(j);
         int page;
         if (!integral(a.table[it.req * a.t0 + pi * a.t1], 0, a.pages - 1, page)) continue;
-        const float* v = a.v + (int64_t)page * a.c0 + (int64_t)it.kvh * a.c1 + (int64_t)(j - pi * a.page.size) * a.c2;
+        const float* v = a.v + (int64_t)page * a.c0 + (int64_t)it.kvh * a.c1 + (int64_t)(j - pi * a.page.size) * a.c2 + 32 * half;
 #pragma unroll
-        for (int d = 0; d < 32; d++) {
-          if (2 * d >= a.D) break;
+        for (int d = 0; d < 16; d++) {
+          if (32 * half + 2 * d >= a.D) break;
           const float2 f = *reinterpret_cast<const float2*>(v + 2 * d);
           if (!finite_bits(__float_as_uint(f.x) & 0x7fffffffu)) o[d].x += f.x;
           if (!finite_bits(__float_as_uint(f.y) & 0x7fffffffu)) o[d].y += f.y;
@@ -529,32 +536,26 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
       // The second group's result goes to the first through the second's P·V columns (free until its next P).
       if (tile == 1 && ok) {
         tmem_st32(cpv, reinterpret_cast<const float*>(o));
-        tmem_st32(cpv + 32, reinterpret_cast<const float*>(o + 16));
         tmem_st_wait();
         fence_before();
         sh.join_m[row] = m;
         sh.join_l[row] = l;
       }
-      bar_named(4, 256);
+      bar_named(kBarJoin, 512);
       if (tile == 0 && ok) {
         fence_after();
         const float m1 = sh.join_m[row], mn = fmaxf(m, m1);
         const float f0 = mn == m ? 1.0f : ex2_sfu(m - mn), f1 = mn == m1 ? 1.0f : ex2_sfu(m1 - mn);
         m = mn;
         l = l * f0 + sh.join_l[row] * f1;
-        tmem_get(base + col_pv(1), x);
-        tmem_get(base + col_pv(1) + 32, y);
-        tmem_ready(x);
-        tmem_ready(y);
         const float2 g0 = make_float2(f0, f0), g1 = make_float2(f1, f1);
+        float x[32];
+        tmem_ld32(base + col_pv(1) + 32 * half, x);
 #pragma unroll
-        for (int d = 0; d < 16; d++) {
-          o[d] = __ffma2_rn(make_float2(x[2 * d], x[2 * d + 1]), g1, __fmul2_rn(o[d], g0));
-          o[16 + d] = __ffma2_rn(make_float2(y[2 * d], y[2 * d + 1]), g1, __fmul2_rn(o[16 + d], g0));
-        }
+        for (int d = 0; d < 16; d++) o[d] = __ffma2_rn(make_float2(x[2 * d], x[2 * d + 1]), g1, __fmul2_rn(o[d], g0));
         fence_before();
       }
-      bar_named(4, 256);
+      bar_named(kBarJoin, 512);
       if (tile == 1) continue;
     }
     bool write = it.whole != 0;
@@ -565,24 +566,25 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
       };
       float* mine = part_of(blockIdx.x);
 #pragma unroll
-      for (int d = 0; d < 32; d++) *reinterpret_cast<float2*>(mine + 2 * d) = o[d];
-      *reinterpret_cast<float2*>(mine + 64) = make_float2(m, l);
+      for (int d = 0; d < 16; d++) *reinterpret_cast<float2*>(mine + 32 * half + 2 * d) = o[d];
+      if (half == 0) *reinterpret_cast<float2*>(mine + 64) = make_float2(m, l);
       __threadfence();
-      bar_named(2 + tile, 128);
-      if (row == 0) {
+      bar_named(end_bar, 256);
+      if (row == 0 && half == 0) {
         unsigned* ticket = &a.tickets[2 * c0 + tile];
         sh.last[tile] = atomicAdd(ticket, 1u) == (unsigned)(c1 - c0);
         if (sh.last[tile]) *ticket = 0;
       }
-      bar_named(2 + tile, 128);
+      bar_named(end_bar, 256);
       write = sh.last[tile] != 0;
       if (write) {
         __threadfence();
         float M = -INFINITY;
+#pragma unroll 1
         for (int b = c0; b <= c1; b++) M = fmaxf(M, __ldcg(part_of(b) + 64));
         l = 0.0f;
 #pragma unroll
-        for (int d = 0; d < 32; d++) o[d] = make_float2(0.0f, 0.0f);
+        for (int d = 0; d < 16; d++) o[d] = make_float2(0.0f, 0.0f);
 #pragma unroll 1
         for (int b = c0; b <= c1; b++) {
           const float* p = part_of(b);
@@ -590,17 +592,17 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
           const float f = M == -INFINITY ? 1.0f : ex2_sfu(ml.x - M);
           l += ml.y * f;
 #pragma unroll
-          for (int d = 0; d < 32; d++)
-            o[d] = __ffma2_rn(__ldcg(reinterpret_cast<const float2*>(p + 2 * d)), make_float2(f, f), o[d]);
+          for (int d = 0; d < 16; d++)
+            o[d] = __ffma2_rn(__ldcg(reinterpret_cast<const float2*>(p + 32 * half + 2 * d)), make_float2(f, f), o[d]);
         }
       }
     }
     if (write && ok && live) {
-      float* out = a.out + ((int64_t)(it.first + s) * a.H + h) * a.D;
+      float* out = a.out + ((int64_t)(it.first + s) * a.H + h) * a.D + 32 * half;
       const float inv = 1.0f / l;
 #pragma unroll
-      for (int d = 0; d < 16; d++)
-        if (4 * d < a.D)
+      for (int d = 0; d < 8; d++)
+        if (32 * half + 4 * d < a.D)
           *reinterpret_cast<float4*>(out + 4 * d) =
               l == 0.0f ? make_float4(0.f, 0.f, 0.f, 0.f)
                         : make_float4(o[2 * d].x * inv, o[2 * d].y * inv, o[2 * d + 1].x * inv, o[2 * d + 1].y * inv);
@@ -615,8 +617,8 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
 // Splits the raw K and V tiles in place.
 __device__ __forceinline__ void convert_role(const AttnArgs& a, TcShared& sh, uint8_t* tiles) {
   const int tid = threadIdx.x - 32 * kConvWarp, warp = tid >> 5, lane = tid & 31;
-  const int tr = tid >> 4, tc4 = tid & 15;  // 16 threads per row, 8 rows per pass
-  uint8_t* dst0 = tiles + tr * 128 + (((tc4 >> 1) ^ tr) << 4) + ((tc4 & 1) << 3);
+  const int tr = tid >> 4, tc4 = tid & 15;  // 16 threads per row, 16 rows per pass
+  uint8_t* dst0 = tiles + tr * 128 + (((tc4 >> 1) ^ (tr & 7)) << 4) + ((tc4 & 1) << 3);
   bool ok = true;
   int J = 0;
   Item it;
@@ -625,7 +627,7 @@ __device__ __forceinline__ void convert_role(const AttnArgs& a, TcShared& sh, ui
     for (int k = 2 * it.t0; k < 2 * it.t1; k++) {
       const int op = k & 1, st = J % kTcStages, slot = J % kTcRing;
       const uint32_t at = (uint32_t)(op * kTcStages + st) * kTile;
-      float4 x[16];
+      float4 x[8];
       __nv_bfloat162 big2 = __floats2bfloat162_rn(0.0f, 0.0f);
       uint32_t big = 0;
       bool odd = false;
@@ -635,18 +637,18 @@ __device__ __forceinline__ void convert_role(const AttnArgs& a, TcShared& sh, ui
         const uint4 seen = *reinterpret_cast<const uint4*>(sh.seen[slot]);
         if (a.D == kTcDim && (seen.x & seen.y & seen.z & seen.w) == 0xffffffffu) {
 #pragma unroll
-          for (int p = 0; p < 16; p++) x[p] = *reinterpret_cast<const float4*>(raw + p * 8 * kTcDim);
+          for (int p = 0; p < 8; p++) x[p] = *reinterpret_cast<const float4*>(raw + p * 16 * kTcDim);
         } else {
           const uint32_t bits[4] = {seen.x, seen.y, seen.z, seen.w};
 #pragma unroll
-          for (int p = 0; p < 16; p++) {
-            const bool have = ((bits[p >> 2] >> ((p * 8 + tr) & 31)) & 1u) && 4 * tc4 < a.D;
-            x[p] = have ? *reinterpret_cast<const float4*>(raw + p * 8 * a.D) : make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int p = 0; p < 8; p++) {
+            const bool have = ((bits[p >> 1] >> ((p * 16 + tr) & 31)) & 1u) && 4 * tc4 < a.D;
+            x[p] = have ? *reinterpret_cast<const float4*>(raw + p * 16 * a.D) : make_float4(0.f, 0.f, 0.f, 0.f);
           }
         }
         // the largest magnitude, in bf16 (only its exponent counts)
 #pragma unroll
-        for (int p = 0; p < 16; p++) {
+        for (int p = 0; p < 8; p++) {
           big2 = __hmax2_nan(big2, __habs2(__floats2bfloat162_rn(x[p].x, x[p].y)));
           big2 = __hmax2_nan(big2, __habs2(__floats2bfloat162_rn(x[p].z, x[p].w)));
         }
@@ -656,7 +658,7 @@ __device__ __forceinline__ void convert_role(const AttnArgs& a, TcShared& sh, ui
         if (odd) {  // the largest finite magnitude
           big = 0;
 #pragma unroll
-          for (int p = 0; p < 16; p++) {
+          for (int p = 0; p < 8; p++) {
             const float v[4] = {x[p].x, x[p].y, x[p].z, x[p].w};
 #pragma unroll
             for (int e = 0; e < 4; e++) {
@@ -669,7 +671,7 @@ __device__ __forceinline__ void convert_role(const AttnArgs& a, TcShared& sh, ui
       big = __reduce_max_sync(0xffffffffu, big);
       odd = __any_sync(0xffffffffu, odd);
       if (lane == 0) sh.max_bits[op][warp] = big | (odd ? 0x80000000u : 0u);
-      bar_named(1, 32 * kConvWarps);  // the maxima are there, and every thread holds its part of the raw tile
+      bar_named(kBarConv, 32 * kConvWarps);  // the maxima are there, and every thread holds its part of the raw tile
       if (ok) {
         uint32_t any = 0;
         big = 0;
@@ -687,7 +689,7 @@ __device__ __forceinline__ void convert_role(const AttnArgs& a, TcShared& sh, ui
         }
         if (odd && op == 1) {  // a value that is not finite would spoil the rows that do not attend it, too
 #pragma unroll
-          for (int p = 0; p < 16; p++) {
+          for (int p = 0; p < 8; p++) {
             if (!isfinite(x[p].x)) x[p].x = 0.0f;
             if (!isfinite(x[p].y)) x[p].y = 0.0f;
             if (!isfinite(x[p].z)) x[p].z = 0.0f;
@@ -697,12 +699,12 @@ __device__ __forceinline__ void convert_role(const AttnArgs& a, TcShared& sh, ui
         const float2 up2 = make_float2(up, up);
         uint8_t* dst = dst0 + at;
 #pragma unroll
-        for (int p = 0; p < 16; p++) {
+        for (int p = 0; p < 8; p++) {
           uint2 hi, lo;
           split2(__fmul2_rn(make_float2(x[p].x, x[p].y), up2), hi.x, lo.x);
           split2(__fmul2_rn(make_float2(x[p].z, x[p].w), up2), hi.y, lo.y);
-          *reinterpret_cast<uint2*>(dst + p * 1024) = hi;
-          *reinterpret_cast<uint2*>(dst + p * 1024 + kHalfTile) = lo;
+          *reinterpret_cast<uint2*>(dst + p * 2048) = hi;
+          *reinterpret_cast<uint2*>(dst + p * 2048 + kHalfTile) = lo;
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
@@ -735,6 +737,7 @@ __device__ __forceinline__ void load_role(const AttnArgs& a, TcShared& sh, uint8
       const int p0 = a.page.div(k0), p1 = k1 > k0 ? a.page.div(k1 - 1) : p0 - 1;
       uint32_t seen[4] = {0, 0, 0, 0};
       int count = 0;
+#pragma unroll 1
       for (int pi = p0 + lane; pi <= p1; pi += 32) {
         int page;
         if (!integral(trow[pi * a.t1], 0, a.pages - 1, page)) {
@@ -752,6 +755,7 @@ __device__ __forceinline__ void load_role(const AttnArgs& a, TcShared& sh, uint8
       count = __reduce_add_sync(0xffffffffu, count);
 #pragma unroll
       for (int g = 0; g < 4; g++) seen[g] = __reduce_or_sync(0xffffffffu, seen[g]);
+#pragma unroll 1
       for (int op = 0; op < 2 && ok; op++) {
         if (!warp_wait_bar(&sh.empty[op][st], parity, &sh.abort)) {
           ok = false;
@@ -768,6 +772,7 @@ __device__ __forceinline__ void load_role(const AttnArgs& a, TcShared& sh, uint8
         __syncwarp();
         copied_k = true;
         const float* src = (op == 0 ? a.k : a.v) + head;
+#pragma unroll 1
         for (int pi = p0 + lane; pi <= p1; pi += 32) {
           int page;
           if (!integral(trow[pi * a.t1], 0, a.pages - 1, page)) continue;
@@ -777,6 +782,7 @@ __device__ __forceinline__ void load_role(const AttnArgs& a, TcShared& sh, uint8
           if (a.c2 == a.D) {
             bulk_g2s(to, from, (uint32_t)(j1 - j0) * row_bytes, &sh.raw[op][st]);
           } else {
+#pragma unroll 1
             for (int j = j0; j < j1; j++) bulk_g2s(to + (uint32_t)(j - j0) * row_bytes, from + (int64_t)(j - j0) * a.c2, row_bytes, &sh.raw[op][st]);
           }
         }
@@ -812,8 +818,10 @@ __device__ __forceinline__ void load_role(const AttnArgs& a, TcShared& sh, uint8
 __device__ __forceinline__ void issue_role(const AttnArgs& a, TcShared& sh, uint8_t* tiles, uint32_t tmem, int tile) {
   constexpr uint32_t is = idesc_f16(kTcRows, kTcKeys, false), ip = idesc_f16(kTcRows, kTcDim, true);
   const int lane = threadIdx.x & 31;
+  // the same in every lane, and known to be: else each product would be wrapped in a loop over the lanes' values
+  auto uniform = [](uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); };
   const uint32_t leader = lane == 0, k_tiles = smem_u32(tiles), v_tiles = k_tiles + kTcStages * kTile;
-  const uint32_t cs = tmem + col_s(tile), cpv = tmem + col_pv(tile), cq = tmem + col_q(tile);
+  const uint32_t cs = uniform(tmem + col_s(tile)), cpv = uniform(tmem + col_pv(tile)), cq = uniform(tmem + col_q(tile));
   bool ok = true;
   int J = 0, C = 0;
   Item it;
@@ -822,7 +830,9 @@ __device__ __forceinline__ void issue_role(const AttnArgs& a, TcShared& sh, uint
   };
   // the CTA's key tiles [j, end) that this query tile does not use: its share of freeing them, once they are split
   auto skip = [&](int j, int end) {
+#pragma unroll 1
     for (; ok && j < end; j++)
+#pragma unroll 1
       for (int op = 0; op < 2 && ok; op++) {
         ok = wait_split(op, j);
         if (ok && lane == 0) mbar_arrive(&sh.empty[op][j % kTcStages]);
@@ -837,44 +847,46 @@ __device__ __forceinline__ void issue_role(const AttnArgs& a, TcShared& sh, uint
     }
     const int step = it.split ? 2 : 1, t0 = it.t0 + (it.split ? tile : 0);
     const int end = t0 + (max(0, (tile == 0 ? it.end[0] : it.end[1]) - t0) + step - 1) / step * step;
-    const int threads = 32 * min(4, (it.rows - first + 31) >> 5) + 32;
-    bar_named(5 + tile, threads);  // Q is in TMEM
+    const int threads = 64 * min(4, (it.rows - first + 31) >> 5) + 32;
+    bar_named(kBarIssue + tile, threads);  // Q is in TMEM
 #pragma unroll 1
     for (int t = t0; t < end; t += step, C++) {
       const int j = J + t - it.t0, st = j % kTcStages;
-      // K is split, and the last P has been read
-      ok = ok && wait_split(0, j) && (C == 0 || warp_wait_bar(&sh.pv_full[tile], (C - 1) & 1, &sh.abort));
+      if (t == t0) ok = ok && wait_split(0, j);
+      ok = ok && (C == 0 || warp_wait_bar(&sh.pv_full[tile], (C - 1) & 1, &sh.abort));  // the last P has been read
       if (ok) {
         fence_after();
-        const uint32_t kh = k_tiles + st * kTile, kl = kh + kHalfTile;
+        const uint32_t kh = uniform(k_tiles + st * kTile);
+#pragma unroll 1
+        for (uint32_t i = 0; i < 3; i++) {  // lo·hi, hi·lo, hi·hi: the small ones first
+          const uint32_t q = cq + (i == 0 ? 32u : 0u);
+          const uint64_t k = desc_sw128(kh + (i == 1 ? kHalfTile : 0u));
 #pragma unroll
-        for (int e = 0; e < 4; e++) mma_f16_ts(cs, cq + 32 + 8 * e, desc_sw128(kh + 32 * e), is, e > 0, leader);
-#pragma unroll
-        for (int e = 0; e < 4; e++) mma_f16_ts(cs, cq + 8 * e, desc_sw128(kl + 32 * e), is, 1u, leader);
-#pragma unroll
-        for (int e = 0; e < 4; e++) mma_f16_ts(cs, cq + 8 * e, desc_sw128(kh + 32 * e), is, 1u, leader);
+          for (uint32_t e = 0; e < 4; e++) mma_f16_ts(cs, q + 8 * e, k + 2 * e, is, i + e, leader);
+        }
         commit_if(&sh.s_full[tile], leader);
         commit_if(&sh.empty[0][st], leader);
         if (it.split) commit_if(&sh.empty[0][st], leader);  // the other query tile's share as well
-        ok = wait_split(1, j);
+        ok = wait_split(1, j) && (t + step >= end || wait_split(0, j + step));  // here, where there is time
       }
-      bar_named(5 + tile, threads);  // P is in TMEM
+      bar_named(kBarIssue + tile, threads);  // P is in TMEM
       if (ok) {
         fence_after();
-        const uint32_t vh = v_tiles + st * kTile, vl = vh + kHalfTile;
-        // 16 keys per product: columns 16 e of P's hi part, 8 further of its lo part
+        const uint32_t vh = uniform(v_tiles + st * kTile);
+#pragma unroll 1
+        for (uint32_t i = 0; i < 3; i++) {
+          // 16 keys per product: columns 16 e of P's hi part, 8 further of its lo part
+          const uint32_t w = cs + (i == 0 ? 8u : 0u);
+          const uint64_t v = desc_sw128(vh + (i == 1 ? kHalfTile : 0u));
 #pragma unroll
-        for (int e = 0; e < 8; e++) mma_f16_ts(cpv, cs + 16 * e + 8, desc_sw128(vh + 2048 * e), ip, e > 0, leader);
-#pragma unroll
-        for (int e = 0; e < 8; e++) mma_f16_ts(cpv, cs + 16 * e, desc_sw128(vl + 2048 * e), ip, 1u, leader);
-#pragma unroll
-        for (int e = 0; e < 8; e++) mma_f16_ts(cpv, cs + 16 * e, desc_sw128(vh + 2048 * e), ip, 1u, leader);
+          for (uint32_t e = 0; e < 8; e++) mma_f16_ts(cpv, w + 16 * e, v + 128 * e, ip, i + e, leader);
+        }
         commit_if(&sh.pv_full[tile], leader);
         commit_if(&sh.empty[1][st], leader);
         if (it.split) commit_if(&sh.empty[1][st], leader);
       }
     }
-    bar_named(7 + tile, 128 + 32);
+    bar_named(kBarEnd + tile, 256 + 32);
     if (!it.split) skip(J + end - it.t0, next);
     J = next;
   }
@@ -920,6 +932,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_tc(const AttnArgs a) {
   const int per = (a.n + kTcThreads - 1) / kTcThreads;
   const int i0 = min(a.n, tid * per), i1 = min(a.n, i0 + per);
   int64_t mine = 0, total;
+#pragma unroll 1
   for (int i = i0; i < i1; i++) {
     Req r;
     if (!load_req(a, i, r)) atomicExch(a.error_flag, 74);
@@ -930,6 +943,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_tc(const AttnArgs a) {
   const int64_t u0 = c * total / max(G, (int64_t)1), u1 = (c + 1) * total / max(G, (int64_t)1);
   if (c < G && before <= u0 && u0 < before + mine) {
     int64_t off = u0 - before;
+#pragma unroll 1
     for (int i = i0; i < i1; i++) {
       Req r;
       load_req(a, i, r);
