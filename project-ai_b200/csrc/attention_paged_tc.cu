@@ -19,8 +19,8 @@
 //                   over S in TMEM, and add the last P·V to their 32 registers of output while the tensor cores compute
 //                   the next S. The two groups take turns at this. (One thread per row left each scheduler one warp at
 //                   this work, 336 cycles per 16 keys, most of it latency; two take 160 each, what the pipes need.)
-//   warps 16-23     split K and V: read a raw fp32 tile from shared memory, write hi and lo (SWIZZLE_128B rows of 64)
-//                   over it;
+//   warps 16-19, 20-23  split K and V: read a raw fp32 tile from shared memory, write hi and lo (SWIZZLE_128B rows of
+//                   64) over it, eight rows at a time;
 //   warp 24         copies raw K and V rows from their pages with bulk copies, up to three tiles ahead;
 //   warps 25, 26    issue S = Q·Kᵀ and P·V of one query tile each;
 //   warp 27         walks the CTA's share of the work and hands the items to the others.
@@ -42,7 +42,6 @@ namespace paged {
 
 using tc::bulk_g2s;
 using tc::commit;
-using tc::desc_sw128;
 using tc::ex2_sfu;
 using tc::fence_after;
 using tc::fence_before;
@@ -60,25 +59,25 @@ constexpr int kTcDim = 64;                   // padded head dim
 constexpr int kTcStages = 3;                 // K and V tiles in shared memory
 constexpr int kTcRing = 8;                   // scales of the last tiles (more than the tiles in flight between two readers)
 constexpr int kSoftmaxWarps = 8;             // per query tile
-constexpr int kConvWarps = 8;
-constexpr int kConvWarp = 2 * kSoftmaxWarps, kLoadWarp = kConvWarp + kConvWarps, kIssueWarp = kLoadWarp + 1;
+constexpr int kConvWarps = 4;                // for K, and for V
+constexpr int kConvWarp = 2 * kSoftmaxWarps, kLoadWarp = kConvWarp + 2 * kConvWarps, kIssueWarp = kLoadWarp + 1;
 constexpr int kWalkWarp = kIssueWarp + 2;
 constexpr int kTcThreads = 32 * (kWalkWarp + 1);  // seven warpgroups
 constexpr int kItems = 4;                         // items handed out ahead
-// Registers per thread of the softmax, conversion and loading/issuing warpgroups: 4·88 + 2·56 + 40 = 504, what the CTA is
+// Registers per thread of the softmax, conversion and loading/issuing warpgroups: 4·96 + 2·40 + 40 = 504, what the CTA is
 // launched with (7·72).
-constexpr int kLaunchRegs = 72, kSoftmaxRegs = 88, kConvRegs = 56, kMiscRegs = 40;
+constexpr int kLaunchRegs = 72, kSoftmaxRegs = 96, kConvRegs = 40, kMiscRegs = 40;
 static_assert(4 * kSoftmaxRegs + 2 * kConvRegs + kMiscRegs <= 7 * kLaunchRegs, "more registers than the launch holds");
 static_assert(kTcThreads == 7 * 128 && kTcThreads * kLaunchRegs <= 65536, "one CTA's registers");
 // Named barriers (0 is __syncthreads)
-constexpr int kBarConv = 1;    // conversion warps
 constexpr int kBarIssue = 2;   // + query tile: softmax warps with rows arrive, the issuing warp waits (Q or P is in TMEM)
 constexpr int kBarTurn = 12;   // + query tile: a group waits for its turn, the other arrives
+constexpr int kBarConv = 14;   // + 1 for V: conversion warps
 constexpr int kBarJoin = 4;    // both groups, at the end of split items
 constexpr int kBarEnd = 5;     // + query tile: end of an item
 constexpr int kBarPair = 8;    // + 2 query tile + quadrant / 2: the warps that share rows, of two quadrants
-constexpr uint32_t kHalfTile = kTcKeys * 128;      // hi or lo: 128 rows of 64 fp16
-constexpr uint32_t kTile = 2 * kHalfTile;          // 32 KB, the size of the raw fp32 tile as well
+// A tile of 128 rows: eight rows take 2 KB, raw (64 fp32 each) or split (64 fp16 of hi each, then of lo).
+constexpr uint32_t kGroup = 2048, kLo = 1024, kTile = 16 * kGroup;
 constexpr int kTcPart = 2 * kTcRows * (kTcDim + 2);  // floats of one partial result
 // TMEM columns: S and P of both query tiles, their P·V, their Q (hi, lo: 32 columns each)
 __host__ __device__ constexpr uint32_t col_s(int t) { return 128u * (uint32_t)t; }
@@ -106,7 +105,7 @@ struct TcShared {
   int64_t off;
   alignas(16) uint32_t seen[kTcRing][4];  // keys of a tile that exist (bit per key)
   float row_x[2][2][kTcRows];    // [query tile][half]: what the two threads of a row exchange
-  alignas(16) uint32_t max_bits[2][kConvWarps];  // converter warps' largest magnitudes; top bit: one is not finite
+  alignas(16) uint32_t max_bits[2][2][kConvWarps];  // converter warps' largest magnitudes; top bit: one is not finite
   float join_m[kTcRows], join_l[kTcRows];        // split items: the second group's maxima and sums
   float scale[2][kTcRing];       // what a product with the tile is multiplied by to undo the tile's scale
   int v_odd[kTcRing];            // a V tile held values that are not finite
@@ -120,6 +119,11 @@ constexpr int kTcSmem = 1024 + 2 * kTcStages * (int)kTile + (int)sizeof(TcShared
 // kind::f16 descriptors: fp16 operands, fp32 accumulator; b_mn: B stored with its N index contiguous.
 __host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool b_mn) {
   return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+// Shared-memory descriptor of hi (or, kLo further, of lo): SWIZZLE_128B, groups of eight rows kGroup apart.
+__device__ __forceinline__ uint64_t desc_split(uint32_t addr) {
+  return (uint64_t)((addr & 0x3FFFF) >> 4) | (uint64_t)1 << 16 | (uint64_t)(kGroup >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 
 // D (TMEM) (+)= A (TMEM, two fp16 per column) · B (shared), issued by the lane whose `leader` is set. The whole warp runs
@@ -292,16 +296,16 @@ __device__ __forceinline__ void walk_role(const AttnArgs& a, TcShared& sh, int r
   }
 }
 
-// Item i for a whole warp (all of it copied, so the slot is free again); false when there is none. Waits the whole time
-// limit whether another role gave up or not: the warps that meet at named barriers must all see an item or none.
-__device__ __forceinline__ bool take_item(TcShared& sh, int i, Item& it) {
+// Item i for a whole warp, in shared memory until free_item(); null when there is none. Waits the whole time limit whether
+// another role gave up or not: the warps that meet at named barriers must all see an item or none.
+__device__ __forceinline__ const Item* take_item(TcShared& sh, int i) {
   const int slot = i % kItems;
-  it.stop = 0;
-  if (!warp_wait_bar(&sh.item_full[slot], (i / kItems) & 1, nullptr)) return false;
-  it = sh.items[slot];
+  if (!warp_wait_bar(&sh.item_full[slot], (i / kItems) & 1, nullptr) || sh.items[slot].stop) return nullptr;
+  return &sh.items[slot];
+}
+__device__ __forceinline__ void free_item(TcShared& sh, int i) {
   __syncwarp();
-  if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.item_free[slot]);
-  return it.stop == 0;
+  if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.item_free[i % kItems]);
 }
 
 // ---------------------------------------------------------------- roles
@@ -323,8 +327,9 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
     bar_named(pair, pair_threads);
     return sh.row_x[tile][half ^ 1][row];
   };
-  Item it;
-  for (int i = 0; take_item(sh, i, it); i++) {
+  const Item* p_it;
+  for (int i = 0; (p_it = take_item(sh, i)) != nullptr; free_item(sh, i), i++) {
+    const Item& it = *p_it;
     const int first = it.row0 + (it.split ? 0 : tile * kTcRows);
     if (first >= it.rows) {
       J += it.t1 - it.t0;
@@ -614,52 +619,54 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
   }
 }
 
-// Splits the raw K and V tiles in place.
-__device__ __forceinline__ void convert_role(const AttnArgs& a, TcShared& sh, uint8_t* tiles) {
-  const int tid = threadIdx.x - 32 * kConvWarp, warp = tid >> 5, lane = tid & 31;
-  const int tr = tid >> 4, tc4 = tid & 15;  // 16 threads per row, 16 rows per pass
-  uint8_t* dst0 = tiles + tr * 128 + (((tc4 >> 1) ^ (tr & 7)) << 4) + ((tc4 & 1) << 3);
+// Splits the raw K (op 0) or V (op 1) tiles in place. A warp has four of a tile's groups of eight rows; a first pass takes
+// the largest magnitude of the whole tile, a second splits group by group, so that few registers are held.
+__device__ __forceinline__ void convert_role(const AttnArgs& a, TcShared& sh, uint8_t* tiles, int op) {
+  const int warp = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
+  const int tr = lane >> 4, tc4 = lane & 15;  // 16 lanes per row, two rows at a time
+  const uint32_t to = tr * 128 + ((tc4 >> 1) << 4) + ((tc4 & 1) << 3);
   bool ok = true;
   int J = 0;
-  Item it;
-  for (int i = 0; take_item(sh, i, it); i++) {
+  const Item* p_it;
+  for (int i = 0; (p_it = take_item(sh, i)) != nullptr; i++) {
+    const int n = p_it->t1 - p_it->t0;
+    free_item(sh, i);
 #pragma unroll 1
-    for (int k = 2 * it.t0; k < 2 * it.t1; k++) {
-      const int op = k & 1, st = J % kTcStages, slot = J % kTcRing;
-      const uint32_t at = (uint32_t)(op * kTcStages + st) * kTile;
-      float4 x[8];
-      __nv_bfloat162 big2 = __floats2bfloat162_rn(0.0f, 0.0f);
+    for (int k = 0; k < n; k++, J++) {
+      const int st = J % kTcStages, slot = J % kTcRing;
+      uint8_t* mine = tiles + (op * kTcStages + st) * kTile + 4 * warp * kGroup;
       uint32_t big = 0;
       bool odd = false;
       if (ok && !warp_wait_bar(&sh.raw[op][st], (J / kTcStages) & 1, &sh.abort)) ok = false;
+      const uint32_t seen = sh.seen[slot][warp];  // of the warp's 32 rows
+      const bool have = 4 * tc4 < a.D;
+      // four elements of row 2 e + tr of group g
+      auto get = [&](int g, int e) {
+        return have && ((seen >> (8 * g + 2 * e + tr)) & 1u) ? *reinterpret_cast<const float4*>(mine + g * kGroup + (2 * e + tr) * 256 + 16 * tc4)
+                                                             : make_float4(0.f, 0.f, 0.f, 0.f);
+      };
       if (ok) {
-        const float* raw = reinterpret_cast<const float*>(tiles + at) + tr * a.D + 4 * tc4;
-        const uint4 seen = *reinterpret_cast<const uint4*>(sh.seen[slot]);
-        if (a.D == kTcDim && (seen.x & seen.y & seen.z & seen.w) == 0xffffffffu) {
+        __nv_bfloat162 big2 = __floats2bfloat162_rn(0.0f, 0.0f);  // in bf16: only its exponent counts
+#pragma unroll 1
+        for (int g = 0; g < 4; g++) {
+          float4 x[4];
 #pragma unroll
-          for (int p = 0; p < 8; p++) x[p] = *reinterpret_cast<const float4*>(raw + p * 16 * kTcDim);
-        } else {
-          const uint32_t bits[4] = {seen.x, seen.y, seen.z, seen.w};
+          for (int e = 0; e < 4; e++) x[e] = get(g, e);
 #pragma unroll
-          for (int p = 0; p < 8; p++) {
-            const bool have = ((bits[p >> 1] >> ((p * 16 + tr) & 31)) & 1u) && 4 * tc4 < a.D;
-            x[p] = have ? *reinterpret_cast<const float4*>(raw + p * 16 * a.D) : make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int e = 0; e < 4; e++) {
+            big2 = __hmax2_nan(big2, __habs2(__floats2bfloat162_rn(x[e].x, x[e].y)));
+            big2 = __hmax2_nan(big2, __habs2(__floats2bfloat162_rn(x[e].z, x[e].w)));
           }
-        }
-        // the largest magnitude, in bf16 (only its exponent counts)
-#pragma unroll
-        for (int p = 0; p < 8; p++) {
-          big2 = __hmax2_nan(big2, __habs2(__floats2bfloat162_rn(x[p].x, x[p].y)));
-          big2 = __hmax2_nan(big2, __habs2(__floats2bfloat162_rn(x[p].z, x[p].w)));
         }
         const uint32_t b2 = *reinterpret_cast<const uint32_t*>(&big2);
         big = max(b2 << 16, b2 & 0xffff0000u);
         odd = !finite_bits(big);
         if (odd) {  // the largest finite magnitude
           big = 0;
-#pragma unroll
-          for (int p = 0; p < 8; p++) {
-            const float v[4] = {x[p].x, x[p].y, x[p].z, x[p].w};
+#pragma unroll 1
+          for (int g = 0; g < 16; g++) {
+            const float4 x = get(g >> 2, g & 3);
+            const float v[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
             for (int e = 0; e < 4; e++) {
               const uint32_t b = __float_as_uint(v[e]) & 0x7fffffffu;
@@ -670,47 +677,49 @@ __device__ __forceinline__ void convert_role(const AttnArgs& a, TcShared& sh, ui
       }
       big = __reduce_max_sync(0xffffffffu, big);
       odd = __any_sync(0xffffffffu, odd);
-      if (lane == 0) sh.max_bits[op][warp] = big | (odd ? 0x80000000u : 0u);
-      bar_named(kBarConv, 32 * kConvWarps);  // the maxima are there, and every thread holds its part of the raw tile
-      if (ok) {
-        uint32_t any = 0;
-        big = 0;
+      uint32_t* maxima = sh.max_bits[op][J & 1];  // two sets: a warp may be a tile ahead of one that still reads
+      if (lane == 0) maxima[warp] = big | (odd ? 0x80000000u : 0u);
+      bar_named(kBarConv + op, 32 * kConvWarps);
+      if (!ok) continue;
+      const uint4 all = *reinterpret_cast<const uint4*>(maxima);
+      odd = ((all.x | all.y | all.z | all.w) >> 31) != 0;
+      big = max(max(all.x & 0x7fffffffu, all.y & 0x7fffffffu), max(all.z & 0x7fffffffu, all.w & 0x7fffffffu));
+      float up, down;
+      tile_scale(big, up, down);
+      if (warp == 0 && lane == 0) {
+        sh.scale[op][slot] = down;
+        if (op == 1) sh.v_odd[slot] = odd;
+      }
+      const float2 up2 = make_float2(up, up);
+#pragma unroll 1
+      for (int g = 0; g < 4; g++) {
+        float4 x[4];
 #pragma unroll
-        for (int w = 0; w < kConvWarps; w++) {
-          any |= sh.max_bits[op][w];
-          big = max(big, sh.max_bits[op][w] & 0x7fffffffu);
-        }
-        odd = (any >> 31) != 0;
-        float up, down;
-        tile_scale(big, up, down);
-        if (tid == 0) {
-          sh.scale[op][slot] = down;
-          if (op == 1) sh.v_odd[slot] = odd;
-        }
+        for (int e = 0; e < 4; e++) x[e] = get(g, e);
         if (odd && op == 1) {  // a value that is not finite would spoil the rows that do not attend it, too
 #pragma unroll
-          for (int p = 0; p < 8; p++) {
-            if (!isfinite(x[p].x)) x[p].x = 0.0f;
-            if (!isfinite(x[p].y)) x[p].y = 0.0f;
-            if (!isfinite(x[p].z)) x[p].z = 0.0f;
-            if (!isfinite(x[p].w)) x[p].w = 0.0f;
+          for (int e = 0; e < 4; e++) {
+            if (!isfinite(x[e].x)) x[e].x = 0.0f;
+            if (!isfinite(x[e].y)) x[e].y = 0.0f;
+            if (!isfinite(x[e].z)) x[e].z = 0.0f;
+            if (!isfinite(x[e].w)) x[e].w = 0.0f;
           }
         }
-        const float2 up2 = make_float2(up, up);
-        uint8_t* dst = dst0 + at;
+        __syncwarp();  // the group's raw rows are in registers
 #pragma unroll
-        for (int p = 0; p < 8; p++) {
+        for (int e = 0; e < 4; e++) {
           uint2 hi, lo;
-          split2(__fmul2_rn(make_float2(x[p].x, x[p].y), up2), hi.x, lo.x);
-          split2(__fmul2_rn(make_float2(x[p].z, x[p].w), up2), hi.y, lo.y);
-          *reinterpret_cast<uint2*>(dst + p * 2048) = hi;
-          *reinterpret_cast<uint2*>(dst + p * 2048 + kHalfTile) = lo;
+          split2(__fmul2_rn(make_float2(x[e].x, x[e].y), up2), hi.x, lo.x);
+          split2(__fmul2_rn(make_float2(x[e].z, x[e].w), up2), hi.y, lo.y);
+          // row r = 2 e + tr: 16-byte chunk c goes to c ^ r
+          uint8_t* dst = mine + g * kGroup + ((to + 2 * e * 128) ^ ((2 * e + tr) << 4));
+          *reinterpret_cast<uint2*>(dst) = hi;
+          *reinterpret_cast<uint2*>(dst + kLo) = lo;
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.conv[op][st]);
       }
-      if (op) J++;
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.conv[op][st]);
     }
   }
   if (!ok && lane == 0) {
@@ -726,8 +735,9 @@ __device__ __forceinline__ void load_role(const AttnArgs& a, TcShared& sh, uint8
   const uint32_t row_bytes = (uint32_t)a.D * 4;
   bool ok = true, bad = false, copied_k = false;
   int J = 0;
-  Item it;
-  for (int i = 0; ok && take_item(sh, i, it); i++) {
+  const Item* p_it;
+  for (int i = 0; ok && (p_it = take_item(sh, i)) != nullptr; free_item(sh, i), i++) {
+    const Item& it = *p_it;
     const float* trow = a.table + (int64_t)it.req * a.t0;
     const int64_t head = (int64_t)it.kvh * a.c1;
     for (int t = it.t0; t < it.t1; t++) {
@@ -778,12 +788,12 @@ __device__ __forceinline__ void load_role(const AttnArgs& a, TcShared& sh, uint8
           if (!integral(trow[pi * a.t1], 0, a.pages - 1, page)) continue;
           const int j0 = max(pi * P, k0), j1 = min((pi + 1) * P, k1);
           const float* from = src + (int64_t)page * a.c0 + (int64_t)(j0 - pi * P) * a.c2;
-          uint8_t* to = tile + (uint32_t)(j0 - k0) * row_bytes;
-          if (a.c2 == a.D) {
+          uint8_t* to = tile + (uint32_t)(j0 - k0) * 256;
+          if (a.c2 == kTcDim && a.D == kTcDim) {
             bulk_g2s(to, from, (uint32_t)(j1 - j0) * row_bytes, &sh.raw[op][st]);
           } else {
 #pragma unroll 1
-            for (int j = j0; j < j1; j++) bulk_g2s(to + (uint32_t)(j - j0) * row_bytes, from + (int64_t)(j - j0) * a.c2, row_bytes, &sh.raw[op][st]);
+            for (int j = j0; j < j1; j++) bulk_g2s(to + (uint32_t)(j - j0) * 256, from + (int64_t)(j - j0) * a.c2, row_bytes, &sh.raw[op][st]);
           }
         }
       }
@@ -824,7 +834,6 @@ __device__ __forceinline__ void issue_role(const AttnArgs& a, TcShared& sh, uint
   const uint32_t cs = uniform(tmem + col_s(tile)), cpv = uniform(tmem + col_pv(tile)), cq = uniform(tmem + col_q(tile));
   bool ok = true;
   int J = 0, C = 0;
-  Item it;
   auto wait_split = [&](int op, int j) {
     return warp_wait_bar(&sh.conv[op][j % kTcStages], (j / kTcStages) & 1, &sh.abort);
   };
@@ -838,7 +847,9 @@ __device__ __forceinline__ void issue_role(const AttnArgs& a, TcShared& sh, uint
         if (ok && lane == 0) mbar_arrive(&sh.empty[op][j % kTcStages]);
       }
   };
-  for (int i = 0; take_item(sh, i, it); i++) {
+  const Item* p_it;
+  for (int i = 0; (p_it = take_item(sh, i)) != nullptr; free_item(sh, i), i++) {
+    const Item it = *p_it;
     const int first = it.row0 + (it.split ? 0 : tile * kTcRows), next = J + it.t1 - it.t0;
     if (first >= it.rows) {
       skip(J, next);
@@ -860,7 +871,7 @@ __device__ __forceinline__ void issue_role(const AttnArgs& a, TcShared& sh, uint
 #pragma unroll 1
         for (uint32_t i = 0; i < 3; i++) {  // lo·hi, hi·lo, hi·hi: the small ones first
           const uint32_t q = cq + (i == 0 ? 32u : 0u);
-          const uint64_t k = desc_sw128(kh + (i == 1 ? kHalfTile : 0u));
+          const uint64_t k = desc_split(kh + (i == 1 ? kLo : 0u));
 #pragma unroll
           for (uint32_t e = 0; e < 4; e++) mma_f16_ts(cs, q + 8 * e, k + 2 * e, is, i + e, leader);
         }
@@ -877,9 +888,9 @@ __device__ __forceinline__ void issue_role(const AttnArgs& a, TcShared& sh, uint
         for (uint32_t i = 0; i < 3; i++) {
           // 16 keys per product: columns 16 e of P's hi part, 8 further of its lo part
           const uint32_t w = cs + (i == 0 ? 8u : 0u);
-          const uint64_t v = desc_sw128(vh + (i == 1 ? kHalfTile : 0u));
+          const uint64_t v = desc_split(vh + (i == 1 ? kLo : 0u));
 #pragma unroll
-          for (uint32_t e = 0; e < 8; e++) mma_f16_ts(cpv, w + 16 * e, v + 128 * e, ip, i + e, leader);
+          for (uint32_t e = 0; e < 8; e++) mma_f16_ts(cpv, w + 16 * e, v + (2 * kGroup >> 4) * e, ip, i + e, leader);
         }
         commit_if(&sh.pv_full[tile], leader);
         commit_if(&sh.empty[1][st], leader);
@@ -966,7 +977,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_tc(const AttnArgs a) {
       softmax_role(a, sh, tmem);
     } else if (warp < kLoadWarp) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvRegs));
-      convert_role(a, sh, tiles);
+      convert_role(a, sh, tiles, (warp - kConvWarp) / kConvWarps);
     } else {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMiscRegs));
       if (warp == kLoadWarp) load_role(a, sh, tiles);
