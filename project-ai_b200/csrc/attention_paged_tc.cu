@@ -252,7 +252,7 @@ __device__ __forceinline__ void walk_role(const AttnArgs& a, TcShared& sh, int r
         off = 0;
         continue;
       }
-      it.kvh = (int)(off / s.units);
+      it.kvh = (int)div_pos(off, s.units);
       int64_t rest = off - it.kvh * s.units;
       int group = 0, tiles;
 #pragma unroll 1
@@ -270,8 +270,8 @@ __device__ __forceinline__ void walk_role(const AttnArgs& a, TcShared& sh, int r
       it.t0 = (int)rest;
       it.t1 = (int)min((int64_t)tiles, rest + (u1 - u));
       it.whole = it.t0 == 0 && it.t1 == tiles;
-      it.c0 = (int)(((u - rest + 1) * G - 1) / total);
-      it.c1 = (int)(((u - rest + tiles) * G - 1) / total);
+      it.c0 = (int)div_pos((u - rest + 1) * G - 1, total);
+      it.c1 = (int)div_pos((u - rest + tiles) * G - 1, total);
       for (int t = 0; t < 2; t++) {
         const int row0 = it.row0 + t * kTcRows, last = min(s.rows, row0 + kTcRows) - 1;
         const int keys = it.shift + last / a.g + 1;  // that the tile's last row attends
@@ -370,45 +370,36 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
     float qdown;  // undoes the row's scale
     {
       const float* p = a.q + (int64_t)(it.first + s) * a.q0 + (int64_t)h * a.q1;
-      auto get = [&](int d) {  // four elements, as scores in powers of two want them; rounded once from 64 bits
-        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (live && d < a.D) {
-          if (a.q_vec) {
-            const float4 f = *reinterpret_cast<const float4*>(p + d);
-            v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
-          } else {
+      float x[32];
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = p[d + e];  // the head dim is a multiple of 4
-          }
-        }
-        return make_float4((float)((double)v[0] * a.scale2), (float)((double)v[1] * a.scale2),
-                           (float)((double)v[2] * a.scale2), (float)((double)v[3] * a.scale2));
-      };
-      uint32_t big = 0;
-#pragma unroll 4
       for (int d = 0; d < 32; d += 4) {
-        const float4 f = get(32 * half + d);
-        const float v[4] = {f.x, f.y, f.z, f.w};
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const uint32_t b = __float_as_uint(v[e]) & 0x7fffffffu;
-          if (finite_bits(b)) big = max(big, b);
+        float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (live && 32 * half + d < a.D) {  // the head dim is a multiple of 4
+          const float* q = p + 32 * half + d;
+          if (a.q_vec) f = *reinterpret_cast<const float4*>(q);
+          else f = make_float4(q[0], q[1], q[2], q[3]);
         }
+        x[d] = f.x; x[d + 1] = f.y; x[d + 2] = f.z; x[d + 3] = f.w;
+      }
+      uint32_t big = 0;
+#pragma unroll
+      for (int d = 0; d < 32; d++) {
+        x[d] = (float)((double)x[d] * a.scale2);  // scores in powers of two; rounded once from 64 bits
+        const uint32_t b = __float_as_uint(x[d]) & 0x7fffffffu;
+        if (finite_bits(b)) big = max(big, b);
       }
       big = max(big, __float_as_uint(exchange(__uint_as_float(big))));
       float up;
       tile_scale(big, up, qdown);
-#pragma unroll 1
+#pragma unroll
       for (int c = 0; c < 2; c++) {  // 16 elements: 8 columns of hi, 8 of lo
         float hi[8], lo[8];
 #pragma unroll
-        for (int d = 0; d < 4; d++) {
-          const float4 f = get(32 * half + 16 * c + 4 * d);
-          uint32_t h0, l0, h1, l1;
-          split2(make_float2(f.x * up, f.y * up), h0, l0);
-          split2(make_float2(f.z * up, f.w * up), h1, l1);
-          hi[2 * d] = __uint_as_float(h0); hi[2 * d + 1] = __uint_as_float(h1);
-          lo[2 * d] = __uint_as_float(l0); lo[2 * d + 1] = __uint_as_float(l1);
+        for (int d = 0; d < 8; d++) {
+          uint32_t h, l;
+          split2(make_float2(x[16 * c + 2 * d] * up, x[16 * c + 2 * d + 1] * up), h, l);
+          hi[d] = __uint_as_float(h);
+          lo[d] = __uint_as_float(l);
         }
         tc::tmem_st8(cq + 8 * c, hi);
         tc::tmem_st8(cq + 32 + 8 * c, lo);
@@ -566,13 +557,14 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
     bool write = it.whole != 0;
     if (!write) {
       const int c0 = it.c0, c1 = it.c1;
+      // a row's pairs of head dims kTcRows apart, so that a warp's 32 rows lie side by side; then its (m, l)
       auto part_of = [&](int b) {
-        return a.part + (size_t)(2 * b + (b == c0 ? 1 : 0)) * kTcPart + (size_t)(tile * kTcRows + row) * (kTcDim + 2);
+        return reinterpret_cast<float2*>(a.part + (size_t)(2 * b + (b == c0 ? 1 : 0)) * kTcPart + (size_t)tile * (kTcPart / 2)) + row;
       };
-      float* mine = part_of(blockIdx.x);
+      float2* mine = part_of(blockIdx.x);
 #pragma unroll
-      for (int d = 0; d < 16; d++) *reinterpret_cast<float2*>(mine + 32 * half + 2 * d) = o[d];
-      if (half == 0) *reinterpret_cast<float2*>(mine + 64) = make_float2(m, l);
+      for (int d = 0; d < 16; d++) mine[(16 * half + d) * kTcRows] = o[d];
+      if (half == 0) mine[32 * kTcRows] = make_float2(m, l);
       __threadfence();
       bar_named(end_bar, 256);
       if (row == 0 && half == 0) {
@@ -584,21 +576,27 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
       write = sh.last[tile] != 0;
       if (write) {
         __threadfence();
-        float M = -INFINITY;
-#pragma unroll 1
-        for (int b = c0; b <= c1; b++) M = fmaxf(M, __ldcg(part_of(b) + 64));
+        // one pass: the sums so far move to a larger reference when one comes
+        float2 ml = __ldcg(part_of(c0) + 32 * kTcRows);
+        m = -INFINITY;
         l = 0.0f;
 #pragma unroll
         for (int d = 0; d < 16; d++) o[d] = make_float2(0.0f, 0.0f);
 #pragma unroll 1
         for (int b = c0; b <= c1; b++) {
-          const float* p = part_of(b);
-          const float2 ml = __ldcg(reinterpret_cast<const float2*>(p + 64));
-          const float f = M == -INFINITY ? 1.0f : ex2_sfu(ml.x - M);
-          l += ml.y * f;
+          const float2* p = part_of(b);
+          float2 x[16];
 #pragma unroll
-          for (int d = 0; d < 16; d++)
-            o[d] = __ffma2_rn(__ldcg(reinterpret_cast<const float2*>(p + 32 * half + 2 * d)), make_float2(f, f), o[d]);
+          for (int d = 0; d < 16; d++) x[d] = __ldcg(p + (16 * half + d) * kTcRows);
+          const float2 now = ml;
+          if (b < c1) ml = __ldcg(part_of(b + 1) + 32 * kTcRows);
+          const float mn = fmaxf(m, now.x);
+          const float f0 = mn == m ? 1.0f : ex2_sfu(m - mn), f1 = mn == now.x ? 1.0f : ex2_sfu(now.x - mn);
+          m = mn;
+          l = l * f0 + now.y * f1;
+          const float2 g0 = make_float2(f0, f0), g1 = make_float2(f1, f1);
+#pragma unroll
+          for (int d = 0; d < 16; d++) o[d] = __ffma2_rn(x[d], g1, __fmul2_rn(o[d], g0));
         }
       }
     }
@@ -951,7 +949,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_tc(const AttnArgs a) {
   }
   const int64_t before = block_prefix<kTcThreads>(mine, sh.tmp, total);
   const int64_t G = min((int64_t)gridDim.x, total), c = blockIdx.x;
-  const int64_t u0 = c * total / max(G, (int64_t)1), u1 = (c + 1) * total / max(G, (int64_t)1);
+  const int64_t u0 = div_pos(c * total, max(G, (int64_t)1)), u1 = div_pos((c + 1) * total, max(G, (int64_t)1));
   if (c < G && before <= u0 && u0 < before + mine) {
     int64_t off = u0 - before;
 #pragma unroll 1

@@ -29,6 +29,8 @@ inline PageDiv page_div(int size) {
 // value per warp.
 template <int THREADS>
 __device__ __forceinline__ int64_t block_prefix(int64_t v, int64_t* tmp, int64_t& total) {
+  static_assert(THREADS % 32 == 0 && THREADS <= 1024, "one value per lane for the warps' sums");
+  constexpr int kWarps = THREADS / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int64_t x = v;
 #pragma unroll
@@ -39,14 +41,21 @@ __device__ __forceinline__ int64_t block_prefix(int64_t v, int64_t* tmp, int64_t
   __syncthreads();  // tmp may still be read from an earlier call
   if (lane == 31) tmp[warp] = x;
   __syncthreads();
-  int64_t before = 0;
-  total = 0;
+  int64_t w = lane < kWarps ? tmp[lane] : 0;  // every warp sums the warps' sums
 #pragma unroll
-  for (int w = 0; w < THREADS / 32; w++) {
-    if (w < warp) before += tmp[w];
-    total += tmp[w];
+  for (int o = 1; o < kWarps; o <<= 1) {
+    int64_t y = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += y;
   }
-  return before + x - v;
+  total = __shfl_sync(0xffffffffu, w, kWarps - 1);
+  const int64_t before = __shfl_sync(0xffffffffu, w, warp > 0 ? warp - 1 : 0);
+  return (warp > 0 ? before : 0) + x - v;
+}
+
+// a / b of numbers that are not negative; most fit 32 bits, whose division is several times shorter.
+__device__ __forceinline__ int64_t div_pos(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
+  return a / b;
 }
 
 }  // namespace paged
