@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsPerSm) k_paged_rows(const A
     const int kvh = (int)(pair / groups), row0 = (int)(pair - (int64_t)kvh * groups) * R;
     const int nrows = (int)min((int64_t)R, (int64_t)r.n * a.g - row0);
 
-    // query rows, scaled to powers of two; the product is rounded once from 64 bits
+    // query rows, scaled so that scores are powers of two
     float4 qv[R];
 #pragma unroll
     for (int x = 0; x < R; x++) {
@@ -140,10 +140,10 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsPerSm) k_paged_rows(const A
       if (x < nrows) {
         const int s = (row0 + x) / a.g, h = kvh * a.g + (row0 + x) - s * a.g;
         const float* p = a.q + (int64_t)(r.first + s) * a.q0 + (int64_t)h * a.q1 + d0;
-        if (d0 < a.D) qv[x].x = (float)((double)p[0] * a.scale2);
-        if (d0 + 1 < a.D) qv[x].y = (float)((double)p[1] * a.scale2);
-        if (d0 + 2 < a.D) qv[x].z = (float)((double)p[2] * a.scale2);
-        if (d0 + 3 < a.D) qv[x].w = (float)((double)p[3] * a.scale2);
+        if (d0 < a.D) qv[x].x = fmaf(p[0], a.scale_hi, p[0] * a.scale_lo);
+        if (d0 + 1 < a.D) qv[x].y = fmaf(p[1], a.scale_hi, p[1] * a.scale_lo);
+        if (d0 + 2 < a.D) qv[x].z = fmaf(p[2], a.scale_hi, p[2] * a.scale_lo);
+        if (d0 + 3 < a.D) qv[x].w = fmaf(p[3], a.scale_hi, p[3] * a.scale_lo);
       }
     }
     // the last key that each kept score's row attends
@@ -384,7 +384,9 @@ PAI_API pai_status pai_sdpa_paged(pai_ctx* ctx, const pai_tensor* q, const pai_t
   a.pages = k_cache->dims[0]; a.max_pages = table->dims[1];
   a.max_new = max_new > 0 ? std::min(max_new, a.rows) : a.rows;
   a.page = paged::page_div(k_cache->dims[2]);
-  a.scale2 = (double)scale * 1.4426950408889634;
+  const double scale2 = (double)scale * 1.4426950408889634;
+  a.scale_hi = (float)scale2;
+  a.scale_lo = (float)(scale2 - (double)a.scale_hi);
   a.tickets = ctx->d_tickets;
   a.error_flag = ctx->d_error_flag;
   if (numel(r) > 0) {

@@ -19,7 +19,9 @@ struct AttnArgs {
   float* out;                              // [rows, H, D]
   int n, rows, H, KVH, g, D, max_pages, pages, max_new;
   PageDiv page;
-  double scale2;                           // scale * log2(e): scores are kept in powers of two
+  // scale * log2(e), so that scores are powers of two, in two parts: q hi + q lo is off by one rounding (a scale in one
+  // part would bend all scores alike, by up to 2^-24 of themselves)
+  float scale_hi, scale_lo;
   int vec, q_vec;                          // cache rows, rows of q may be read as float4
   float* part;                             // partial results, two slots per block
   unsigned* tickets;                       // arrivals, one counter per block (all zero between launches)
