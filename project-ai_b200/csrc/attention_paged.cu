@@ -9,16 +9,34 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "attention_paged.cuh"
+#include "tc_common.cuh"
 
 namespace pai {
 namespace paged {
+
+using tc::ex2_sfu;
+using tc::smem_u32;
 
 constexpr int kRowsThreads = 256;
 constexpr int kRowsWarps = kRowsThreads / 32;
 constexpr int kRowsPerSm = 2;  // resident blocks (registers)
 constexpr int kUnit = 64;      // keys per unit of the work split
+constexpr int kGroupKeys = 2;  // consecutive keys per lane group
+constexpr float kRise = 8.0f;  // a row's reference follows its maximum when that is 2^kRise above it
+
+__device__ __forceinline__ void copy_async16(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void copy_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
+}
+
+constexpr int kRingBytes = 12288;  // per warp
 
 // V values per lane, summed over the L lanes of a group: each lane is left with max(1, V / L) of the sums, value
 // index base(lane) + i. Each step halves the values a lane keeps and sends the other half to its partner.
@@ -52,18 +70,31 @@ struct Scatter {
 
 // R query rows of one kv head (token-major: row = token * g + head of the group) against its keys.
 //
-// LPK lanes hold one key's or value's head dims (a float4 each) and the query rows' same dims in registers; a warp has
+// LPK lanes hold one key's or value's head dims (NV float4 each) and the query rows' same dims in registers; a warp has
 // 32 / LPK such groups with KH consecutive keys each. The KH * R partial dot products of a group are summed over its
 // lanes by Scatter, which leaves each lane one (row, key) score to exponentiate; the probabilities go back to the
-// group's lanes by shuffles for P V. Nothing passes through shared memory until a segment ends, and the next keys'
-// loads are in flight while these are computed.
+// group's lanes by shuffles for P V. Keys and values come through a ring in shared memory, which each lane fills by
+// asynchronous copies two steps ahead with what it reads itself, so the ring needs no barrier and the keys on their way
+// (128 KB per SM) no registers. Weights are taken against a reference that follows the row maximum only when that rises
+// by 2^8 (fp32 holds such weights as well), so the sums are hardly ever rescaled. Steps of keys that every row attends
+// have no masks, and where pages hold whole groups a group's page is looked up once.
 //
 // Work split: every (request, kv head, group of R rows) is ceil(len / 64) units; the units of all of them, in order,
-// are divided evenly over the blocks, so lengths need not be alike. A block's share is a run of segments; a segment
-// that is a whole (request, kv head, rows) writes its result, a partial one goes to the block's slot in `part`, and the
-// last of its blocks to arrive joins the slots in block order (the same sum whichever comes last).
-template <int R, int KH, int LPK>
+// are divided evenly over the blocks, so lengths need not be alike. A block's share is a run of segments, listed in
+// shared memory before the first begins: under load a dependent read takes 3,000 cycles and more, so the copies run on
+// into the next segment while one ends, and its queries are read while the one before is computed. A segment that is a
+// whole (request, kv head, rows) writes its result, a partial one goes to the block's slot in `part`, and the last of
+// its blocks to arrive joins the slots in block order (the same sum whichever comes last).
+struct Seg {
+  int req, first, row0, rows, kvh, shift;  // request and its first row; rows of the group; p_t = shift + t
+  int j0, jend, open;                      // keys j0 .. jend - 1; before `open`, every row attends every key
+  int whole, c0, c1;                       // not split; first and last block of a split one
+};
+constexpr int kSegs = 32;  // listed at a time
+
+template <int R, int LPK, int NV>
 __global__ void __launch_bounds__(kRowsThreads, kRowsPerSm) k_paged_rows(const AttnArgs a) {
+  constexpr int KH = kGroupKeys;
   constexpr int kGroups = 32 / LPK;       // key groups per warp
   constexpr int kStep = kGroups * KH;     // keys per warp step
   constexpr int kStride = kRowsWarps * kStep;
@@ -72,287 +103,472 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsPerSm) k_paged_rows(const A
   constexpr int kKeep = S::kKeep, kRep = S::kRep;
   constexpr int kOwn = kKeep >= KH ? kKeep / KH : 1;             // rows whose scores a lane keeps
   constexpr int kRowLanes = kKeep >= KH ? 1 : KH / kKeep;        // lanes (kRep apart) that share a row
-  constexpr int kWidth = 4 * LPK;                                // padded head dim
-  constexpr int kParts = kRowsWarps * kGroups;
-  constexpr int kSlot = R * (kWidth + 2);
-  __shared__ float s_acc[kParts][R][kWidth];
-  __shared__ float s_m[kParts][R], s_l[kParts][R];
+  constexpr int kWidth = 4 * LPK * NV;                           // padded head dim
+  constexpr int kOut = R * kWidth;
+  constexpr int kSlot = kOut + 2 * R;
+  constexpr int kStage = 2 * KH * NV * 32;                       // float4s of a warp's ring per step
+  constexpr int kStages = kRingBytes / (16 * kStage);
+  static_assert(kStages >= 3 && kStages * 4 <= 32, "copies ahead, and their bits in `wrong`");
+  constexpr int kRound = kOut < kRowsThreads ? R : kRowsThreads / kWidth;  // rows whose parts are joined at a time
+  constexpr int kQ = (kOut + kRowsThreads - 1) / kRowsThreads;
+  extern __shared__ float4 s_ring[];  // [warp][stage][K, V][KH][NV][lane]
+  __shared__ __align__(16) float s_acc[kRowsWarps][kRound][kWidth];
+  __shared__ __align__(16) float s_q[R][kWidth];
+  __shared__ float s_m[kRowsWarps][R], s_l[kRowsWarps][R];
   __shared__ int64_t s_tmp[kRowsWarps];
-  __shared__ int64_t s_off;
-  __shared__ int s_req, s_last;
+  __shared__ int64_t s_pair[2];
+  __shared__ Seg s_seg[kSegs], s_split[2];
+  __shared__ int s_last[2];
   pdl_trigger();
   pdl_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int grp = lane / LPK, gl = lane % LPK;
-  const int d0 = 4 * gl;
+  const int d0 = 4 * gl;  // the lane's head dims: d0 + 4 LPK h ..+ 3
 
-  zero_rest(a);
   auto units_of = [&](const Req& r, int& groups, int& tiles) -> int64_t {
-    groups = (int)(((int64_t)r.n * a.g + R - 1) / R);
+    groups = r.n > 0 ? (int)(((int64_t)r.n * a.g + R - 1) / R) : 0;
     tiles = max(1, (r.len + kUnit - 1) / kUnit);
-    return r.n > 0 ? (int64_t)a.KVH * groups * tiles : 0;
+    return (int64_t)a.KVH * groups * tiles;
   };
-  // the block's share of the units, and the request it starts in
+  // the block's share of the units
   const int per = (a.n + kRowsThreads - 1) / kRowsThreads;
   const int i0 = min(a.n, tid * per), i1 = min(a.n, i0 + per);
-  int64_t mine = 0, total;
+  int64_t units = 0, pairs = 0, total, all_pairs;
   int groups, tiles;
+  Req r;
   for (int i = i0; i < i1; i++) {
-    Req r;
     if (!load_req(a, i, r)) atomicExch(a.error_flag, 74);
-    mine += units_of(r, groups, tiles);
+    units += units_of(r, groups, tiles);
+    pairs += (int64_t)a.KVH * groups;
   }
-  const int64_t before = block_prefix<kRowsThreads>(mine, s_tmp, total);
+  const int64_t before = block_prefix<kRowsThreads>(units, s_tmp, total);
+  const int64_t pairs_before = block_prefix<kRowsThreads>(pairs, s_tmp, all_pairs);
   const int64_t G = min((int64_t)gridDim.x, total), c = blockIdx.x;
-  if (c >= G) return;
+  if (c >= G) {
+    zero_rest(a);
+    return;
+  }
   const int64_t u0 = c * total / G, u1 = (c + 1) * total / G;
-  if (before <= u0 && u0 < before + mine) {
-    int64_t off = u0 - before;
-    for (int i = i0; i < i1; i++) {
-      Req r;
-      load_req(a, i, r);
+  // the requests of this thread that have units in the block's share: f(request, its first unit, its first pair, its units)
+  auto each = [&](auto f) {
+    int64_t ub = before, pb = pairs_before;
+    for (int i = i0; i < i1 && ub < u1; i++) {
+      if (per > 1) load_req(a, i, r);
       const int64_t u = units_of(r, groups, tiles);
-      if (off < u) { s_req = i; s_off = off; break; }
-      off -= u;
+      if (u > 0 && ub + u > u0) f(i, ub, pb, u);
+      ub += u;
+      pb += (int64_t)a.KVH * groups;
     }
+  };
+  each([&](int, int64_t ub, int64_t pb, int64_t u) {
+    if (ub <= u0) s_pair[0] = pb + div_pos(u0 - ub, tiles);
+    if (u1 <= ub + u) s_pair[1] = pb + div_pos(u1 - 1 - ub, tiles);
+  });
+
+  auto store = [&](const Seg& g, int y, int d, float A, float L) {
+    if (y < g.rows && d < a.D) {
+      const int s = (g.row0 + y) / a.g, h = g.kvh * a.g + (g.row0 + y) - s * a.g;
+      a.out[((int64_t)(g.first + s) * a.H + h) * a.D + d] = L == 0.0f ? 0.0f : A / L;
+    }
+  };
+  float4* const ring = s_ring + warp * (kStages * kStage) + lane;
+  if (d0 + 4 * LPK * (NV - 1) >= a.D) {  // nothing is copied for lanes past the head dims
+#pragma unroll 1
+    for (int x = 0; x < kStages * 2 * KH * NV; x++) ring[x * 32] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
   __syncthreads();
-  int req = s_req;
-  int64_t off = s_off;
+  const int64_t p0 = s_pair[0];
+  const int segs = (int)(s_pair[1] - p0) + 1;
   bool bad_page = false;
+  int splits = 0;
 
-  for (int64_t u = u0; u < u1;) {
-    Req r;
-    load_req(a, req, r);
-    const int64_t units = units_of(r, groups, tiles);
-    if (off >= units) { req++; off = 0; continue; }
-    const int64_t pair = off / tiles;
-    const int tile0 = (int)(off - pair * tiles);
-    const int tile1 = (int)min((int64_t)tiles, tile0 + (u1 - u));
-    const int kvh = (int)(pair / groups), row0 = (int)(pair - (int64_t)kvh * groups) * R;
-    const int nrows = (int)min((int64_t)R, (int64_t)r.n * a.g - row0);
-
-    // query rows, scaled so that scores are powers of two
-    float4 qv[R];
-#pragma unroll
-    for (int x = 0; x < R; x++) {
-      qv[x] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (x < nrows) {
-        const int s = (row0 + x) / a.g, h = kvh * a.g + (row0 + x) - s * a.g;
-        const float* p = a.q + (int64_t)(r.first + s) * a.q0 + (int64_t)h * a.q1 + d0;
-        if (d0 < a.D) qv[x].x = fmaf(p[0], a.scale_hi, p[0] * a.scale_lo);
-        if (d0 + 1 < a.D) qv[x].y = fmaf(p[1], a.scale_hi, p[1] * a.scale_lo);
-        if (d0 + 2 < a.D) qv[x].z = fmaf(p[2], a.scale_hi, p[2] * a.scale_lo);
-        if (d0 + 3 < a.D) qv[x].w = fmaf(p[3], a.scale_hi, p[3] * a.scale_lo);
+  for (int base = 0; base < segs; base += kSegs) {
+    const int ns = min(kSegs, segs - base);
+    each([&](int i, int64_t ub, int64_t pb, int64_t u) {
+      const int64_t lo = max(u0, ub) - ub, hi = min(u1, ub + u) - ub;
+      const int64_t first = max(pb + div_pos(lo, tiles), p0 + base), last = min(pb + div_pos(hi - 1, tiles), p0 + base + ns - 1);
+      for (int64_t pair = first; pair <= last; pair++) {
+        Seg g;
+        const int64_t at = ub + (pair - pb) * tiles;  // the pair's first unit
+        const int tile0 = (int)(max(u0, at) - at), tile1 = (int)(min(u1, at + tiles) - at);
+        g.req = i;
+        g.first = r.first;
+        g.kvh = (int)(pair - pb) / groups;
+        g.row0 = ((int)(pair - pb) - g.kvh * groups) * R;
+        g.rows = (int)min((int64_t)R, (int64_t)r.n * a.g - g.row0);
+        g.shift = r.len - r.n;
+        g.j0 = tile0 * kUnit;
+        g.jend = min(tile1 * kUnit, g.shift + (g.row0 + g.rows - 1) / a.g + 1);
+        g.open = min(g.jend, g.shift + g.row0 / a.g + 1);
+        g.whole = tile0 == 0 && tile1 == tiles;
+        g.c0 = (int)div_pos((at + 1) * G - 1, total);
+        g.c1 = (int)div_pos((at + tiles) * G - 1, total);
+        s_seg[pair - p0 - base] = g;
       }
-    }
-    // the last key that each kept score's row attends
-    int limit[kOwn];
-#pragma unroll
-    for (int o = 0; o < kOwn; o++) {
-      const int x = S::base(gl) / KH + o;
-      limit[o] = x < nrows ? r.len - r.n + (row0 + x) / a.g : -1;
-    }
-    const int most = r.len - r.n + (row0 + nrows - 1) / a.g;  // the last row's
-    const int jend = min(tile1 * kUnit, most + 1);
+    });
+    __syncthreads();
 
-    float4 acc[R];
-    float m[kOwn], l[kOwn];
+    // the queries of a segment, scaled so that scores are powers of two
+    float qn[kQ];
+    auto read_q = [&](const Seg& g) {
 #pragma unroll
-    for (int x = 0; x < R; x++) acc[x] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int o = 0; o < kOwn; o++) { m[o] = -INFINITY; l[o] = 0.0f; }
-
-    const float* trow = a.table + (int64_t)req * a.t0;
-    const int64_t head_off = (int64_t)kvh * a.c1 + d0;
-    // keys j .. j+KH-1 of this lane's group; bit e of `seen` is set where key j + e exists
-    auto load = [&](int j, float4 (&kf)[KH], float4 (&vf)[KH]) -> unsigned {
-      unsigned seen = 0;
-#pragma unroll
-      for (int e = 0; e < KH; e++) {
-        kf[e] = vf[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (j + e < jend) {
-          const int pi = a.page.div(j + e);
-          int page;
-          if (integral(trow[pi * a.t1], 0, a.pages - 1, page)) {
-            seen |= 1u << e;
-            const int64_t at = (int64_t)page * a.c0 + (int64_t)(j + e - pi * a.page.size) * a.c2 + head_off;
-            if (a.vec) {
-              if (d0 < a.D) {
-                kf[e] = *reinterpret_cast<const float4*>(a.k + at);
-                vf[e] = *reinterpret_cast<const float4*>(a.v + at);
-              }
-            } else {
-              if (d0 < a.D) { kf[e].x = a.k[at]; vf[e].x = a.v[at]; }
-              if (d0 + 1 < a.D) { kf[e].y = a.k[at + 1]; vf[e].y = a.v[at + 1]; }
-              if (d0 + 2 < a.D) { kf[e].z = a.k[at + 2]; vf[e].z = a.v[at + 2]; }
-              if (d0 + 3 < a.D) { kf[e].w = a.k[at + 3]; vf[e].w = a.v[at + 3]; }
-            }
-          } else {
-            bad_page = true;
-          }
+      for (int i = 0; i < kQ; i++) {
+        const int t = tid + i * kRowsThreads, y = t / kWidth, d = t % kWidth;
+        qn[i] = 0.0f;
+        if (t < kOut && y < g.rows && d < a.D) {
+          const int s = (g.row0 + y) / a.g, head = g.kvh * a.g + (g.row0 + y) - s * a.g;
+          qn[i] = a.q[(int64_t)(g.first + s) * a.q0 + (int64_t)head * a.q1 + d];
         }
       }
-      return seen;
+    };
+    auto write_q = [&] {
+#pragma unroll
+      for (int i = 0; i < kQ; i++) {
+        const int t = tid + i * kRowsThreads;
+        if (t < kOut) s_q[t / kWidth][t % kWidth] = fmaf(qn[i], a.scale_hi, qn[i] * a.scale_lo);
+      }
     };
 
-    float4 kf[KH], vf[KH];
-    int j = tile0 * kUnit + warp * kStep;  // the warp's keys; its groups' are KH apart
-    unsigned seen = load(j + grp * KH, kf, vf);
-    while (j < jend) {
-      float4 kn[KH], vn[KH];
-      const unsigned seen_next = load(j + kStride + grp * KH, kn, vn);
-      float x[V];
+    // what the copies read next: step ld_j (a warp's groups' keys are KH apart) of segment ld
+    int ld = -1, ld_j = 0, ld_end = 0;
+    const float* trow = nullptr;
+    int64_t head_off = 0;
+    float id = 0.0f;      // of the page of the lane's first key there
+    unsigned wrong = 0;   // four bits per stage: the keys whose page is named wrongly
+    auto advance = [&] {
+      ld_j += kStride;
+      while (ld_j >= ld_end && ++ld < ns) {
+        const Seg& g = s_seg[ld];
+        ld_j = g.j0 + warp * kStep;
+        ld_end = g.jend;
+        trow = a.table + (int64_t)g.req * a.t0;
+        head_off = (int64_t)g.kvh * a.c1 + d0;
+      }
+      if (ld < ns) id = trow[a.page.div(min(ld_j + grp * KH, ld_end - 1)) * a.t1];
+    };
+    // Starts the copies of the lane's part of that step's KH keys and values into stage `st`. Keys that do not exist or
+    // whose page is named wrongly are zero or unused.
+    auto stage = [&](int st) {
+      wrong &= ~(15u << (4 * st));
+      if (ld < ns) {
+        const int jg = ld_j + grp * KH;
+        float4* to = ring + st * kStage;
+        if (a.whole_groups && ld_j + kStep <= ld_end) {
+          int page;
+          if (!integral(id, 0, a.pages - 1, page)) {
+            wrong |= 15u << (4 * st);
+            page = 0;
+          }
+          const int64_t at = (int64_t)page * a.c0 + (jg - a.page.div(jg) * a.page.size) * a.c2 + head_off;
+          const float* kp = a.k + at;
+          const float* vp = a.v + at;
+#pragma unroll
+          for (int h = 0; h < NV; h++)
+            if (d0 + 4 * LPK * h < a.D) {
+#pragma unroll
+              for (int e = 0; e < KH; e++) {
+                copy_async16(to + (e * NV + h) * 32, kp + e * a.c2 + 4 * LPK * h);
+                copy_async16(to + ((KH + e) * NV + h) * 32, vp + e * a.c2 + 4 * LPK * h);
+              }
+            }
+        } else {
+#pragma unroll 1
+          for (int e = 0; e < KH; e++) {
+            int64_t at = -1;
+            if (jg + e < ld_end) {
+              const int pi = a.page.div(jg + e);
+              int page;
+              if (integral(trow[pi * a.t1], 0, a.pages - 1, page))
+                at = (int64_t)page * a.c0 + (int64_t)(jg + e - pi * a.page.size) * a.c2 + head_off;
+              else
+                wrong |= 1u << (4 * st + e);
+            }
+#pragma unroll 1
+            for (int h = 0; h < NV; h++) {
+              const int d = d0 + 4 * LPK * h;
+              const float* kp = a.k + at + 4 * LPK * h;
+              const float* vp = a.v + at + 4 * LPK * h;
+              float4 kf = make_float4(0.f, 0.f, 0.f, 0.f), vf = kf;
+              if (at >= 0 && a.vec) {
+                if (d < a.D) {
+                  kf = *reinterpret_cast<const float4*>(kp);
+                  vf = *reinterpret_cast<const float4*>(vp);
+                }
+              } else if (at >= 0) {
+                if (d < a.D) { kf.x = kp[0]; vf.x = vp[0]; }
+                if (d + 1 < a.D) { kf.y = kp[1]; vf.y = vp[1]; }
+                if (d + 2 < a.D) { kf.z = kp[2]; vf.z = vp[2]; }
+                if (d + 3 < a.D) { kf.w = kp[3]; vf.w = vp[3]; }
+              }
+              to[(e * NV + h) * 32] = kf;
+              to[((KH + e) * NV + h) * 32] = vf;
+            }
+          }
+        }
+        bad_page = bad_page || wrong != 0;
+        advance();
+      }
+      copy_async_commit();
+    };
+
+    read_q(s_seg[0]);
+    advance();
+    write_q();
+#pragma unroll
+    for (int x = 0; x < kStages - 1; x++) stage(x);
+    __syncthreads();
+    int turn = 0;
+    for (int x = 0; x < ns; x++) {
+      const Seg& g = s_seg[x];
+      float4 qv[R][NV];
+      float2 acc[R][2 * NV];
 #pragma unroll
       for (int y = 0; y < R; y++)
 #pragma unroll
-        for (int e = 0; e < KH; e++)
-          x[y * KH + e] = fmaf(qv[y].w, kf[e].w, fmaf(qv[y].z, kf[e].z, fmaf(qv[y].y, kf[e].y, qv[y].x * kf[e].x)));
-      S::run(x, gl);
-      const int jg = j + grp * KH;
-      float p[kKeep];
-      bool vis[kKeep], hidden = false, grew = false;
-      float alpha[kOwn];
-#pragma unroll
-      for (int i = 0; i < kKeep; i++) {
-        const int e = (S::base(gl) + i) % KH;
-        vis[i] = ((seen >> e) & 1u) && jg + e <= limit[i / KH < kOwn ? i / KH : 0];
-        hidden = hidden || !vis[i];
-      }
+        for (int h = 0; h < NV; h++) {
+          qv[y][h] = *reinterpret_cast<const float4*>(&s_q[y][d0 + 4 * LPK * h]);
+          acc[y][2 * h] = acc[y][2 * h + 1] = make_float2(0.f, 0.f);
+        }
+      if (x + 1 < ns) read_q(s_seg[x + 1]);
+      float m[kOwn], ref[kOwn], l[kOwn];  // reference, the same or 0 while there is none, sum
+      int limit[kOwn];                    // the last key that each kept score's row attends
 #pragma unroll
       for (int o = 0; o < kOwn; o++) {
-        float mx = m[o];
-#pragma unroll
-        for (int i = 0; i < kKeep; i++)
-          if (kOwn == 1 || i / KH == o) mx = vis[i] ? fmaxf(mx, x[i]) : mx;
-#pragma unroll
-        for (int sh = kRep; sh < kRep * kRowLanes; sh <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, sh));
-        alpha[o] = mx == m[o] ? 1.0f : pow2(m[o] - mx);
-        grew = grew || mx != m[o];
-        const float ref = mx == -INFINITY ? 0.0f : mx;  // no key so far: a NaN score stays one
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kKeep; i++)
-          if (kOwn == 1 || i / KH == o) {
-            p[i] = vis[i] ? pow2(x[i] - ref) : 0.0f;
-            sum += p[i];
-          }
-        l[o] = l[o] * alpha[o] + sum;
-        m[o] = mx;
+        const int y = S::base(gl) / KH + o;
+        limit[o] = y < g.rows ? g.shift + (g.row0 + y) / a.g : -1;
+        m[o] = -INFINITY;
+        ref[o] = l[o] = 0.0f;
       }
-      if (__any_sync(0xffffffffu, grew)) {
-#pragma unroll
-        for (int y = 0; y < R; y++) {
-          const float f = __shfl_sync(0xffffffffu, alpha[(y * KH % kKeep) / KH < kOwn ? (y * KH % kKeep) / KH : 0],
-                                      S::lane_of(y * KH), LPK);
-          acc[y].x *= f; acc[y].y *= f; acc[y].z *= f; acc[y].w *= f;
-        }
-      }
-      // a hidden key's value may be NaN or infinite: it is skipped, not multiplied by 0
-      const bool any_hidden = __any_sync(0xffffffffu, hidden);
-#pragma unroll
-      for (int y = 0; y < R; y++)
+      const int jend = g.jend, open = g.open;
+
+      // Scores, weights and sums of a group's keys from jg on; MASKED: some row attends not all of them.
+      auto compute = [&](auto masked, int jg, const float4* from, unsigned wrong_keys) {
+        constexpr bool MASKED = decltype(masked)::value;
+        float x[V];
 #pragma unroll
         for (int e = 0; e < KH; e++) {
-          const int vi = y * KH + e;
-          const float w = __shfl_sync(0xffffffffu, p[vi % kKeep], S::lane_of(vi), LPK);
-          if (!any_hidden || w != 0.0f) {
-            acc[y].x = fmaf(w, vf[e].x, acc[y].x);
-            acc[y].y = fmaf(w, vf[e].y, acc[y].y);
-            acc[y].z = fmaf(w, vf[e].z, acc[y].z);
-            acc[y].w = fmaf(w, vf[e].w, acc[y].w);
+          float4 kf[NV];
+#pragma unroll
+          for (int h = 0; h < NV; h++) kf[h] = from[(e * NV + h) * 32];
+#pragma unroll
+          for (int y = 0; y < R; y++) {
+            float2 t = __fmul2_rn(make_float2(qv[y][0].x, qv[y][0].y), make_float2(kf[0].x, kf[0].y));
+            t = __ffma2_rn(make_float2(qv[y][0].z, qv[y][0].w), make_float2(kf[0].z, kf[0].w), t);
+#pragma unroll
+            for (int h = 1; h < NV; h++) {
+              t = __ffma2_rn(make_float2(qv[y][h].x, qv[y][h].y), make_float2(kf[h].x, kf[h].y), t);
+              t = __ffma2_rn(make_float2(qv[y][h].z, qv[y][h].w), make_float2(kf[h].z, kf[h].w), t);
+            }
+            x[y * KH + e] = t.x + t.y;
+          }
+        }
+        S::run(x, gl);
+        bool hidden = false, rise = false;
+        if (MASKED) {
+#pragma unroll
+          for (int i = 0; i < kKeep; i++) {
+            const int e = (S::base(gl) + i) % KH;
+            if (jg + e > limit[i / KH < kOwn ? i / KH : 0] || ((wrong_keys >> e) & 1u)) {
+              x[i] = -INFINITY;
+              hidden = true;
+            }
           }
         }
 #pragma unroll
-      for (int e = 0; e < KH; e++) { kf[e] = kn[e]; vf[e] = vn[e]; }
-      seen = seen_next;
-      j += kStride;
-    }
+        for (int i = 0; i < kKeep; i++) rise = rise || x[i] > m[i / KH < kOwn ? i / KH : 0] + kRise;  // never on NaN
+        if (__any_sync(0xffffffffu, rise)) {
+          float alpha[kOwn];
+#pragma unroll
+          for (int o = 0; o < kOwn; o++) {
+            float mx = m[o];
+#pragma unroll
+            for (int i = 0; i < kKeep; i++)
+              if (kOwn == 1 || i / KH == o) mx = fmaxf(mx, x[i]);
+#pragma unroll
+            for (int sh = kRep; sh < kRep * kRowLanes; sh <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, sh));
+            if (mx > m[o] + kRise) {
+              alpha[o] = ex2_sfu(m[o] - mx);
+              m[o] = ref[o] = mx;
+              l[o] *= alpha[o];
+            } else {
+              alpha[o] = 1.0f;
+            }
+          }
+#pragma unroll
+          for (int y = 0; y < R; y++) {
+            const float f = __shfl_sync(0xffffffffu, alpha[(y * KH % kKeep) / KH < kOwn ? (y * KH % kKeep) / KH : 0],
+                                        S::lane_of(y * KH), LPK);
+#pragma unroll
+            for (int h = 0; h < 2 * NV; h++) acc[y][h] = __fmul2_rn(acc[y][h], make_float2(f, f));
+          }
+        }
+        float p[kKeep];
+#pragma unroll
+        for (int i = 0; i < kKeep; i++) {
+          const int o = i / KH < kOwn ? i / KH : 0;
+          p[i] = ex2_sfu(x[i] - ref[o]);  // a NaN score stays one
+          l[o] += p[i];
+        }
+        // a hidden key's value may be NaN or infinite: it is skipped, not multiplied by 0
+        const bool any_hidden = MASKED && __any_sync(0xffffffffu, hidden);
+#pragma unroll
+        for (int e = 0; e < KH; e++) {
+          float4 vf[NV];
+#pragma unroll
+          for (int h = 0; h < NV; h++) vf[h] = from[((KH + e) * NV + h) * 32];
+#pragma unroll
+          for (int y = 0; y < R; y++) {
+            const int vi = y * KH + e;
+            const float w = __shfl_sync(0xffffffffu, p[vi % kKeep], S::lane_of(vi), LPK);
+            if (!any_hidden || w != 0.0f) {
+#pragma unroll
+              for (int h = 0; h < NV; h++) {
+                acc[y][2 * h] = __ffma2_rn(make_float2(w, w), make_float2(vf[h].x, vf[h].y), acc[y][2 * h]);
+                acc[y][2 * h + 1] = __ffma2_rn(make_float2(w, w), make_float2(vf[h].z, vf[h].w), acc[y][2 * h + 1]);
+              }
+            }
+          }
+        }
+      };
 
-    // join the warps' groups
-#pragma unroll
-    for (int o = 0; o < kOwn; o++)
-#pragma unroll
-      for (int sh = kRep; sh < kRep * kRowLanes; sh <<= 1) l[o] += __shfl_xor_sync(0xffffffffu, l[o], sh);
-    __syncthreads();  // the last segment's sums have been read
-    const int part = warp * kGroups + grp;
-#pragma unroll
-    for (int y = 0; y < R; y++) {
-      *reinterpret_cast<float4*>(&s_acc[part][y][d0]) = acc[y];
-      if (gl == S::lane_of(y * KH)) {
-        const int o = (y * KH % kKeep) / KH < kOwn ? (y * KH % kKeep) / KH : 0;
-        s_m[part][y] = m[o];
-        s_l[part][y] = l[o];
+      for (int j = g.j0 + warp * kStep; j < jend; j += kStride) {
+        copy_async_wait<kStages - 2>();
+        const unsigned wrong_keys = (wrong >> (4 * turn)) & 15u;
+        stage(turn == 0 ? kStages - 1 : turn - 1);  // the step before has been read
+        const float4* from = ring + turn * kStage;
+        if (j + kStep <= open && __all_sync(0xffffffffu, wrong_keys == 0)) compute(std::false_type{}, j + grp * KH, from, 0u);
+        else compute(std::true_type{}, j + grp * KH, from, wrong_keys);
+        turn = turn + 1 == kStages ? 0 : turn + 1;
       }
+
+      // join the warp's groups
+#pragma unroll
+      for (int o = 0; o < kOwn; o++)
+#pragma unroll
+        for (int sh = kRep; sh < kRep * kRowLanes; sh <<= 1) l[o] += __shfl_xor_sync(0xffffffffu, l[o], sh);
+#pragma unroll
+      for (int y = 0; y < R; y++) {
+        constexpr int kLast = kOwn - 1;
+        const int o = y * KH % kKeep / KH < kLast ? y * KH % kKeep / KH : kLast;
+        const float my = __shfl_sync(0xffffffffu, m[o], S::lane_of(y * KH), LPK);
+        float ly = __shfl_sync(0xffffffffu, l[o], S::lane_of(y * KH), LPK), M = my;
+#pragma unroll
+        for (int sh = LPK; sh < 32; sh <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, sh));
+        const float f = M == -INFINITY ? 1.0f : ex2_sfu(my - M);
+        ly *= f;
+#pragma unroll
+        for (int h = 0; h < 2 * NV; h++) acc[y][h] = __fmul2_rn(acc[y][h], make_float2(f, f));
+#pragma unroll
+        for (int sh = LPK; sh < 32; sh <<= 1) {
+          ly += __shfl_xor_sync(0xffffffffu, ly, sh);
+#pragma unroll
+          for (int h = 0; h < 2 * NV; h++) {
+            acc[y][h].x += __shfl_xor_sync(0xffffffffu, acc[y][h].x, sh);
+            acc[y][h].y += __shfl_xor_sync(0xffffffffu, acc[y][h].y, sh);
+          }
+        }
+        if (lane == 0) {
+          s_m[warp][y] = M;
+          s_l[warp][y] = ly;
+        }
+      }
+      // ... and the warps
+      float* slot = a.part + (size_t)(2 * c + (c == g.c0 ? 1 : 0)) * kSlot;
+#pragma unroll
+      for (int y0 = 0; y0 < R; y0 += kRound) {
+        if (grp == 0) {
+#pragma unroll
+          for (int y = 0; y < kRound; y++)
+#pragma unroll
+            for (int h = 0; h < NV; h++)
+              *reinterpret_cast<float4*>(&s_acc[warp][y][d0 + 4 * LPK * h]) = make_float4(
+                  acc[y0 + y][2 * h].x, acc[y0 + y][2 * h].y, acc[y0 + y][2 * h + 1].x, acc[y0 + y][2 * h + 1].y);
+        }
+        __syncthreads();
+        if (y0 == 0 && x + 1 < ns) write_q();  // this segment's are in registers
+        if (tid < kRound * kWidth) {
+          const int y = y0 + tid / kWidth, d = tid % kWidth;
+          float M = -INFINITY, A = 0.0f, L = 0.0f;
+#pragma unroll
+          for (int w = 0; w < kRowsWarps; w++) M = fmaxf(M, s_m[w][y]);
+#pragma unroll
+          for (int w = 0; w < kRowsWarps; w++) {
+            const float f = M == -INFINITY ? 1.0f : ex2_sfu(s_m[w][y] - M);
+            L += s_l[w][y] * f;
+            A += s_acc[w][y - y0][d] * f;
+          }
+          if (g.whole) {
+            store(g, y, d, A, L);
+          } else {
+            slot[y * kWidth + d] = A;
+            if (d == 0) { slot[kOut + y] = M; slot[kOut + R + y] = L; }
+          }
+        }
+        __syncthreads();
+      }
+      if (!g.whole) {  // the block's first segment, its last or both
+        if (tid == 0) s_split[splits] = g;
+        splits++;
+      }
+    }
+    copy_async_wait<0>();
+    __syncthreads();  // the list has been read
+  }
+
+  zero_rest(a);
+  if (splits > 0) {
+    __threadfence();
+    __syncthreads();
+    if (tid < splits) {
+      const Seg& g = s_split[tid];
+      s_last[tid] = atomicAdd(&a.tickets[g.c0], 1u) == (unsigned)(g.c1 - g.c0);
+      if (s_last[tid]) a.tickets[g.c0] = 0;
     }
     __syncthreads();
-    const bool whole = tile0 == 0 && tile1 == tiles;
-    const int64_t first_unit = u - tile0, last_unit = first_unit + tiles - 1;  // of this pair, in the whole list
-    const int c0 = (int)(((first_unit + 1) * G - 1) / total), c1 = (int)(((last_unit + 1) * G - 1) / total);
-    auto store = [&](int y, int d, float A, float L) {
-      if (y < nrows && d < a.D) {
-        const int s = (row0 + y) / a.g, h = kvh * a.g + (row0 + y) - s * a.g;
-        a.out[((int64_t)(r.first + s) * a.H + h) * a.D + d] = L == 0.0f ? 0.0f : A / L;
-      }
-    };
-    float* slot = a.part + (size_t)(2 * c + (c == c0 ? 1 : 0)) * kSlot;
-    for (int t = tid; t < R * kWidth; t += kRowsThreads) {
-      const int y = t / kWidth, d = t % kWidth;
-      float M = -INFINITY, A = 0.0f, L = 0.0f;
-#pragma unroll
-      for (int x = 0; x < kParts; x++) M = fmaxf(M, s_m[x][y]);
-#pragma unroll
-      for (int x = 0; x < kParts; x++) {
-        const float f = M == -INFINITY ? 1.0f : pow2(s_m[x][y] - M);
-        L += s_l[x][y] * f;
-        A += s_acc[x][y][d] * f;
-      }
-      if (whole) {
-        store(y, d, A, L);
-      } else {
-        slot[t] = A;
-        if (d == 0) { slot[R * kWidth + y] = M; slot[R * kWidth + R + y] = L; }
-      }
-    }
-    if (!whole) {
+    for (int k = 0; k < splits; k++) {
+      if (!s_last[k]) continue;
+      const Seg& g = s_split[k];
       __threadfence();
-      __syncthreads();
-      if (tid == 0) {
-        s_last = atomicAdd(&a.tickets[c0], 1u) == (unsigned)(c1 - c0);
-        if (s_last) a.tickets[c0] = 0;
-      }
-      __syncthreads();
-      if (s_last) {
-        __threadfence();
-        for (int t = tid; t < R * kWidth; t += kRowsThreads) {
-          const int y = t / kWidth, d = t % kWidth;
-          float M = -INFINITY, A = 0.0f, L = 0.0f;
-          for (int b = c0; b <= c1; b++)
-            M = fmaxf(M, __ldcg(a.part + (size_t)(2 * b + (b == c0 ? 1 : 0)) * kSlot + R * kWidth + y));
-#pragma unroll 4
-          for (int b = c0; b <= c1; b++) {
-            const float* sl = a.part + (size_t)(2 * b + (b == c0 ? 1 : 0)) * kSlot;
-            const float f = M == -INFINITY ? 1.0f : pow2(__ldcg(sl + R * kWidth + y) - M);
-            L += __ldcg(sl + R * kWidth + R + y) * f;
-            A += __ldcg(sl + t) * f;
-          }
-          store(y, d, A, L);
+      for (int t = tid; t < kOut; t += kRowsThreads) {
+        const int y = t / kWidth, d = t % kWidth;
+        float M = -INFINITY, A = 0.0f, L = 0.0f;
+#pragma unroll 8
+        for (int b = g.c0; b <= g.c1; b++)
+          M = fmaxf(M, __ldcg(a.part + (size_t)(2 * b + (b == g.c0 ? 1 : 0)) * kSlot + kOut + y));
+#pragma unroll 8
+        for (int b = g.c0; b <= g.c1; b++) {
+          const float* sl = a.part + (size_t)(2 * b + (b == g.c0 ? 1 : 0)) * kSlot;
+          const float f = M == -INFINITY ? 1.0f : ex2_sfu(__ldcg(sl + kOut + y) - M);
+          L += __ldcg(sl + kOut + R + y) * f;
+          A += __ldcg(sl + t) * f;
         }
+        store(g, y, d, A, L);
       }
     }
-    u += tile1 - tile0;
-    off += tile1 - tile0;
   }
   if (bad_page) atomicExch(a.error_flag, 75);
 }
 
-template <int LPK>
-static cudaError_t launch_rows(const AttnArgs& a, int R, dim3 grid, cudaStream_t stream) {
-  const dim3 block(kRowsThreads);
-  if (R == 1) return launch_pdl(k_paged_rows<1, 4, LPK>, grid, block, 0, stream, a);
-  if (R == 2) return launch_pdl(k_paged_rows<2, 4, LPK>, grid, block, 0, stream, a);
-  if (R == 4) return launch_pdl(k_paged_rows<4, 4, LPK>, grid, block, 0, stream, a);
-  return launch_pdl(k_paged_rows<8, 2, LPK>, grid, block, 0, stream, a);
+template <int R, int LPK, int NV>
+static cudaError_t launch_rows(pai_ctx* ctx, const AttnArgs& a, int grid) {
+  constexpr int bytes = kRowsWarps * kRingBytes;
+  cudaError_t e = smem_limit(ctx, k_paged_rows<R, LPK, NV>, bytes);
+  return e != cudaSuccess ? e : launch_pdl(k_paged_rows<R, LPK, NV>, dim3(grid), dim3(kRowsThreads), bytes, ctx->stream, a);
+}
+
+// Up to four rows a lane holds eight head dims: half the shuffles of four, which bound the kernel otherwise.
+template <int R>
+static cudaError_t launch_rows(pai_ctx* ctx, const AttnArgs& a, int grid) {
+  if (a.D <= 16) return launch_rows<R, 4, 1>(ctx, a, grid);
+  if constexpr (R <= 4) {
+    if (a.D <= 32) return launch_rows<R, 4, 2>(ctx, a, grid);
+    if (a.D <= 64) return launch_rows<R, 8, 2>(ctx, a, grid);
+    return launch_rows<R, 16, 2>(ctx, a, grid);
+  } else {
+    if (a.D <= 32) return launch_rows<R, 8, 1>(ctx, a, grid);
+    if (a.D <= 64) return launch_rows<R, 16, 1>(ctx, a, grid);
+    return launch_rows<R, 32, 1>(ctx, a, grid);
+  }
 }
 
 }  // namespace paged
@@ -398,6 +614,7 @@ PAI_API pai_status pai_sdpa_paged(pai_ctx* ctx, const pai_tensor* q, const pai_t
     };
     a.vec = a.D % 4 == 0 && aligned(*k_cache) && aligned(*v_cache);
     a.q_vec = a.D % 4 == 0 && aligned(*q);
+    a.whole_groups = a.vec && a.page.size % paged::kGroupKeys == 0 && a.pages > 0;
     const int64_t most = (int64_t)a.max_new * a.g;  // rows of one kv head
     const bool tc = most > 8 && paged::tc_fits(a);
     const int R = most <= 1 ? 1 : most <= 2 ? 2 : most <= 4 ? 4 : 8;
@@ -405,18 +622,18 @@ PAI_API pai_status pai_sdpa_paged(pai_ctx* ctx, const pai_tensor* q, const pai_t
     const int64_t groups = (most + R - 1) / R, tiles = std::max<int64_t>(1, ((int64_t)a.max_pages * a.page.size + 63) / 64);
     const int64_t units = std::max<int64_t>(1, (int64_t)a.n * a.KVH) * groups * tiles;
     const int grid = (int)std::min<int64_t>(std::min(ctx->sm_count * paged::kRowsPerSm, kTickets), units);
-    const int lanes = a.D <= 16 ? 4 : a.D <= 32 ? 8 : a.D <= 64 ? 16 : 32;
+    const int width = a.D <= 16 ? 16 : a.D <= 32 ? 32 : a.D <= 64 ? 64 : 128;
     Scratch part;
-    PAI_TRY(scratch(ctx, tc ? paged::tc_part_bytes(ctx) : (size_t)grid * 2 * R * (4 * lanes + 2) * 4, &part));
+    PAI_TRY(scratch(ctx, tc ? paged::tc_part_bytes(ctx) : (size_t)grid * 2 * R * (width + 2) * 4, &part));
     a.part = static_cast<float*>(part.p);
     KernelTimerScope timer(ctx, "attn_paged", 0.0);
     if (tc) {
       PAI_TRY(paged::tc_launch(ctx, a));
     } else {
-      cudaError_t e = lanes == 4    ? paged::launch_rows<4>(a, R, dim3(grid), ctx->stream)
-                      : lanes == 8  ? paged::launch_rows<8>(a, R, dim3(grid), ctx->stream)
-                      : lanes == 16 ? paged::launch_rows<16>(a, R, dim3(grid), ctx->stream)
-                                    : paged::launch_rows<32>(a, R, dim3(grid), ctx->stream);
+      cudaError_t e = R == 1   ? paged::launch_rows<1>(ctx, a, grid)
+                      : R == 2 ? paged::launch_rows<2>(ctx, a, grid)
+                      : R == 4 ? paged::launch_rows<4>(ctx, a, grid)
+                               : paged::launch_rows<8>(ctx, a, grid);
       PAI_PDL_LAUNCH(e, "paged attention");
     }
   }

@@ -23,13 +23,11 @@ struct AttnArgs {
   // part would bend all scores alike, by up to 2^-24 of themselves)
   float scale_hi, scale_lo;
   int vec, q_vec;                          // cache rows, rows of q may be read as float4
+  int whole_groups;                        // ... and no group of keys straddles pages
   float* part;                             // partial results, two slots per block
   unsigned* tickets;                       // arrivals, one counter per block (all zero between launches)
   int* error_flag;
 };
-
-// 2^x with the library's range handling; 2^-inf = 0.
-__device__ __forceinline__ float pow2(float x) { return exp2f(x); }
 
 struct Req {
   int first, n, len;  // first row, new tokens, keys
@@ -37,10 +35,11 @@ struct Req {
 
 // Request i; false when its values are invalid (sets the error flag), n = 0 when it has no new token.
 __device__ __forceinline__ bool load_req(const AttnArgs& a, int i, Req& r) {
+  const float first = a.start[i * a.start_s], last = a.start[(i + 1) * a.start_s], keys = a.len[i * a.len_s];
   int end = 0;
   r.first = r.n = r.len = 0;
-  if (!integral(a.start[i * a.start_s], 0, a.rows, r.first) || !integral(a.start[(i + 1) * a.start_s], 0, a.rows, end) ||
-      !integral(a.len[i * a.len_s], 0, a.max_pages * a.page.size, r.len) || end < r.first || end - r.first > a.max_new) {
+  if (!integral(first, 0, a.rows, r.first) || !integral(last, 0, a.rows, end) ||
+      !integral(keys, 0, a.max_pages * a.page.size, r.len) || end < r.first || end - r.first > a.max_new) {
     return false;
   }
   r.n = end - r.first;
@@ -49,8 +48,9 @@ __device__ __forceinline__ bool load_req(const AttnArgs& a, int i, Req& r) {
 
 // Rows of out that belong to no request are zero.
 __device__ __forceinline__ void zero_rest(const AttnArgs& a) {
+  const float first = a.start[0], last = a.start[a.n * a.start_s];
   int lo, hi;
-  if (!integral(a.start[0], 0, a.rows, lo) || !integral(a.start[a.n * a.start_s], 0, a.rows, hi) || hi < lo) return;
+  if (!integral(first, 0, a.rows, lo) || !integral(last, 0, a.rows, hi) || hi < lo) return;
   const int per = a.H * a.D, rest = lo + (a.rows - hi);
 #pragma unroll 1
   for (int r = blockIdx.x; r < rest; r += gridDim.x) {

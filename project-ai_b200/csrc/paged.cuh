@@ -14,15 +14,19 @@ __device__ __forceinline__ bool integral(float f, int lo, int hi, int& out) {
   return true;
 }
 
-// Division by a page size: a shift for powers of two (shift >= 0), else a plain division.
+// Exact division of 0 <= x < 2^31 by a page size d: with 2^(l-1) < d <= 2^l and m = ceil(2^(31+l) / d) <= 2^32 - 1,
+// x m / 2^(31+l) exceeds x / d by less than x 2^l / (d 2^(31+l)) < 1 / d, which reaches no further integer.
 struct PageDiv {
-  int size, shift;
-  __device__ __forceinline__ int div(int x) const { return shift >= 0 ? x >> shift : x / size; }
+  int size;
+  unsigned mul;
+  int shift;
+  __device__ __forceinline__ int div(int x) const { return (int)(((uint64_t)(unsigned)x * mul) >> shift); }
 };
 inline PageDiv page_div(int size) {
-  int s = 0;
-  while (s < 24 && (1 << s) < size) s++;
-  return PageDiv{size, (1 << s) == size ? s : -1};
+  const uint64_t d = size > 0 ? size : 1;
+  int l = 0;
+  while (1ull << l < d) l++;
+  return PageDiv{size, (unsigned)(((1ull << (31 + l)) + d - 1) / d), 31 + l};
 }
 
 // Exclusive prefix sum of one value per thread over the block, in thread order; total in every thread. `tmp` holds one
