@@ -21,9 +21,9 @@
 //                   this work, 336 cycles per 16 keys, most of it latency; two take 160 each, what the pipes need.)
 //   warps 16-19, 20-23  split K and V: read a raw fp32 tile from shared memory, write hi and lo (SWIZZLE_128B rows of
 //                   64) over it, eight rows at a time;
-//   warp 24         copies raw K and V rows from their pages with bulk copies, up to three tiles ahead;
+//   warp 24         copies raw K rows from their pages with bulk copies, up to three tiles ahead;
 //   warps 25, 26    issue S = Q·Kᵀ and P·V of one query tile each;
-//   warp 27         walks the CTA's share of the work and hands the items to the others.
+//   warp 27         walks the CTA's share of the work, hands the items to the others, and copies V as warp 24 does K.
 // Both query tiles use each converted K and V tile, which halves conversion and shared-memory writes per product. Up to
 // 128 rows there is one query tile: both softmax groups then work on it, each on every second key tile; the second hands
 // its result to the first through TMEM.
@@ -63,6 +63,7 @@ constexpr int kConvWarps = 4;                // for K, and for V
 constexpr int kConvWarp = 2 * kSoftmaxWarps, kLoadWarp = kConvWarp + 2 * kConvWarps, kIssueWarp = kLoadWarp + 1;
 constexpr int kWalkWarp = kIssueWarp + 2;
 constexpr int kTcThreads = 32 * (kWalkWarp + 1);  // seven warpgroups
+constexpr int kMaxGroups = 1;                     // groups of eight rows that a converter takes the maximum of at a time
 constexpr int kItems = 4;                         // items handed out ahead
 // Registers per thread of the softmax, conversion and loading/issuing warpgroups: 4·96 + 2·40 + 40 = 504, what the CTA is
 // launched with (7·72).
@@ -103,7 +104,7 @@ struct TcShared {
   Item items[kItems];
   int64_t tmp[kTcThreads / 32];
   int64_t off;
-  alignas(16) uint32_t seen[kTcRing][4];  // keys of a tile that exist (bit per key)
+  alignas(16) uint32_t seen[2][kTcRing][4];  // [K, V]: keys of a tile that exist (bit per key)
   float row_x[2][2][kTcRows];    // [query tile][half]: what the two threads of a row exchange
   alignas(16) uint32_t max_bits[2][2][kConvWarps];  // converter warps' largest magnitudes; top bit: one is not finite
   float join_m[kTcRows], join_l[kTcRows];        // split items: the second group's maxima and sums
@@ -235,67 +236,6 @@ __device__ __forceinline__ Shape shape_of(const AttnArgs& a, const Req& r) {
   return s;
 }
 
-// Hands out the CTA's share of the units, [u, u1) from unit `off` of request `req` on, as items.
-__device__ __forceinline__ void walk_role(const AttnArgs& a, TcShared& sh, int req, int64_t off, int64_t u, int64_t u1,
-                                          int64_t total) {
-  const int64_t G = min((int64_t)gridDim.x, total);
-  for (int i = 0;; i++) {
-    Item it{};
-    it.stop = 1;
-#pragma unroll 1
-    while (u < u1) {
-      Req r;
-      load_req(a, req, r);
-      const Shape s = shape_of(a, r);
-      if (off >= s.units * a.KVH) {
-        req++;
-        off = 0;
-        continue;
-      }
-      it.kvh = (int)div_pos(off, s.units);
-      int64_t rest = off - it.kvh * s.units;
-      int group = 0, tiles;
-#pragma unroll 1
-      for (;; group++) {
-        tiles = group_tiles(a, r, s.rows, group);
-        if (rest < tiles) break;
-        rest -= tiles;
-      }
-      it.req = req;
-      it.first = r.first;
-      it.shift = r.len - r.n;
-      it.len = r.len;
-      it.row0 = group * 2 * kTcRows;
-      it.rows = s.rows;
-      it.t0 = (int)rest;
-      it.t1 = (int)min((int64_t)tiles, rest + (u1 - u));
-      it.whole = it.t0 == 0 && it.t1 == tiles;
-      it.c0 = (int)div_pos((u - rest + 1) * G - 1, total);
-      it.c1 = (int)div_pos((u - rest + tiles) * G - 1, total);
-      for (int t = 0; t < 2; t++) {
-        const int row0 = it.row0 + t * kTcRows, last = min(s.rows, row0 + kTcRows) - 1;
-        const int keys = it.shift + last / a.g + 1;  // that the tile's last row attends
-        it.end[t] = row0 < s.rows ? max(it.t0, min(it.t1, (keys + kTcKeys - 1) / kTcKeys)) : it.t0;
-      }
-      it.split = it.row0 + kTcRows >= s.rows && it.end[0] - it.t0 >= 2;
-      if (it.split) it.end[1] = it.end[0];
-      it.stop = 0;
-      u += it.t1 - it.t0;
-      off += it.t1 - it.t0;
-      break;
-    }
-    const int slot = i % kItems;
-    if (!wait_bar(&sh.item_free[slot], ((i / kItems) & 1) ^ 1, &sh.abort)) {
-      atomicExch(a.error_flag, 80);
-      sh.abort = 1;
-      return;
-    }
-    sh.items[slot] = it;
-    mbar_arrive(&sh.item_full[slot]);
-    if (it.stop) return;
-  }
-}
-
 // Item i for a whole warp, in shared memory until free_item(); null when there is none. Waits the whole time limit whether
 // another role gave up or not: the warps that meet at named barriers must all see an item or none.
 __device__ __forceinline__ const Item* take_item(TcShared& sh, int i) {
@@ -421,13 +361,13 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
       fence_after();
       // kept finite and above 0: a score of 0 or -inf times it stays one
       const float c = fminf(fmaxf(qdown * sh.scale[0][slot], 1.1754944e-38f), 3.4028235e38f);
-      const uint4 seen = *reinterpret_cast<const uint4*>(sh.seen[slot]);
+      const uint4 seen = *reinterpret_cast<const uint4*>(sh.seen[0][slot]);
       if (t * kTcKeys + kTcKeys - 1 > first_limit || (seen.x & seen.y & seen.z & seen.w) != 0xffffffffu) {
         // scores of keys that do not exist or that the row does not attend become -inf in place
 #pragma unroll 1
         for (int g = 0; g < 4; g++) {
           const int k0 = 64 * half + 16 * g, n = limit - (t * kTcKeys + k0) + 1;
-          const uint32_t vis = (sh.seen[slot][k0 >> 5] >> (k0 & 31)) & (n >= 16 ? 0xffffu : n <= 0 ? 0u : (1u << n) - 1u);
+          const uint32_t vis = (sh.seen[0][slot][k0 >> 5] >> (k0 & 31)) & (n >= 16 ? 0xffffu : n <= 0 ? 0u : (1u << n) - 1u);
           float x[16];
           tc::tmem_ld16(cs + 16 * g, x);
 #pragma unroll
@@ -636,22 +576,23 @@ __device__ __forceinline__ void convert_role(const AttnArgs& a, TcShared& sh, ui
       uint32_t big = 0;
       bool odd = false;
       if (ok && !warp_wait_bar(&sh.raw[op][st], (J / kTcStages) & 1, &sh.abort)) ok = false;
-      const uint32_t seen = sh.seen[slot][warp];  // of the warp's 32 rows
-      const bool have = 4 * tc4 < a.D;
+      const uint32_t seen = sh.seen[op][slot][warp];  // of the warp's 32 rows
       // four elements of row 2 e + tr of group g
-      auto get = [&](int g, int e) {
-        return have && ((seen >> (8 * g + 2 * e + tr)) & 1u) ? *reinterpret_cast<const float4*>(mine + g * kGroup + (2 * e + tr) * 256 + 16 * tc4)
-                                                             : make_float4(0.f, 0.f, 0.f, 0.f);
-      };
+      auto at = [&](int g, int e) -> float4& { return *reinterpret_cast<float4*>(mine + g * kGroup + (2 * e + tr) * 256 + 16 * tc4); };
       if (ok) {
+        if (seen != 0xffffffffu || a.D < kTcDim) {  // nothing was copied there
+#pragma unroll 1
+          for (int e = 0; e < 16; e++)
+            if (4 * tc4 >= a.D || !((seen >> (2 * e + tr)) & 1u)) at(e >> 2, e & 3) = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
         __nv_bfloat162 big2 = __floats2bfloat162_rn(0.0f, 0.0f);  // in bf16: only its exponent counts
 #pragma unroll 1
-        for (int g = 0; g < 4; g++) {
-          float4 x[4];
+        for (int g = 0; g < 4; g += kMaxGroups) {
+          float4 x[4 * kMaxGroups];
 #pragma unroll
-          for (int e = 0; e < 4; e++) x[e] = get(g, e);
+          for (int e = 0; e < 4 * kMaxGroups; e++) x[e] = at(g + e / 4, e % 4);
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
+          for (int e = 0; e < 4 * kMaxGroups; e++) {
             big2 = __hmax2_nan(big2, __habs2(__floats2bfloat162_rn(x[e].x, x[e].y)));
             big2 = __hmax2_nan(big2, __habs2(__floats2bfloat162_rn(x[e].z, x[e].w)));
           }
@@ -663,7 +604,7 @@ __device__ __forceinline__ void convert_role(const AttnArgs& a, TcShared& sh, ui
           big = 0;
 #pragma unroll 1
           for (int g = 0; g < 16; g++) {
-            const float4 x = get(g >> 2, g & 3);
+            const float4 x = at(g >> 2, g & 3);
             const float v[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
             for (int e = 0; e < 4; e++) {
@@ -693,7 +634,7 @@ __device__ __forceinline__ void convert_role(const AttnArgs& a, TcShared& sh, ui
       for (int g = 0; g < 4; g++) {
         float4 x[4];
 #pragma unroll
-        for (int e = 0; e < 4; e++) x[e] = get(g, e);
+        for (int e = 0; e < 4; e++) x[e] = at(g, e);
         if (odd && op == 1) {  // a value that is not finite would spoil the rows that do not attend it, too
 #pragma unroll
           for (int e = 0; e < 4; e++) {
@@ -734,110 +675,184 @@ __device__ __forceinline__ void copies_hold(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-// Copies the raw K and V tiles out of their pages: a page's rows with one bulk copy where they make 1 KB or more (a bulk
-// copy takes some 70 cycles to issue), else 16 bytes at a time, a lane per row.
-__device__ __forceinline__ void load_role(const AttnArgs& a, TcShared& sh, uint8_t* tiles) {
+// Copies the raw K (op 0) or V (op 1) tiles of an item out of their pages, the CTA's tiles J and on: a page's rows with one
+// bulk copy where they make 1 KB or more (a bulk copy takes some 100 cycles to issue), else 16 bytes at a time, a lane per
+// row. False if a wait gave up.
+__device__ __forceinline__ bool load_item(const AttnArgs& a, TcShared& sh, uint8_t* tiles, int op, const Item& it, int& J,
+                                          bool& bad) {
   const int lane = threadIdx.x & 31;
   const int P = a.page.size;
   const bool bulk = a.D == kTcDim && a.c2 == kTcDim && P >= 4;
-  bool ok = true, bad = false, copied_k = false;
-  int J = 0;
-  const Item* p_it;
-  for (int i = 0; ok && (p_it = take_item(sh, i)) != nullptr; free_item(sh, i), i++) {
-    const Item& it = *p_it;
-    const float* trow = a.table + (int64_t)it.req * a.t0;
-    const int64_t head = (int64_t)it.kvh * a.c1;
-    for (int t = it.t0; t < it.t1; t++) {
-      const int st = J % kTcStages, slot = J % kTcRing;
-      const uint32_t parity = ((J / kTcStages) & 1) ^ 1;
-      const int k0 = t * kTcKeys, k1 = min(k0 + kTcKeys, it.len);
-      const int p0 = a.page.div(k0), p1 = k1 > k0 ? a.page.div(k1 - 1) : p0 - 1;
-      uint32_t seen[4] = {0, 0, 0, 0};
-      int count = 0;
+  const float* trow = a.table + (int64_t)it.req * a.t0;
+  const float* src = (op == 0 ? a.k : a.v) + (int64_t)it.kvh * a.c1;
+  const int len = it.len, t1 = it.t1;
+  // the id of the lane's page of a tile (P >= 4: one per lane at most), read a tile ahead
+  auto page_id = [&](int t) -> float {
+    const int pi = a.page.div(t * kTcKeys) + lane;
+    return t < t1 && pi * P < min((t + 1) * kTcKeys, len) ? trow[pi * a.t1] : 0.0f;
+  };
+  float id = page_id(it.t0);
 #pragma unroll 1
-      for (int pi = p0 + lane; pi <= p1; pi += 32) {
-        int page;
-        if (!integral(trow[pi * a.t1], 0, a.pages - 1, page)) {
-          bad = true;
-          continue;
-        }
-        const int lo = max(pi * P, k0) - k0, hi = min((pi + 1) * P, k1) - k0;  // key rows of the tile
-        count += hi - lo;
-#pragma unroll
-        for (int g = 0; g < 4; g++) {
-          const int x0 = max(lo - 32 * g, 0), x1 = min(hi - 32 * g, 32);
-          if (x0 < x1) seen[g] |= (x1 - x0 == 32 ? 0xffffffffu : ((1u << (x1 - x0)) - 1u) << x0);
-        }
-      }
-      count = __reduce_add_sync(0xffffffffu, count);
-#pragma unroll
-      for (int g = 0; g < 4; g++) seen[g] = __reduce_or_sync(0xffffffffu, seen[g]);
-#pragma unroll 1
-      for (int op = 0; op < 2 && ok; op++) {
-        if (!warp_wait_bar(&sh.empty[op][st], parity, &sh.abort)) {
-          ok = false;
-          break;
-        }
-        uint8_t* tile = tiles + (op * kTcStages + st) * kTile;
-        if (lane == 0) {
-          if (op == 0) {
-#pragma unroll
-            for (int g = 0; g < 4; g++) sh.seen[slot][g] = seen[g];
-          }
-          if (bulk) mbar_expect_tx(&sh.raw[op][st], (uint32_t)count * 256);
-        }
-        __syncwarp();
-        copied_k = true;
-        const float* src = (op == 0 ? a.k : a.v) + head;
-        if (bulk) {
-#pragma unroll 1
-          for (int pi = p0 + lane; pi <= p1; pi += 32) {
-            int page;
-            if (!integral(trow[pi * a.t1], 0, a.pages - 1, page)) continue;
-            const int j0 = max(pi * P, k0), j1 = min((pi + 1) * P, k1);
-            bulk_g2s(tile + (uint32_t)(j0 - k0) * 256, src + (int64_t)page * a.c0 + (int64_t)(j0 - pi * P) * a.c2,
-                     (uint32_t)(j1 - j0) * 256, &sh.raw[op][st]);
-          }
+  for (int t = it.t0; t < t1; t++, J++) {
+    const int st = J % kTcStages, slot = J % kTcRing;
+    const int k0 = t * kTcKeys, k1 = min(k0 + kTcKeys, len);
+    const int p0 = a.page.div(k0), p1 = k1 > k0 ? a.page.div(k1 - 1) : p0 - 1;
+    uint32_t seen[4] = {~0u, ~0u, ~0u, ~0u};
+    int to = 0;          // the lane's page's rows start at `to`,
+    uint32_t bytes = 0;  // make this much
+    int64_t from = 0;    // and come from this element on
+    const float ahead = page_id(t + 1);
+    bool whole = k1 - k0 == kTcKeys && P >= 4;
+    if (P >= 4) {
+      const int pi = p0 + lane, lo = max(pi * P, k0), hi = min((pi + 1) * P, k1);
+      int page;
+      if (pi <= p1) {
+        if (integral(id, 0, a.pages - 1, page)) {
+          to = lo - k0;
+          bytes = (uint32_t)(hi - lo) * 256;
+          from = (int64_t)page * a.c0 + (lo - pi * P) * a.c2;
         } else {
-#pragma unroll 1
-          for (int j = k0 + lane; j < k1; j += 32) {
-            const int pi = a.page.div(j);
-            int page;
-            if (!integral(trow[pi * a.t1], 0, a.pages - 1, page)) continue;
-            const float* from = src + (int64_t)page * a.c0 + (int64_t)(j - pi * P) * a.c2;
-            uint8_t* to = tile + (uint32_t)(j - k0) * 256;
-#pragma unroll 4
-            for (int e = 0; e < a.D; e += 4) copy16(to + 4 * e, from + e);
-          }
-          copies_hold(&sh.raw[op][st]);
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.raw[op][st]);
+          bad = true;
+          whole = false;
         }
       }
-      if (!ok) break;
-      J++;
-      copied_k = false;
+    }
+    uint32_t count = kTcKeys;  // rows that exist
+    if (!__all_sync(0xffffffffu, whole)) {
+      count = 0;
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        const int j = k0 + 32 * g + lane;
+        int page;
+        const bool has = j < k1 && integral(trow[a.page.div(j) * a.t1], 0, a.pages - 1, page);
+        if (j < k1 && !has) bad = true;
+        seen[g] = __ballot_sync(0xffffffffu, has);
+        count += __popc(seen[g]);
+      }
+    }
+    id = ahead;
+    if (!warp_wait_bar(&sh.empty[op][st], ((J / kTcStages) & 1) ^ 1, &sh.abort)) return false;
+    uint8_t* tile = tiles + (op * kTcStages + st) * kTile;
+    if (lane == 0) {
+      *reinterpret_cast<uint4*>(sh.seen[op][slot]) = make_uint4(seen[0], seen[1], seen[2], seen[3]);
+      if (bulk) mbar_expect_tx(&sh.raw[op][st], count * 256);
+    }
+    __syncwarp();
+    if (bulk) {
+      if (bytes > 0) bulk_g2s(tile + to * 256, src + from, bytes, &sh.raw[op][st]);
+    } else {
+#pragma unroll 1
+      for (int j = k0 + lane; j < k1; j += 32) {
+        const int pi = a.page.div(j);
+        int page;
+        if (!integral(trow[pi * a.t1], 0, a.pages - 1, page)) continue;
+        const float* row = src + (int64_t)page * a.c0 + (int64_t)(j - pi * P) * a.c2;
+        uint8_t* dst = tile + (uint32_t)(j - k0) * 256;
+#pragma unroll 4
+        for (int e = 0; e < a.D; e += 4) copy16(dst + 4 * e, row + e);
+      }
+      copies_hold(&sh.raw[op][st]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.raw[op][st]);
     }
   }
+  return true;
+}
+// After the last of its J tiles: every product has signalled its stage, or at least every copy has landed, before the CTA
+// may exit.
+__device__ __forceinline__ void load_end(const AttnArgs& a, TcShared& sh, int op, int J, bool ok, bool bad) {
   if (bad) atomicExch(a.error_flag, 75);
-  if (!ok && lane == 0) {
+  if ((threadIdx.x & 31) != 0) return;
+  if (!ok) {
     atomicExch(a.error_flag, 78);
     sh.abort = 1;
   }
-  // every product has signalled its stage, or at least every copy has landed, before the CTA may exit
-  if (lane == 0) {
-    for (int j = max(0, J - kTcStages); j <= J; j++) {
-      for (int op = 0; op < 2; op++) {
-        const int st = j % kTcStages;
-        const uint32_t parity = (j / kTcStages) & 1;
-        if (j == J) {  // a K tile copied without its V tile, when a wait gave up in between
-          if (!ok && copied_k && op == 0) tc::mbar_wait(&sh.raw[0][st], parity);
-        } else if (!wait_bar(&sh.empty[op][st], parity, &sh.abort)) {
-          tc::mbar_wait(&sh.raw[op][st], parity);
-        }
-      }
-    }
+#pragma unroll 1
+  for (int j = max(0, J - kTcStages); j < J; j++) {
+    const int st = j % kTcStages;
+    const uint32_t parity = (j / kTcStages) & 1;
+    if (!wait_bar(&sh.empty[op][st], parity, &sh.abort)) tc::mbar_wait(&sh.raw[op][st], parity);
   }
+}
+__device__ __forceinline__ void load_k_role(const AttnArgs& a, TcShared& sh, uint8_t* tiles) {
+  bool ok = true, bad = false;
+  int J = 0;
+  const Item* it;
+  for (int i = 0; ok && (it = take_item(sh, i)) != nullptr; free_item(sh, i), i++) ok = load_item(a, sh, tiles, 0, *it, J, bad);
+  load_end(a, sh, 0, J, ok, bad);
+}
+
+// Hands out the CTA's share of the units, [u, u1) from unit `off` of request `req` on, as items, and copies their V tiles.
+// An item is published before the V tiles of the one before are copied.
+__device__ __forceinline__ void walk_role(const AttnArgs& a, TcShared& sh, uint8_t* tiles, int req, int64_t off, int64_t u,
+                                          int64_t u1, int64_t total) {
+  const int64_t G = min((int64_t)gridDim.x, total);
+  bool ok = true, bad = false, stopped = false;
+  int J = 0;
+  auto publish = [&](int i) {
+    Item it{};
+    it.stop = 1;
+#pragma unroll 1
+    while (u < u1) {
+      Req r;
+      load_req(a, req, r);
+      const Shape s = shape_of(a, r);
+      if (off >= s.units * a.KVH) {
+        req++;
+        off = 0;
+        continue;
+      }
+      it.kvh = (int)div_pos(off, s.units);
+      int64_t rest = off - it.kvh * s.units;
+      int group = 0, tiles;
+#pragma unroll 1
+      for (;; group++) {
+        tiles = group_tiles(a, r, s.rows, group);
+        if (rest < tiles) break;
+        rest -= tiles;
+      }
+      it.req = req;
+      it.first = r.first;
+      it.shift = r.len - r.n;
+      it.len = r.len;
+      it.row0 = group * 2 * kTcRows;
+      it.rows = s.rows;
+      it.t0 = (int)rest;
+      it.t1 = (int)min((int64_t)tiles, rest + (u1 - u));
+      it.whole = it.t0 == 0 && it.t1 == tiles;
+      it.c0 = (int)div_pos((u - rest + 1) * G - 1, total);
+      it.c1 = (int)div_pos((u - rest + tiles) * G - 1, total);
+      for (int t = 0; t < 2; t++) {
+        const int row0 = it.row0 + t * kTcRows, last = min(s.rows, row0 + kTcRows) - 1;
+        const int keys = it.shift + last / a.g + 1;  // that the tile's last row attends
+        it.end[t] = row0 < s.rows ? max(it.t0, min(it.t1, (keys + kTcKeys - 1) / kTcKeys)) : it.t0;
+      }
+      it.split = it.row0 + kTcRows >= s.rows && it.end[0] - it.t0 >= 2;
+      if (it.split) it.end[1] = it.end[0];
+      it.stop = 0;
+      u += it.t1 - it.t0;
+      off += it.t1 - it.t0;
+      break;
+    }
+    if (!warp_wait_bar(&sh.item_free[i % kItems], ((i / kItems) & 1) ^ 1, &sh.abort)) {
+      if ((threadIdx.x & 31) == 0) atomicExch(a.error_flag, 80);
+      return false;
+    }
+    if ((threadIdx.x & 31) == 0) {
+      sh.items[i % kItems] = it;
+      mbar_arrive(&sh.item_full[i % kItems]);
+    }
+    __syncwarp();
+    stopped = it.stop != 0;
+    return true;
+  };
+  ok = publish(0);
+#pragma unroll 1
+  for (int i = 0; ok && !sh.items[i % kItems].stop; i++) {
+    if (!stopped) ok = publish(i + 1);
+    if (ok) ok = load_item(a, sh, tiles, 1, sh.items[i % kItems], J, bad);
+  }
+  load_end(a, sh, 1, J, ok, bad);
 }
 
 // Issues the products of query tile `tile`; the whole warp runs this. The named barriers that the softmax warps wait at are
@@ -931,7 +946,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_tc(const AttnArgs a) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   TcShared& sh = *reinterpret_cast<TcShared*>(tiles + 2 * kTcStages * kTile);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = tid >> 5;
   if (tid == 0) {
     for (int op = 0; op < 2; op++)
       for (int i = 0; i < kTcStages; i++) {
@@ -997,9 +1012,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_tc(const AttnArgs a) {
       convert_role(a, sh, tiles, (warp - kConvWarp) / kConvWarps);
     } else {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMiscRegs));
-      if (warp == kLoadWarp) load_role(a, sh, tiles);
+      if (warp == kLoadWarp) load_k_role(a, sh, tiles);
       else if (warp < kWalkWarp) issue_role(a, sh, tiles, tmem, warp - kIssueWarp);
-      else if (lane == 0) walk_role(a, sh, sh.req, sh.off, u0, u1, total);
+      else walk_role(a, sh, tiles, sh.req, sh.off, u0, u1, total);
     }
   }
   fence_before();
