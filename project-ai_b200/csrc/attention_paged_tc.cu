@@ -216,10 +216,17 @@ __device__ __forceinline__ void split2(float2 x, uint32_t& hi, uint32_t& lo) {
   lo = pack2(__float22half2_rn(__ffma2_rn(f, make_float2(-1.0f, -1.0f), x)));
 }
 
-// A request's units: per kv head, groups of 256 rows, each with the key tiles that its last row attends.
+// A request's units: per kv head, groups of 256 rows, each with the key tiles that its last row attends. A tile counts as
+// many units as it takes time, 9,000 cycles for two query tiles and 5,900 for one, unless there are so few that a CTA has
+// no more than two: then each counts alike.
+struct Weights {
+  int one, two;  // units of a key tile of a group of one, of two query tiles
+  __device__ __forceinline__ int of(int rows, int group) const { return rows - group * 2 * kTcRows > kTcRows ? two : one; }
+};
 struct Shape {
-  int rows, groups;  // per kv head
-  int64_t units;     // of one kv head
+  int rows, groups;   // per kv head
+  int64_t ones, twos;  // key tiles of one kv head's groups of one and of two query tiles
+  __device__ __forceinline__ int64_t units(const Weights& w) const { return ones * w.one + twos * w.two; }
 };
 __device__ __forceinline__ int group_tiles(const AttnArgs& a, const Req& r, int rows, int group) {
   const int last = min(rows, (group + 1) * 2 * kTcRows) - 1;
@@ -230,9 +237,9 @@ __device__ __forceinline__ Shape shape_of(const AttnArgs& a, const Req& r) {
   Shape s;
   s.rows = r.n * a.g;
   s.groups = (s.rows + 2 * kTcRows - 1) / (2 * kTcRows);
-  s.units = 0;
+  s.ones = s.twos = 0;
 #pragma unroll 1
-  for (int i = 0; i < s.groups; i++) s.units += group_tiles(a, r, s.rows, i);
+  for (int i = 0; i < s.groups; i++) (i + 1 < s.groups || s.rows - i * 2 * kTcRows > kTcRows ? s.twos : s.ones) += group_tiles(a, r, s.rows, i);
   return s;
 }
 
@@ -785,8 +792,7 @@ __device__ __forceinline__ void load_k_role(const AttnArgs& a, TcShared& sh, uin
 // Hands out the CTA's share of the units, [u, u1) from unit `off` of request `req` on, as items, and copies their V tiles.
 // An item is published before the V tiles of the one before are copied.
 __device__ __forceinline__ void walk_role(const AttnArgs& a, TcShared& sh, uint8_t* tiles, int req, int64_t off, int64_t u,
-                                          int64_t u1, int64_t total) {
-  const int64_t G = min((int64_t)gridDim.x, total);
+                                          int64_t u1, int64_t total, int64_t G, const Weights& weights) {
   bool ok = true, bad = false, stopped = false;
   int J = 0;
   auto publish = [&](int i) {
@@ -797,31 +803,41 @@ __device__ __forceinline__ void walk_role(const AttnArgs& a, TcShared& sh, uint8
       Req r;
       load_req(a, req, r);
       const Shape s = shape_of(a, r);
-      if (off >= s.units * a.KVH) {
+      const int64_t units = s.units(weights);
+      if (off >= units * a.KVH) {
         req++;
         off = 0;
         continue;
       }
-      it.kvh = (int)div_pos(off, s.units);
-      int64_t rest = off - it.kvh * s.units;
-      int group = 0, tiles;
+      it.kvh = (int)div_pos(off, units);
+      int64_t rest = off - it.kvh * units;
+      int group = 0, tiles, w;
 #pragma unroll 1
       for (;; group++) {
         tiles = group_tiles(a, r, s.rows, group);
-        if (rest < tiles) break;
-        rest -= tiles;
+        w = weights.of(s.rows, group);
+        if (rest < (int64_t)tiles * w) break;
+        rest -= (int64_t)tiles * w;
       }
+      // the tiles whose first unit is in the share: an earlier share holds that of a tile cut at its start
+      const int64_t base = u - rest;
+      const int t0 = (int)div_pos(rest + w - 1, w);
+      const int t1 = (int)min((int64_t)tiles, div_pos(rest + (u1 - u) + w - 1, w));
+      const int64_t step = min((int64_t)tiles * w - rest, u1 - u);
+      u += step;
+      off += step;
+      if (t0 >= t1) continue;
       it.req = req;
       it.first = r.first;
       it.shift = r.len - r.n;
       it.len = r.len;
       it.row0 = group * 2 * kTcRows;
       it.rows = s.rows;
-      it.t0 = (int)rest;
-      it.t1 = (int)min((int64_t)tiles, rest + (u1 - u));
+      it.t0 = t0;
+      it.t1 = t1;
       it.whole = it.t0 == 0 && it.t1 == tiles;
-      it.c0 = (int)div_pos((u - rest + 1) * G - 1, total);
-      it.c1 = (int)div_pos((u - rest + tiles) * G - 1, total);
+      it.c0 = (int)div_pos((base + 1) * G - 1, total);
+      it.c1 = (int)div_pos((base + (int64_t)(tiles - 1) * w + 1) * G - 1, total);
       for (int t = 0; t < 2; t++) {
         const int row0 = it.row0 + t * kTcRows, last = min(s.rows, row0 + kTcRows) - 1;
         const int keys = it.shift + last / a.g + 1;  // that the tile's last row attends
@@ -830,8 +846,6 @@ __device__ __forceinline__ void walk_role(const AttnArgs& a, TcShared& sh, uint8
       it.split = it.row0 + kTcRows >= s.rows && it.end[0] - it.t0 >= 2;
       if (it.split) it.end[1] = it.end[0];
       it.stop = 0;
-      u += it.t1 - it.t0;
-      off += it.t1 - it.t0;
       break;
     }
     if (!warp_wait_bar(&sh.item_free[i % kItems], ((i / kItems) & 1) ^ 1, &sh.abort)) {
@@ -974,14 +988,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_tc(const AttnArgs a) {
   // this CTA's share of the units
   const int per = (a.n + kTcThreads - 1) / kTcThreads;
   const int i0 = min(a.n, tid * per), i1 = min(a.n, i0 + per);
-  int64_t mine = 0, total;
+  int64_t ones = 0, twos = 0, all_ones, all_twos;
 #pragma unroll 1
   for (int i = i0; i < i1; i++) {
     Req r;
     if (!load_req(a, i, r)) atomicExch(a.error_flag, 74);
-    mine += shape_of(a, r).units * a.KVH;
+    const Shape s = shape_of(a, r);
+    ones += s.ones * a.KVH;
+    twos += s.twos * a.KVH;
   }
-  const int64_t before = block_prefix<kTcThreads>(mine, sh.tmp, total);
+  const int64_t ones_before = block_prefix<kTcThreads>(ones, sh.tmp, all_ones);
+  const int64_t twos_before = block_prefix<kTcThreads>(twos, sh.tmp, all_twos);
+  const bool few = all_ones + all_twos <= 2 * (int64_t)gridDim.x;
+  const Weights weights = few ? Weights{1, 1} : Weights{2, 3};
+  const int64_t mine = ones * weights.one + twos * weights.two, before = ones_before * weights.one + twos_before * weights.two;
+  const int64_t total = all_ones * weights.one + all_twos * weights.two;
+  // with two units or more per tile there are enough for each share to hold some tile's first unit
   const int64_t G = min((int64_t)gridDim.x, total), c = blockIdx.x;
   const int64_t u0 = div_pos(c * total, max(G, (int64_t)1)), u1 = div_pos((c + 1) * total, max(G, (int64_t)1));
   if (c < G && before <= u0 && u0 < before + mine) {
@@ -990,7 +1012,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_tc(const AttnArgs a) {
     for (int i = i0; i < i1; i++) {
       Req r;
       load_req(a, i, r);
-      const int64_t units = shape_of(a, r).units * a.KVH;
+      const int64_t units = shape_of(a, r).units(weights) * a.KVH;
       if (off < units) {
         sh.req = i;
         sh.off = off;
@@ -1014,7 +1036,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_tc(const AttnArgs a) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMiscRegs));
       if (warp == kLoadWarp) load_k_role(a, sh, tiles);
       else if (warp < kWalkWarp) issue_role(a, sh, tiles, tmem, warp - kIssueWarp);
-      else walk_role(a, sh, tiles, sh.req, sh.off, u0, u1, total);
+      else walk_role(a, sh, tiles, sh.req, sh.off, u0, u1, total, G, weights);
     }
   }
   fence_before();
