@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsPerSm) k_paged_rows(const A
     zero_rest(a);
     return;
   }
-  const int64_t u0 = c * total / G, u1 = (c + 1) * total / G;
+  const int64_t u0 = div_pos(c * total, G), u1 = div_pos((c + 1) * total, G);
   // the requests of this thread that have units in the block's share: f(request, its first unit, its first pair, its units)
   auto each = [&](auto f) {
     int64_t ub = before, pb = pairs_before;
@@ -201,8 +201,9 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsPerSm) k_paged_rows(const A
         g.jend = min(tile1 * kUnit, g.shift + (g.row0 + g.rows - 1) / a.g + 1);
         g.open = min(g.jend, g.shift + g.row0 / a.g + 1);
         g.whole = tile0 == 0 && tile1 == tiles;
-        g.c0 = (int)div_pos((at + 1) * G - 1, total);
-        g.c1 = (int)div_pos((at + tiles) * G - 1, total);
+        g.c0 = g.c1 = (int)c;
+        if (at < u0) g.c0 = (int)div_pos((at + 1) * G - 1, total);
+        if (at + tiles > u1) g.c1 = (int)div_pos((at + tiles) * G - 1, total);
         s_seg[pair - p0 - base] = g;
       }
     });
