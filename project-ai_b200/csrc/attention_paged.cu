@@ -314,9 +314,9 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsPerSm) k_paged_rows(const A
 
     read_q(s_seg[0]);
     advance();
-    write_q();
 #pragma unroll
     for (int x = 0; x < kStages - 1; x++) stage(x);
+    write_q();
     __syncthreads();
     int turn = 0;
     for (int x = 0; x < ns; x++) {

@@ -450,6 +450,49 @@ def test_attention_of_many_requests(be, new):
     assert be.check_device_error() == 0
 
 
+@pytest.mark.parametrize("h,new", [(16, 1), (16, 2), (32, 2), (64, 2), (64, 6)])
+@pytest.mark.gpu
+def test_attention_of_more_requests_than_a_block_lists(cuda, h, new):
+    """900 requests of 16 kv heads and a few keys: each block's share is more (request, kv head) pairs than it lists at a
+    time, and some of its requests are empty."""
+    reqs = [((i * 7) % 11, 0 if i % 9 == 4 else 1 + i % new) for i in range(900)]
+    case = paged_case(61, h, 16, 16, 4, reqs, 1)
+    ref, most, rms = attend_ref(*case, 0.25)
+    check_attention(ref, attend(cuda, *case, 0.25, new), 16, 16, np.nanmax(np.abs(case[2])), most, rms)
+    assert cuda.check_device_error() == 0
+
+
+@pytest.mark.gpu
+def test_two_captured_calls_and_eager_ones_share_the_context(cuda):
+    """A captured decode step of split requests and a captured chunk, replayed in turn with eager calls between them."""
+    cases = [paged_case(67, 8, 2, 64, 16, [(3000, 1), (9, 1)]), paged_case(71, 8, 2, 64, 16, [(1200, 90), (700, 1)]),
+             paged_case(73, 8, 2, 64, 16, [(2000, 2)])]
+    refs = [attend_ref(*c, 0.125) for c in cases]
+    held = [[cuda.from_host(x) for x in c] for c in cases]
+    new = [1, 90, 2]
+    graphs = []
+    for i in range(2):
+        cuda.sdpa_paged(*held[i], 0.125, new[i])
+        cuda.graph_begin()
+        out = cuda.sdpa_paged(*held[i], 0.125, new[i])
+        graphs.append((cuda.graph_end(), out))
+
+    def check(i, got):
+        ref, most, rms = refs[i]
+        check_attention(ref, got, 64, 3001, np.nanmax(np.abs(cases[i][2])), most, rms)
+
+    for i in (0, 1, 1, 0, 1, 0):
+        graph, out = graphs[i]
+        cuda.graph_launch(graph)
+        eager = cuda.sdpa_paged(*held[2], 0.125, 2)
+        check(i, cuda.to_host(out))
+        check(2, cuda.to_host(eager))
+        cuda.release(eager)
+    assert cuda.check_device_error() == 0
+    for graph, _ in graphs:
+        cuda.graph_destroy(graph)
+
+
 @pytest.mark.parametrize("new", [2, 90])
 def test_rows_without_keys_and_rows_of_no_request_are_zero(be, new):
     q, kc, vc, table, q_start, kv_len = paged_case(19, 4, 2, 64, 16, [(0, new), (5, 1)], 2)
