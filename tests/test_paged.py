@@ -463,6 +463,23 @@ def test_attention_of_more_requests_than_a_block_lists(cuda, h, new):
 
 
 @pytest.mark.gpu
+def test_attention_of_a_table_of_very_many_positions(cuda):
+    """8192 requests of up to 2^24 positions (one page, over and over), a few of them with keys."""
+    n, h, kvh, d, page = 1 << 13, 4, 2, 16, 4
+    new, length = np.zeros(n, np.int64), np.zeros(n, np.int64)
+    for i, (x, t) in {0: (1, 700), 5: (2, 300), 4000: (1, 256), 4001: (1, 257), n - 1: (2, 1000)}.items():
+        new[i], length[i] = x, t
+    rng = np.random.default_rng(79)
+    kc, vc = (rng.standard_normal((1, kvh, page, d)).astype(np.float32) for _ in range(2))
+    q_start = np.concatenate([[0], np.cumsum(new)])
+    q = rng.standard_normal((int(q_start[-1]), h, d)).astype(np.float32)
+    ref, most, rms = attend_ref(q, kc, vc, np.zeros((n, 250), np.int64), q_start, length, 0.25)
+    table = cabi.broadcast_to(cuda.from_host(np.zeros((1, 1), np.float32)), (n, (1 << 24) // page))
+    check_attention(ref, attend(cuda, q, kc, vc, table, q_start, length, 0.25, 2), d, 1000, np.abs(vc).max(), most, rms)
+    assert cuda.check_device_error() == 0
+
+
+@pytest.mark.gpu
 def test_two_captured_calls_and_eager_ones_share_the_context(cuda):
     """A captured decode step of split requests and a captured chunk, replayed in turn with eager calls between them."""
     cases = [paged_case(67, 8, 2, 64, 16, [(3000, 1), (9, 1)]), paged_case(71, 8, 2, 64, 16, [(1200, 90), (700, 1)]),
