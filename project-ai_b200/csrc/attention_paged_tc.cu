@@ -965,7 +965,8 @@ __device__ __forceinline__ void issue_role(const AttnArgs& a, TcShared& sh, uint
 
 __global__ void __launch_bounds__(kTcThreads, 1) k_paged_tc(const AttnArgs a) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  // an offset, not an address rounded up as an integer: the compiler then knows all of it for shared memory
+  uint8_t* tiles = smem_raw + (-smem_u32(smem_raw) & 1023u);
   TcShared& sh = *reinterpret_cast<TcShared*>(tiles + 2 * kTcStages * kTile);
   const int tid = threadIdx.x, warp = tid >> 5;
   if (tid == 0) {
