@@ -69,7 +69,6 @@ constexpr int kConvWarps = 4;                // for K, and for V
 constexpr int kConvWarp = 2 * kSoftmaxWarps, kLoadWarp = kConvWarp + 2 * kConvWarps, kIssueWarp = kLoadWarp + 1;
 constexpr int kWalkWarp = kIssueWarp + 2;
 constexpr int kTcThreads = 32 * (kWalkWarp + 1);  // seven warpgroups
-constexpr int kMaxGroups = 1;                     // groups of eight rows that a converter takes the maximum of at a time
 constexpr int kItems = 4;                         // items handed out ahead
 // Registers per thread of the softmax, conversion and loading/issuing warpgroups: 4·96 + 2·40 + 40 = 504, what the CTA is
 // launched with (7·72).
@@ -576,103 +575,97 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
 __device__ __forceinline__ void convert_role(const AttnArgs& a, TcShared& sh, uint8_t* tiles, int op) {
   const int warp = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
   const int tr = lane >> 4, tc4 = lane & 15;  // 16 lanes per row, two rows at a time
-  const uint32_t to = tr * 128 + ((tc4 >> 1) << 4) + ((tc4 & 1) << 3);
+  // four elements of the warp's row tr (two rows are 512 bytes), and where their hi parts go: 16-byte chunk c of row r of
+  // eight is stored as chunk c ^ r
+  const uint32_t from = 4 * warp * kGroup + tr * 256 + 16 * tc4;
+  const uint32_t to = 4 * warp * kGroup + ((tr * 128 + ((tc4 >> 1) << 4) + ((tc4 & 1) << 3)) ^ (tr << 4));
   bool ok = true;
-  int J = 0;
+  int J = 0, st = 0, parity = 0;
   const Item* p_it;
   for (int i = 0; (p_it = take_item(sh, i)) != nullptr; i++) {
-    const int n = p_it->t1 - p_it->t0;
+    int n = p_it->t1 - p_it->t0;
     free_item(sh, i);
 #pragma unroll 1
-    for (int k = 0; k < n; k++, J++) {
-      const int st = J % kTcStages, slot = J % kTcRing;
-      uint8_t* mine = tiles + (op * kTcStages + st) * kTile + 4 * warp * kGroup;
+    for (; n > 0; n--) {
+      uint8_t* tile = tiles + (op * kTcStages + st) * kTile;
       uint32_t big = 0;
-      bool odd = false;
-      if (ok && !warp_wait_bar(&sh.raw[op][st], (J / kTcStages) & 1, &sh.abort)) ok = false;
-      const uint32_t seen = sh.seen[op][slot][warp];  // of the warp's 32 rows
-      // four elements of row 2 e + tr of group g
-      auto at = [&](int g, int e) -> float4& { return *reinterpret_cast<float4*>(mine + g * kGroup + (2 * e + tr) * 256 + 16 * tc4); };
+      if (ok && !warp_wait_bar(&sh.raw[op][st], parity, &sh.abort)) ok = false;
       if (ok) {
+        const uint32_t seen = sh.seen[op][J % kTcRing][warp];  // of the warp's 32 rows
         if (seen != 0xffffffffu || a.D < kTcDim) {  // nothing was copied there
 #pragma unroll 1
           for (int e = 0; e < 16; e++)
-            if (4 * tc4 >= a.D || !((seen >> (2 * e + tr)) & 1u)) at(e >> 2, e & 3) = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (4 * tc4 >= a.D || !((seen >> (2 * e + tr)) & 1u))
+              *reinterpret_cast<float4*>(tile + from + e * 512) = make_float4(0.f, 0.f, 0.f, 0.f);
         }
         __nv_bfloat162 big2 = __floats2bfloat162_rn(0.0f, 0.0f);  // in bf16: only its exponent counts
 #pragma unroll 1
-        for (int g = 0; g < 4; g += kMaxGroups) {
-          float4 x[4 * kMaxGroups];
+        for (int g = 0; g < 4; g++) {
+          float4 x[4];
 #pragma unroll
-          for (int e = 0; e < 4 * kMaxGroups; e++) x[e] = at(g + e / 4, e % 4);
+          for (int e = 0; e < 4; e++) x[e] = *reinterpret_cast<const float4*>(tile + from + g * kGroup + e * 512);
 #pragma unroll
-          for (int e = 0; e < 4 * kMaxGroups; e++) {
+          for (int e = 0; e < 4; e++) {
             big2 = __hmax2_nan(big2, __habs2(__floats2bfloat162_rn(x[e].x, x[e].y)));
             big2 = __hmax2_nan(big2, __habs2(__floats2bfloat162_rn(x[e].z, x[e].w)));
           }
         }
         const uint32_t b2 = *reinterpret_cast<const uint32_t*>(&big2);
         big = max(b2 << 16, b2 & 0xffff0000u);
-        odd = !finite_bits(big);
-        if (odd) {  // the largest finite magnitude
+        if (!finite_bits(big)) {  // the largest finite magnitude, and a mark
           big = 0;
 #pragma unroll 1
-          for (int g = 0; g < 16; g++) {
-            const float4 x = at(g >> 2, g & 3);
-            const float v[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-              const uint32_t b = __float_as_uint(v[e]) & 0x7fffffffu;
+          for (int e = 0; e < 16; e++) {
+            float* v = reinterpret_cast<float*>(tile + from + e * 512);
+#pragma unroll 1
+            for (int c = 0; c < 4; c++) {
+              const uint32_t b = __float_as_uint(v[c]) & 0x7fffffffu;
               if (finite_bits(b)) big = max(big, b);
+              else if (op == 1) v[c] = 0.0f;  // it would spoil the rows that do not attend it, too
             }
           }
+          big |= 0x80000000u;
         }
       }
-      big = __reduce_max_sync(0xffffffffu, big);
-      odd = __any_sync(0xffffffffu, odd);
+      const uint32_t odd = __any_sync(0xffffffffu, (int)big < 0) ? 0x80000000u : 0u;
+      big = __reduce_max_sync(0xffffffffu, big & 0x7fffffffu) | odd;
       uint32_t* maxima = sh.max_bits[op][J & 1];  // two sets: a warp may be a tile ahead of one that still reads
-      if (lane == 0) maxima[warp] = big | (odd ? 0x80000000u : 0u);
+      if (lane == 0) maxima[warp] = big;
       bar_named(kBarConv + op, 32 * kConvWarps);
-      if (!ok) continue;
-      const uint4 all = *reinterpret_cast<const uint4*>(maxima);
-      odd = ((all.x | all.y | all.z | all.w) >> 31) != 0;
-      big = max(max(all.x & 0x7fffffffu, all.y & 0x7fffffffu), max(all.z & 0x7fffffffu, all.w & 0x7fffffffu));
-      float up, down;
-      tile_scale(big, up, down);
-      if (warp == 0 && lane == 0) {
-        sh.scale[op][slot] = down;
-        if (op == 1) sh.v_odd[slot] = odd;
-      }
-      const float2 up2 = make_float2(up, up);
+      if (ok) {
+        const uint4 all = *reinterpret_cast<const uint4*>(maxima);
+        float up, down;
+        tile_scale(max(max(all.x & 0x7fffffffu, all.y & 0x7fffffffu), max(all.z & 0x7fffffffu, all.w & 0x7fffffffu)), up, down);
+        if (warp == 0 && lane == 0) {
+          sh.scale[op][J % kTcRing] = down;
+          if (op == 1) sh.v_odd[J % kTcRing] = (all.x | all.y | all.z | all.w) >> 31;
+        }
+        const float2 up2 = make_float2(up, up);
 #pragma unroll 1
-      for (int g = 0; g < 4; g++) {
-        float4 x[4];
+        for (int g = 0; g < 4; g++) {
+          float4 x[4];
 #pragma unroll
-        for (int e = 0; e < 4; e++) x[e] = at(g, e);
-        if (odd && op == 1) {  // a value that is not finite would spoil the rows that do not attend it, too
+          for (int e = 0; e < 4; e++) x[e] = *reinterpret_cast<const float4*>(tile + from + g * kGroup + e * 512);
+          __syncwarp();  // the group's raw rows are in registers
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            if (!isfinite(x[e].x)) x[e].x = 0.0f;
-            if (!isfinite(x[e].y)) x[e].y = 0.0f;
-            if (!isfinite(x[e].z)) x[e].z = 0.0f;
-            if (!isfinite(x[e].w)) x[e].w = 0.0f;
+            uint2 hi, lo;
+            split2(__fmul2_rn(make_float2(x[e].x, x[e].y), up2), hi.x, lo.x);
+            split2(__fmul2_rn(make_float2(x[e].z, x[e].w), up2), hi.y, lo.y);
+            uint8_t* dst = tile + (to ^ (e << 5)) + g * kGroup + e * 256;
+            *reinterpret_cast<uint2*>(dst) = hi;
+            *reinterpret_cast<uint2*>(dst + kLo) = lo;
           }
         }
-        __syncwarp();  // the group's raw rows are in registers
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          uint2 hi, lo;
-          split2(__fmul2_rn(make_float2(x[e].x, x[e].y), up2), hi.x, lo.x);
-          split2(__fmul2_rn(make_float2(x[e].z, x[e].w), up2), hi.y, lo.y);
-          // row r = 2 e + tr: 16-byte chunk c goes to c ^ r
-          uint8_t* dst = mine + g * kGroup + ((to + 2 * e * 128) ^ ((2 * e + tr) << 4));
-          *reinterpret_cast<uint2*>(dst) = hi;
-          *reinterpret_cast<uint2*>(dst + kLo) = lo;
-        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.conv[op][st]);
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.conv[op][st]);
+      J++;
+      if (++st == kTcStages) {
+        st = 0;
+        parity ^= 1;
+      }
     }
   }
   if (!ok && lane == 0) {
