@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsPerSm) k_paged_rows(const A
   __shared__ __align__(16) float s_acc[kRowsWarps][kRound][kWidth];
   __shared__ __align__(16) float s_q[R][kWidth];
   __shared__ float s_m[kRowsWarps][R], s_l[kRowsWarps][R];
-  __shared__ int64_t s_tmp[kRowsWarps];
+  __shared__ int64_t s_tmp[2 * kRowsWarps];
   __shared__ int64_t s_pair[2];
   __shared__ Seg s_seg[kSegs], s_split[2];
   __shared__ int s_last[2];
@@ -135,16 +135,16 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsPerSm) k_paged_rows(const A
   // the block's share of the units
   const int per = (a.n + kRowsThreads - 1) / kRowsThreads;
   const int i0 = min(a.n, tid * per), i1 = min(a.n, i0 + per);
-  int64_t units = 0, pairs = 0, total, all_pairs;
+  int64_t count[2] = {0, 0}, count_before[2], all[2];  // units, pairs (kv head, rows)
   int groups, tiles;
   Req r;
   for (int i = i0; i < i1; i++) {
     if (!load_req(a, i, r)) atomicExch(a.error_flag, 74);
-    units += units_of(r, groups, tiles);
-    pairs += (int64_t)a.KVH * groups;
+    count[0] += units_of(r, groups, tiles);
+    count[1] += (int64_t)a.KVH * groups;
   }
-  const int64_t before = block_prefix<kRowsThreads>(units, s_tmp, total);
-  const int64_t pairs_before = block_prefix<kRowsThreads>(pairs, s_tmp, all_pairs);
+  block_prefix<kRowsThreads>(count, s_tmp, count_before, all);
+  const int64_t total = all[0], before = count_before[0], pairs_before = count_before[1];
   const int64_t G = min((int64_t)gridDim.x, total), c = blockIdx.x;
   if (c >= G) {
     zero_rest(a);
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsPerSm) k_paged_rows(const A
 
   auto store = [&](const Seg& g, int y, int d, float A, float L) {
     if (y < g.rows && d < a.D) {
-      const int s = (g.row0 + y) / a.g, h = g.kvh * a.g + (g.row0 + y) - s * a.g;
+      const int s = a.heads.div(g.row0 + y), h = g.kvh * a.g + (g.row0 + y) - s * a.g;
       a.out[((int64_t)(g.first + s) * a.H + h) * a.D + d] = L == 0.0f ? 0.0f : A / L;
     }
   };
@@ -200,8 +200,8 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsPerSm) k_paged_rows(const A
         g.rows = (int)min((int64_t)R, (int64_t)r.n * a.g - g.row0);
         g.shift = r.len - r.n;
         g.j0 = tile0 * kUnit;
-        g.jend = min(tile1 * kUnit, g.shift + (g.row0 + g.rows - 1) / a.g + 1);
-        g.open = min(g.jend, g.shift + g.row0 / a.g + 1);
+        g.jend = min(tile1 * kUnit, g.shift + a.heads.div(g.row0 + g.rows - 1) + 1);
+        g.open = min(g.jend, g.shift + a.heads.div(g.row0) + 1);
         g.whole = tile0 == 0 && tile1 == tiles;
         g.c0 = g.c1 = (int)c;
         if (at < u0) g.c0 = (int)div_pos((at + 1) * G - 1, total);
@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsPerSm) k_paged_rows(const A
         const int t = tid + i * kRowsThreads, y = t / kWidth, d = t % kWidth;
         qn[i] = 0.0f;
         if (t < kOut && y < g.rows && d < a.D) {
-          const int s = (g.row0 + y) / a.g, head = g.kvh * a.g + (g.row0 + y) - s * a.g;
+          const int s = a.heads.div(g.row0 + y), head = g.kvh * a.g + (g.row0 + y) - s * a.g;
           qn[i] = a.q[(int64_t)(g.first + s) * a.q0 + (int64_t)head * a.q1 + d];
         }
       }
@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsPerSm) k_paged_rows(const A
 #pragma unroll
       for (int o = 0; o < kOwn; o++) {
         const int y = S::base(gl) / KH + o;
-        limit[o] = y < g.rows ? g.shift + (g.row0 + y) / a.g : -1;
+        limit[o] = y < g.rows ? g.shift + a.heads.div(g.row0 + y) : -1;
         m[o] = -INFINITY;
         ref[o] = l[o] = 0.0f;
       }
@@ -600,7 +600,7 @@ PAI_API pai_status pai_sdpa_paged(pai_ctx* ctx, const pai_tensor* q, const pai_t
   a.len = fptr(*kv_len); a.len_s = kv_len->strides[0];
   a.out = fptr(r);
   a.n = table->dims[0]; a.rows = q->dims[0]; a.H = q->dims[1]; a.D = q->dims[2];
-  a.KVH = k_cache->dims[1]; a.g = a.H / a.KVH;
+  a.KVH = k_cache->dims[1]; a.g = a.H / a.KVH; a.heads = paged::page_div(a.g);
   a.pages = k_cache->dims[0]; a.max_pages = table->dims[1];
   a.max_new = max_new > 0 ? std::min(max_new, a.rows) : a.rows;
   a.page = paged::page_div(k_cache->dims[2]);

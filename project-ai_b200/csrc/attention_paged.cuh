@@ -18,7 +18,7 @@ struct AttnArgs {
   const float* len; int64_t len_s;         // kv_len [n]
   float* out;                              // [rows, H, D]
   int n, rows, H, KVH, g, D, max_pages, pages, max_new;
-  PageDiv page;
+  PageDiv page, heads;                     // division by the page size, by g
   // scale * log2(e), so that scores are powers of two, in two parts: q hi + q lo is off by one rounding (a scale in one
   // part would bend all scores alike, by up to 2^-24 of themselves)
   float scale_hi, scale_lo;

@@ -107,7 +107,7 @@ struct TcShared {
   uint64_t s_full[2], pv_full[2], drained[2];  // per query tile
   uint64_t item_full[kItems], item_free[kItems];
   Item items[kItems];
-  int64_t tmp[kTcThreads / 32];
+  int64_t tmp[2 * kTcThreads / 32];
   int64_t off;
   alignas(16) uint32_t seen[2][kTcRing][4];  // [K, V]: keys of a tile that exist (bit per key)
   float row_x[2][2][kTcRows];    // [query tile][half]: what the two threads of a row exchange
@@ -236,7 +236,7 @@ struct Shape {
 };
 __device__ __forceinline__ int group_tiles(const AttnArgs& a, const Req& r, int rows, int group) {
   const int last = min(rows, (group + 1) * 2 * kTcRows) - 1;
-  const int keys = r.len - r.n + last / a.g + 1;  // that the group's last row attends
+  const int keys = r.len - r.n + a.heads.div(last) + 1;  // that the group's last row attends
   return max(1, (keys + kTcKeys - 1) / kTcKeys);
 }
 __device__ __forceinline__ Shape shape_of(const AttnArgs& a, const Req& r) {
@@ -317,9 +317,9 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
     pair_threads = 64 * min(2, quads - (quad & 2));
     const int r = first + row;
     const bool live = r < it.rows;
-    const int s = r / a.g, h = it.kvh * a.g + (r - s * a.g);
+    const int s = a.heads.div(r), h = it.kvh * a.g + (r - s * a.g);
     const int limit = live ? it.shift + s : -1;  // the last key this row attends
-    const int first_limit = it.shift + first / a.g;
+    const int first_limit = it.shift + a.heads.div(first);
     float qdown;  // undoes the row's scale
     {
       const float* p = a.q + (int64_t)(it.first + s) * a.q0 + (int64_t)h * a.q1;
@@ -796,8 +796,12 @@ __device__ __forceinline__ void walk_role(const AttnArgs& a, TcShared& sh, uint8
   bool ok = true, bad = false, stopped = false;
   int J = 0;
   auto publish = [&](int i) {
-    Item it{};
-    it.stop = 1;
+    if (!warp_wait_bar(&sh.item_free[i % kItems], ((i / kItems) & 1) ^ 1, &sh.abort)) {
+      if ((threadIdx.x & 31) == 0) atomicExch(a.error_flag, 80);
+      return false;
+    }
+    Item& it = sh.items[i % kItems];  // every lane writes the same
+    stopped = true;
 #pragma unroll 1
     while (u < u1) {
       Req r;
@@ -821,8 +825,8 @@ __device__ __forceinline__ void walk_role(const AttnArgs& a, TcShared& sh, uint8
       }
       // the tiles whose first unit is in the share: an earlier share holds that of a tile cut at its start
       const int64_t base = u - rest;
-      const int t0 = (int)div_pos(rest + w - 1, w);
-      const int t1 = (int)min((int64_t)tiles, div_pos(rest + (u1 - u) + w - 1, w));
+      auto ceil_w = [&](int x) { return w == 1 ? x : w == 2 ? (x + 1) >> 1 : (x + 2) / 3; };
+      const int t0 = ceil_w((int)rest), t1 = ceil_w((int)min(rest + (u1 - u), (int64_t)tiles * w));
       const int64_t step = min((int64_t)tiles * w - rest, u1 - u);
       u += step;
       off += step;
@@ -836,28 +840,22 @@ __device__ __forceinline__ void walk_role(const AttnArgs& a, TcShared& sh, uint8
       it.t0 = t0;
       it.t1 = t1;
       it.whole = it.t0 == 0 && it.t1 == tiles;
-      it.c0 = (int)div_pos((base + 1) * G - 1, total);
-      it.c1 = (int)div_pos((base + (int64_t)(tiles - 1) * w + 1) * G - 1, total);
+      it.c0 = it.c1 = blockIdx.x;
+      if (t0 > 0) it.c0 = (int)div_pos((base + 1) * G - 1, total);
+      if (t1 < tiles) it.c1 = (int)div_pos((base + (int64_t)(tiles - 1) * w + 1) * G - 1, total);
       for (int t = 0; t < 2; t++) {
         const int row0 = it.row0 + t * kTcRows, last = min(s.rows, row0 + kTcRows) - 1;
-        const int keys = it.shift + last / a.g + 1;  // that the tile's last row attends
+        const int keys = it.shift + a.heads.div(last) + 1;  // that the tile's last row attends
         it.end[t] = row0 < s.rows ? max(it.t0, min(it.t1, (keys + kTcKeys - 1) / kTcKeys)) : it.t0;
       }
       it.split = it.row0 + kTcRows >= s.rows && it.end[0] - it.t0 >= 2;
       if (it.split) it.end[1] = it.end[0];
-      it.stop = 0;
+      stopped = false;
       break;
     }
-    if (!warp_wait_bar(&sh.item_free[i % kItems], ((i / kItems) & 1) ^ 1, &sh.abort)) {
-      if ((threadIdx.x & 31) == 0) atomicExch(a.error_flag, 80);
-      return false;
-    }
-    if ((threadIdx.x & 31) == 0) {
-      sh.items[i % kItems] = it;
-      mbar_arrive(&sh.item_full[i % kItems]);
-    }
+    it.stop = stopped;
     __syncwarp();
-    stopped = it.stop != 0;
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.item_full[i % kItems]);
     return true;
   };
   ok = publish(0);
@@ -989,21 +987,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_tc(const AttnArgs a) {
   // this CTA's share of the units
   const int per = (a.n + kTcThreads - 1) / kTcThreads;
   const int i0 = min(a.n, tid * per), i1 = min(a.n, i0 + per);
-  int64_t ones = 0, twos = 0, all_ones, all_twos;
+  int64_t count[2] = {0, 0}, count_before[2], all[2];  // key tiles of groups of one, of two query tiles
 #pragma unroll 1
   for (int i = i0; i < i1; i++) {
     Req r;
     if (!load_req(a, i, r)) atomicExch(a.error_flag, 74);
     const Shape s = shape_of(a, r);
-    ones += s.ones * a.KVH;
-    twos += s.twos * a.KVH;
+    count[0] += s.ones * a.KVH;
+    count[1] += s.twos * a.KVH;
   }
-  const int64_t ones_before = block_prefix<kTcThreads>(ones, sh.tmp, all_ones);
-  const int64_t twos_before = block_prefix<kTcThreads>(twos, sh.tmp, all_twos);
-  const bool few = all_ones + all_twos <= 2 * (int64_t)gridDim.x;
+  block_prefix<kTcThreads>(count, sh.tmp, count_before, all);
+  const bool few = all[0] + all[1] <= 2 * (int64_t)gridDim.x;
   const Weights weights = few ? Weights{1, 1} : Weights{2, 3};
-  const int64_t mine = ones * weights.one + twos * weights.two, before = ones_before * weights.one + twos_before * weights.two;
-  const int64_t total = all_ones * weights.one + all_twos * weights.two;
+  const int64_t mine = count[0] * weights.one + count[1] * weights.two;
+  const int64_t before = count_before[0] * weights.one + count_before[1] * weights.two;
+  const int64_t total = all[0] * weights.one + all[1] * weights.two;
   // with two units or more per tile there are enough for each share to hold some tile's first unit
   const int64_t G = min((int64_t)gridDim.x, total), c = blockIdx.x;
   const int64_t u0 = div_pos(c * total, max(G, (int64_t)1)), u1 = div_pos((c + 1) * total, max(G, (int64_t)1));

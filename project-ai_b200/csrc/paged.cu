@@ -53,7 +53,7 @@ __device__ __forceinline__ PlanReq plan_req(const PlanArgs& a, int i) {
 
 __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const PlanArgs a) {
   __shared__ int pre[3][kPlanThreads + 1];  // exclusive sums of tokens, pages taken, pages returned over the threads
-  __shared__ int64_t tmp[kPlanThreads / 32];
+  __shared__ int64_t tmp[3 * kPlanThreads / 32];
   pdl_trigger();
   pdl_wait();
   const int tid = threadIdx.x, P = a.page.size;
@@ -69,11 +69,11 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const PlanArgs a) {
   }
   int head = 0, count = 0;
   ok = ok && integral(a.state[0], 0, max(0, a.pages - 1), head) && integral(a.state[a.state_s], 0, a.pages, count);
-  int64_t total[3];
+  int64_t total[3], sums_before[3];
+  block_prefix<kPlanThreads>(sum, tmp, sums_before, total);
 #pragma unroll
   for (int k = 0; k < 3; k++) {
-    const int64_t before = block_prefix<kPlanThreads>(sum[k], tmp, total[k]);
-    pre[k][tid] = (int)min(before, (int64_t)INT32_MAX);
+    pre[k][tid] = (int)min(sums_before[k], (int64_t)INT32_MAX);
     if (tid == kPlanThreads - 1) pre[k][kPlanThreads] = (int)min(total[k], (int64_t)INT32_MAX);
   }
   ok = __syncthreads_and(ok) && total[0] <= a.rows && total[1] <= count && count + total[2] <= a.pages;

@@ -14,7 +14,7 @@ __device__ __forceinline__ bool integral(float f, int lo, int hi, int& out) {
   return true;
 }
 
-// Exact division of 0 <= x < 2^31 by a page size d: with 2^(l-1) < d <= 2^l and m = ceil(2^(31+l) / d) <= 2^32 - 1,
+// Exact division of 0 <= x < 2^31 by d (a page size, the heads of a group): with 2^(l-1) < d <= 2^l and m = ceil(2^(31+l) / d) <= 2^32 - 1,
 // x m / 2^(31+l) exceeds x / d by less than x 2^l / (d 2^(31+l)) < 1 / d, which reaches no further integer.
 struct PageDiv {
   int size;
@@ -29,31 +29,41 @@ inline PageDiv page_div(int size) {
   return PageDiv{size, (unsigned)(((1ull << (31 + l)) + d - 1) / d), 31 + l};
 }
 
-// Exclusive prefix sum of one value per thread over the block, in thread order; total in every thread. `tmp` holds one
-// value per warp.
-template <int THREADS>
-__device__ __forceinline__ int64_t block_prefix(int64_t v, int64_t* tmp, int64_t& total) {
+// Exclusive prefix sums of N values per thread over the block, in thread order; totals in every thread. `tmp` holds N values
+// per warp.
+template <int THREADS, int N>
+__device__ __forceinline__ void block_prefix(const int64_t (&v)[N], int64_t* tmp, int64_t (&before)[N], int64_t (&total)[N]) {
   static_assert(THREADS % 32 == 0 && THREADS <= 1024, "one value per lane for the warps' sums");
   constexpr int kWarps = THREADS / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int64_t x = v;
+  int64_t x[N];
+#pragma unroll
+  for (int k = 0; k < N; k++) x[k] = v[k];
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, x[k], o);
+      if (lane >= o) x[k] += y;
+    }
   }
   __syncthreads();  // tmp may still be read from an earlier call
-  if (lane == 31) tmp[warp] = x;
-  __syncthreads();
-  int64_t w = lane < kWarps ? tmp[lane] : 0;  // every warp sums the warps' sums
 #pragma unroll
-  for (int o = 1; o < kWarps; o <<= 1) {
-    int64_t y = __shfl_up_sync(0xffffffffu, w, o);
-    if (lane >= o) w += y;
+  for (int k = 0; k < N; k++)
+    if (lane == 31) tmp[k * kWarps + warp] = x[k];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < N; k++) {
+    int64_t w = lane < kWarps ? tmp[k * kWarps + lane] : 0;  // every warp sums the warps' sums
+#pragma unroll
+    for (int o = 1; o < kWarps; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += y;
+    }
+    total[k] = __shfl_sync(0xffffffffu, w, kWarps - 1);
+    const int64_t warps = __shfl_sync(0xffffffffu, w, warp > 0 ? warp - 1 : 0);
+    before[k] = (warp > 0 ? warps : 0) + x[k] - v[k];
   }
-  total = __shfl_sync(0xffffffffu, w, kWarps - 1);
-  const int64_t before = __shfl_sync(0xffffffffu, w, warp > 0 ? warp - 1 : 0);
-  return (warp > 0 ? before : 0) + x - v;
 }
 
 // a / b of numbers that are not negative; most fit 32 bits, whose division is several times shorter.
