@@ -5,8 +5,8 @@
 //
 // k_paged_rows serves few query rows per kv head: decode steps and small chunks. It computes in fp32 and reads each key and
 // value once for all the rows of a kv head's group, about two multiply-adds per byte at four rows, so HBM bounds it: 32
-// requests of 2,800 keys, 32 query heads over 8 kv heads of 64 (375 MB), 73 us = 5.1 TB/s, four of 39,000 (639 MB) 124 us.
-// About 7 us of either are its start (reading the requests, listing the share, the first keys: a chain of reads) and its
+// requests of 2,800 keys, 32 query heads over 8 kv heads of 64 (375 MB), 72 us = 5.2 TB/s, four of 39,000 (639 MB) 121 us.
+// About 6 us of either are its start (reading the requests, listing the share, the first keys: a chain of reads) and its
 // end; in between it reads 5.7 to 6 TB/s. Many rows take the tensor-core kernel of attention_paged_tc.cu.
 #include <math.h>
 
@@ -621,8 +621,8 @@ PAI_API pai_status pai_sdpa_paged(pai_ctx* ctx, const pai_tensor* q, const pai_t
     a.whole_groups = a.vec && a.page.size % paged::kGroupKeys == 0 && a.pages > 0;
     // Rows of one kv head: up to 8 the fp32 kernel reads each key once for all of them. Above, it would read keys again
     // for every 8 rows and its multiply-adds bound it; the tensor-core kernel's time hardly depends on the rows up to 128.
-    // Measured, 16 requests of about 1,900 keys, 8 kv heads of 64, us (fp32, tensor cores): 4 rows 44, 72; 8 rows 59, 72;
-    // 12 rows 85, 72; 24 rows 113, 74; 32 rows 145, 75; 12 kv heads, 8 rows 72, 93; 16 rows 112, 93.
+    // Measured, 16 requests of about 1,900 keys, 8 kv heads of 64, us (fp32, tensor cores): 4 rows 45, 65; 8 rows 59, 65;
+    // 12 rows 85, 66; 24 rows 113, 67; 32 rows 143, 68; 12 kv heads, 8 rows 73, 81; 16 rows 112, 81.
     const int64_t most = (int64_t)a.max_new * a.g;
     const bool tc = most > 8 && paged::tc_fits(a);
     const int R = most <= 1 ? 1 : most <= 2 ? 2 : most <= 4 ? 4 : 8;

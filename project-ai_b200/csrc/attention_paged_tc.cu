@@ -26,13 +26,13 @@
 //   warp 27         walks the CTA's share of the work, hands the items to the others, and copies V as warp 24 does K.
 // Both query tiles use each converted K and V tile, which halves conversion and shared-memory writes per product. Up to
 // 128 rows there is one query tile: both softmax groups then work on it, each on every second key tile; the second hands
-// its result to the first through TMEM (six rows of 16 requests: 74 us, 84 with one group; a chunk among decoding requests
-// 142 and 168).
+// its result to the first through TMEM (six new tokens of 16 requests: 68 us, with one group 80; chunks among decoding
+// requests 135 and 155).
 //
-// Measured, 32 query heads over 8 kv heads of 64: four chunks of 2,000 tokens over 2,000 cached ones 0.71 to 0.74 ms, 220 TFLOP/s of
-// results (158 GFLOP), i.e. 660 of fp16 products. A key tile takes 9,000 cycles there: the chain of a query tile (scores 770
-// of tensor work, softmax 4,000, P·V 1,000, the waits between) with the other query tile's in the gaps, and 53% of the issue
-// slots. With one query tile of few rows a key tile takes 5,900, the time to split K and V.
+// Measured, 32 query heads over 8 kv heads of 64: four chunks of 2,000 tokens over 2,000 cached ones 0.66 to 0.70 ms, 227
+// to 240 TFLOP/s of results (158 GFLOP), i.e. 680 to 720 of fp16 products. A key tile takes 8,300 cycles there: the chain of
+// a query tile (scores 770 of tensor work, softmax 4,000, P·V 1,000, the waits between) with the other query tile's in the
+// gaps, and half of the issue slots.
 //
 // Work split: as in k_paged_rows, the (item, key tile) units of all requests in one line, divided evenly over the CTAs;
 // an item that crosses CTAs leaves fp32 partial results that the last of them to finish joins in CTA order.
@@ -222,7 +222,7 @@ __device__ __forceinline__ void split2(float2 x, uint32_t& hi, uint32_t& lo) {
 }
 
 // A request's units: per kv head, groups of 256 rows, each with the key tiles that its last row attends. A tile counts as
-// many units as it takes time, 9,000 cycles for two query tiles and 5,900 for one (chunks among decoding requests 142 us, 158
+// many units as it takes time, about 8,300 cycles for two query tiles, 5,300 for one (chunks among decoding requests 135 us, 151
 // when all count alike), unless there are so few that a CTA has no more than two: then each counts alike, so that more
 // CTAs have one (small heads, 131 new tokens of 5 requests: 34 us, 40 with weights).
 struct Weights {
@@ -684,7 +684,7 @@ __device__ __forceinline__ void copies_hold(uint64_t* bar) {
 
 // Copies the raw K (op 0) or V (op 1) tiles of an item out of their pages, the CTA's tiles J and on: a page's rows with one
 // bulk copy where they make 1 KB or more (a bulk copy takes some 100 cycles to issue), else 16 bytes at a time, a lane per
-// row: six new tokens of 16 requests, pages of 16 or 8 positions 74 us, of 4 75, by 16 bytes 84 to 86. False if a wait gave up.
+// row: six new tokens of 16 requests, pages of 16 or 8 positions 67 us, of 4 69; 16 bytes at a time 76. False if a wait gave up.
 __device__ __forceinline__ bool load_item(const AttnArgs& a, TcShared& sh, uint8_t* tiles, int op, const Item& it, int& J,
                                           bool& bad) {
   const int lane = threadIdx.x & 31;
