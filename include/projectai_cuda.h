@@ -269,8 +269,9 @@ pai_status pai_paged_plan(pai_ctx* ctx, const pai_tensor* lengths, const pai_ten
  * full [T, D] tables (RotaryEmbedding's values); q goes to the new tensor q_out [rows, H, D], and k, with v copied, to
  * `slots` [rows] of the caches. Rows of slot -1 write nothing to the caches (their q is still rotated). A slot outside
  * [-1, pages * P) sets the error flag and writes nothing; a position outside the tables too, and its row of q_out is
- * 0. Slots other than -1 must differ from one another (pai_paged_plan's do): of two rows with one slot, each element
- * that the cache ends up with is one of theirs. q, k and v rows may be strided (unit head-dim stride). */
+ * 0. The tables have 2^24 rows at most. Slots other than -1 must differ from one another (pai_paged_plan's do): of two
+ * rows with one slot, each element that the cache ends up with is one of theirs. q, k and v rows may be strided (unit
+ * head-dim stride). */
 pai_status pai_paged_rope_append(pai_ctx* ctx, const pai_tensor* q, const pai_tensor* k, const pai_tensor* v,
                                  const pai_tensor* cos_table, const pai_tensor* sin_table, const pai_tensor* positions,
                                  const pai_tensor* slots, const pai_tensor* k_cache, const pai_tensor* v_cache,

@@ -84,6 +84,10 @@ inline pai_status check_append(Fail fail, const pai_tensor* q, const pai_tensor*
   if (d % 2) return fail(PAI_ERR_ARGUMENT, "PagedRopeAppend: odd head dim %d", d);
   if (cos_table->dims[1] != d || sin_table->dims[1] != d || sin_table->dims[0] != cos_table->dims[0])
     return fail(PAI_ERR_ARGUMENT, "PagedRopeAppend: tables must be [T, %d]", d);
+  // a longer table's last row would round up to one behind it where positions are compared with it
+  if (cos_table->dims[0] > kMaxIndex)
+    return fail(PAI_ERR_UNSUPPORTED, "PagedRopeAppend: tables of %d rows: above 2^24, F32 holds no exact positions",
+                cos_table->dims[0]);
   if (q->strides[2] != 1 || k->strides[2] != 1 || v->strides[2] != 1 || cos_table->strides[1] != 1 ||
       sin_table->strides[1] != 1 || (cos_table->dims[0] > 1 && cos_table->strides[0] != sin_table->strides[0]))
     return fail(PAI_ERR_UNSUPPORTED, "PagedRopeAppend: rows must be contiguous and the tables share one layout");

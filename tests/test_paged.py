@@ -330,6 +330,23 @@ def test_append_refusals(be):
         call(q=cabi.transpose(be.from_host(rnd(1, 3, d, 4)), 1, 2))
 
 
+def test_append_refuses_tables_whose_rows_f32_cannot_name(be):
+    """Beyond 2^24 rows the largest position rounds up to one behind the table: 2^24 + 4 rows, position 2^24 + 4."""
+    d, rows = 16, (1 << 24) + 4
+    kc, vc = be.from_host(rnd(4, 2, 1, 4, d)), be.from_host(rnd(5, 2, 1, 4, d))
+    args = [be.from_host(rnd(s, 1, n, d)) for s, n in ((1, 2), (2, 1), (3, 1))]
+    one = be.from_host(rnd(6, 1, d))
+    for n in (rows, 1 << 24):
+        wide = cabi.broadcast_to(one, (n, d))
+        call = lambda: be.paged_rope_append(*args, wide, wide, be.from_host([(1 << 24) - 1.0]), be.from_host([1.0]), kc, vc)  # noqa: E731
+        if n > 1 << 24:
+            with pytest.raises(UnsupportedError):
+                call()
+        else:
+            call()
+    assert be.check_device_error() == 0
+
+
 # ---------------------------------------------------------------- attention
 def attend_ref(q, kc, vc, table, q_start, kv_len, scale):
     """float64, row by row; also max and root mean square of sum |q||k| scale for the tolerance."""
