@@ -278,14 +278,14 @@ pai_status pai_paged_rope_append(pai_ctx* ctx, const pai_tensor* q, const pai_te
                                  pai_tensor* q_out);
 /* Causal attention of a step's new tokens over their requests' pages, the values of pai_sdpa_fwd per request: row r of
  * request i stands at position p = kv_len[i] - (q_start[i+1] - q_start[i]) + (r - q_start[i]) and attends positions 0
- * .. p of table's row i. q [rows, H, D] (any strides, unit along D), H % KVH == 0, D <= 128; out [rows, H, D]. Rows
- * without a key (p < 0) and rows that belong to no request are 0. max_new bounds the new tokens of one request (0:
- * rows is taken); it is a host value because the kernels and their launch sizes are chosen by it. One long chunk and
- * many single tokens may share a call. Cache positions that a row does not attend may hold anything, NaN and
- * infinities included; a row that attends such a key or value is not finite or unspecified. A q_start that does not
- * rise or leaves [0, rows], a kv_len outside [0, max_pages * P] or a request of more than max_new tokens sets the
- * error flag and the request is skipped (its rows of out are unspecified); a page id outside the caches sets it too,
- * and its positions are not attended. */
+ * .. p of table's row i. q [rows, H, D] (any strides, unit along D), H % KVH == 0, D <= 128, rows * H <= 2^30; out
+ * [rows, H, D]. Rows without a key (p < 0) and rows that belong to no request are 0. max_new bounds the new tokens of
+ * one request (0: rows is taken); it is a host value because the kernels and their launch sizes are chosen by it. One
+ * long chunk and many single tokens may share a call. Cache positions that a row does not attend may hold anything,
+ * NaN and infinities included; a row that attends such a key or value is not finite or unspecified. A q_start that
+ * does not rise or leaves [0, rows], a kv_len outside [0, max_pages * P] or a request of more than max_new tokens sets
+ * the error flag and the request is skipped (its rows of out are unspecified); a page id outside the caches sets it
+ * too, and its positions are not attended. */
 pai_status pai_sdpa_paged(pai_ctx* ctx, const pai_tensor* q, const pai_tensor* k_cache, const pai_tensor* v_cache,
                           const pai_tensor* table, const pai_tensor* q_start, const pai_tensor* kv_len, float scale,
                           int32_t max_new, pai_tensor* out);

@@ -626,10 +626,10 @@ PAI_API pai_status pai_sdpa_paged(pai_ctx* ctx, const pai_tensor* q, const pai_t
     const int64_t most = (int64_t)a.max_new * a.g;
     const bool tc = most > 8 && paged::tc_fits(a);
     const int R = most <= 1 ? 1 : most <= 2 ? 2 : most <= 4 ? 4 : 8;
-    // no more blocks than units there can be
+    // no more blocks than units there can be (a bound on them may pass 64 bits, not a double's range)
     const int64_t groups = (most + R - 1) / R, tiles = std::max<int64_t>(1, ((int64_t)a.max_pages * a.page.size + 63) / 64);
-    const int64_t units = std::max<int64_t>(1, (int64_t)a.n * a.KVH) * groups * tiles;
-    const int grid = (int)std::min<int64_t>(std::min(ctx->sm_count * paged::kRowsPerSm, kTickets), units);
+    const double units = std::max(1.0, (double)a.n * a.KVH) * (double)groups * (double)tiles;
+    const int grid = (int)std::min((double)std::min(ctx->sm_count * paged::kRowsPerSm, kTickets), units);
     const int width = a.D <= 16 ? 16 : a.D <= 32 ? 32 : a.D <= 64 ? 64 : 128;
     Scratch part;
     PAI_TRY(scratch(ctx, tc ? paged::tc_part_bytes(ctx) : (size_t)grid * 2 * R * (width + 2) * 4, &part));

@@ -14,6 +14,8 @@ typedef pai_status (*Fail)(pai_status, const char*, ...);
 // F32 holds every integer up to 2^24: the bound on slots, positions and rows.
 constexpr int64_t kMaxIndex = 1 << 24;
 constexpr int kMaxHeadDim = 128;
+// rows x heads of one attention call, and its requests: the kernels count them, rounded up to their tiles, in 32 bits.
+constexpr int64_t kMaxQueryRows = 1 << 30;
 
 // An in-place operand: no two elements at one address by a zero stride.
 inline bool writable(const pai_tensor& t) {
@@ -116,6 +118,8 @@ inline pai_status check_sdpa(Fail fail, const pai_tensor* q, const pai_tensor* k
   if (q->dims[0] > kMaxIndex || (int64_t)table->dims[1] * k_cache->dims[2] > kMaxIndex)
     return fail(PAI_ERR_UNSUPPORTED, "SdpaPaged: %d rows, %d pages of %d positions per request: above 2^24, F32 holds no exact positions",
                 q->dims[0], table->dims[1], k_cache->dims[2]);
+  if ((int64_t)q->dims[0] * h > kMaxQueryRows || n > kMaxQueryRows)
+    return fail(PAI_ERR_UNSUPPORTED, "SdpaPaged: %d rows of %d heads, %d requests: above 2^30", q->dims[0], h, n);
   return PAI_OK;
 }
 

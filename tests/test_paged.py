@@ -694,6 +694,24 @@ def test_attention_refusals(be):
         call(table=cabi.broadcast_to(be.from_host(np.zeros((1, 1), np.float32)), (2, (1 << 22) + 1)))
 
 
+def test_attention_refuses_more_query_rows_than_32_bits_count(be):
+    """rows x H counts query rows in 32 bits: 2^24 rows of 128 heads would wrap to a negative row. A batch whose tables
+    could hold 2^63 pieces of work and more is no error: its launch is bounded."""
+    one = be.from_host(np.zeros((1, 1, 1), np.float32))
+    kc, vc = be.from_host(rnd(1, 2, 1, 4, 1)), be.from_host(rnd(2, 2, 1, 4, 1))
+    with pytest.raises(UnsupportedError):
+        be.sdpa_paged(cabi.broadcast_to(one, (1 << 24, 128, 1)), kc, vc, *map(be.from_host, ([[0.0]], [0.0, 0.0], [0.0])), 1.0, 1)
+    with pytest.raises(UnsupportedError):
+        be.sdpa_paged(cabi.broadcast_to(one, (1 << 24, 128, 1)), kc, vc, *map(be.from_host, ([[0.0]], [0.0, 0.0], [0.0])), 1.0, 0)
+    kc, vc = be.from_host(rnd(1, 2, 64, 4, 1)), be.from_host(rnd(2, 2, 64, 4, 1))
+    n, rows = 1 << 23, 1 << 20
+    zero = be.from_host(np.zeros(1, np.float32))
+    table = cabi.broadcast_to(be.from_host(np.zeros((1, 1), np.float32)), (n, 1 << 22))
+    out = be.sdpa_paged(cabi.broadcast_to(one, (rows, 64, 1)), kc, vc, table, cabi.broadcast_to(zero, (n + 1,)), cabi.broadcast_to(zero, (n,)), 1.0, 0)
+    assert not be.to_host(out).any()
+    assert be.check_device_error() == 0
+
+
 # ---------------------------------------------------------------- the operators together
 class Server:
     """Steps of a server over one layer: plan, append, attend, with the dense float64 history beside it."""
