@@ -284,8 +284,8 @@ pai_status pai_paged_rope_append(pai_ctx* ctx, const pai_tensor* q, const pai_te
  * long chunk and many single tokens may share a call. Cache positions that a row does not attend may hold anything,
  * NaN and infinities included; a row that attends such a key or value is not finite or unspecified. A q_start that
  * does not rise or leaves [0, rows], a kv_len outside [0, max_pages * P] or a request of more than max_new tokens sets
- * the error flag and the request is skipped (its rows of out are unspecified); a page id outside the caches sets it
- * too, and its positions are not attended. */
+ * the error flag and the request is skipped (its rows of out are unspecified, and where q_start is wrong those of no
+ * request too); a page id outside the caches sets it too, and its positions are not attended. */
 pai_status pai_sdpa_paged(pai_ctx* ctx, const pai_tensor* q, const pai_tensor* k_cache, const pai_tensor* v_cache,
                           const pai_tensor* table, const pai_tensor* q_start, const pai_tensor* kv_len, float scale,
                           int32_t max_new, pai_tensor* out);

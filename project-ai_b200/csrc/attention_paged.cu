@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsPerSm) k_paged_rows(const A
   __shared__ int64_t s_tmp[2 * kRowsWarps];
   __shared__ int64_t s_pair[2];
   __shared__ Seg s_seg[kSegs], s_split[2];
-  __shared__ int s_last[2];
+  __shared__ int s_last[2], s_unplaced;  // a row range is invalid
   pdl_trigger();
   pdl_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -138,16 +138,21 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsPerSm) k_paged_rows(const A
   int64_t count[2] = {0, 0}, count_before[2], all[2];  // units, pairs (kv head, rows)
   int groups, tiles;
   Req r;
+  bool placed = true;
+  if (tid == 0) s_unplaced = 0;  // set behind block_prefix's barriers
   for (int i = i0; i < i1; i++) {
     if (!load_req(a, i, r)) atomicExch(a.error_flag, 74);
+    placed = placed && r.placed;
     count[0] += units_of(r, groups, tiles);
     count[1] += (int64_t)a.KVH * groups;
   }
   block_prefix<kRowsThreads>(count, s_tmp, count_before, all);
+  if (!placed) s_unplaced = 1;
   const int64_t total = all[0], before = count_before[0], pairs_before = count_before[1];
   const int64_t G = min((int64_t)gridDim.x, total), c = blockIdx.x;
   if (c >= G) {
-    zero_rest(a);
+    __syncthreads();
+    if (!s_unplaced) zero_rest(a);
     return;
   }
   const int64_t u0 = div_pos(c * total, G), u1 = div_pos((c + 1) * total, G);
@@ -518,7 +523,7 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsPerSm) k_paged_rows(const A
     __syncthreads();  // the list has been read
   }
 
-  zero_rest(a);
+  if (!s_unplaced) zero_rest(a);
   if (splits > 0) {
     __threadfence();
     __syncthreads();

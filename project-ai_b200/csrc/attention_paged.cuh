@@ -31,6 +31,7 @@ struct AttnArgs {
 
 struct Req {
   int first, n, len;  // first row, new tokens, keys
+  bool placed;        // its row range is valid
 };
 
 // Request i; false when its values are invalid (sets the error flag), n = 0 when it has no new token.
@@ -38,19 +39,18 @@ __device__ __forceinline__ bool load_req(const AttnArgs& a, int i, Req& r) {
   const float first = a.start[i * a.start_s], last = a.start[(i + 1) * a.start_s], keys = a.len[i * a.len_s];
   int end = 0;
   r.first = r.n = r.len = 0;
-  if (!integral(first, 0, a.rows, r.first) || !integral(last, 0, a.rows, end) ||
-      !integral(keys, 0, a.max_pages * a.page.size, r.len) || end < r.first || end - r.first > a.max_new) {
-    return false;
-  }
+  r.placed = integral(first, 0, a.rows, r.first) && integral(last, 0, a.rows, end) && end >= r.first;
+  if (!r.placed || !integral(keys, 0, a.max_pages * a.page.size, r.len) || end - r.first > a.max_new) return false;
   r.n = end - r.first;
   return true;
 }
 
-// Rows of out that belong to no request are zero.
+// Rows of out that belong to no request are zero: those before the first request and behind the last, when all row ranges
+// are valid (else a row behind the last range may be another request's).
 __device__ __forceinline__ void zero_rest(const AttnArgs& a) {
   const float first = a.start[0], last = a.start[a.n * a.start_s];
   int lo, hi;
-  if (!integral(first, 0, a.rows, lo) || !integral(last, 0, a.rows, hi) || hi < lo) return;
+  if (!integral(first, 0, a.rows, lo) || !integral(last, 0, a.rows, hi)) return;
   const int per = a.H * a.D, rest = lo + (a.rows - hi);
 #pragma unroll 1
   for (int r = blockIdx.x; r < rest; r += gridDim.x) {

@@ -116,6 +116,7 @@ struct TcShared {
   float scale[2][kTcRing];       // what a product with the tile is multiplied by to undo the tile's scale
   int v_odd[kTcRing];            // a V tile held values that are not finite
   int req;
+  int unplaced;                  // a row range is invalid
   volatile int abort;
   int last[2];
   uint32_t tmem;
@@ -977,12 +978,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_tc(const AttnArgs a) {
       mbar_init(&sh.drained[t], 1);
     }
     sh.abort = 0;
+    sh.unplaced = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 0) tc::tmem_alloc(&sh.tmem, 512);
   pdl_trigger();
   pdl_wait();
-  zero_rest(a);
+  __syncthreads();  // `unplaced` is set below
 
   // this CTA's share of the units
   const int per = (a.n + kTcThreads - 1) / kTcThreads;
@@ -992,11 +994,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_tc(const AttnArgs a) {
   for (int i = i0; i < i1; i++) {
     Req r;
     if (!load_req(a, i, r)) atomicExch(a.error_flag, 74);
+    if (!r.placed) sh.unplaced = 1;
     const Shape s = shape_of(a, r);
     count[0] += s.ones * a.KVH;
     count[1] += s.twos * a.KVH;
   }
   block_prefix<kTcThreads>(count, sh.tmp, count_before, all);
+  if (!sh.unplaced) zero_rest(a);
   const bool few = all[0] + all[1] <= 2 * (int64_t)gridDim.x;
   const Weights weights = few ? Weights{1, 1} : Weights{2, 3};
   const int64_t mine = count[0] * weights.one + count[1] * weights.two;

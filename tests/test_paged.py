@@ -694,6 +694,19 @@ def test_attention_refusals(be):
         call(table=cabi.broadcast_to(be.from_host(np.zeros((1, 1), np.float32)), (2, (1 << 22) + 1)))
 
 
+@pytest.mark.parametrize("new", [3, 40])
+def test_a_contradicting_row_range_leaves_the_other_requests_rows(be, new):
+    """q_start falls behind the first request's end: its last rows are its own, not rows behind the last request."""
+    q, kc, vc, table, _, _ = paged_case(83, 4, 2, 64, 16, [(70, new), (7, 1)], 2, stale=0.0)
+    start = np.array([0, new, new - 2], np.float32)
+    ref, most, rms = attend_ref(q[:new], kc, vc, table[:1], [0, new], [70 + new], 0.125)
+    for _ in range(5):
+        got = attend(be, q, kc, vc, table, start, [70.0 + new, 8.0], 0.125, new)
+        check_attention(ref, got[:new], 64, 70 + new, np.abs(vc).max(), most, rms)
+        with pytest.raises(DeviceTimeoutError):
+            be.check_device_error()
+
+
 def test_attention_refuses_more_query_rows_than_32_bits_count(be):
     """rows x H counts query rows in 32 bits: 2^24 rows of 128 heads would wrap to a negative row. A batch whose tables
     could hold 2^63 pieces of work and more is no error: its launch is bounded."""
