@@ -282,10 +282,13 @@ pai_status pai_paged_rope_append(pai_ctx* ctx, const pai_tensor* q, const pai_te
  * [rows, H, D]. Rows without a key (p < 0) and rows that belong to no request are 0. max_new bounds the new tokens of
  * one request (0: rows is taken); it is a host value because the kernels and their launch sizes are chosen by it. One
  * long chunk and many single tokens may share a call. Cache positions that a row does not attend may hold anything,
- * NaN and infinities included; a row that attends such a key or value is not finite or unspecified. A q_start that
- * does not rise or leaves [0, rows], a kv_len outside [0, max_pages * P] or a request of more than max_new tokens sets
- * the error flag and the request is skipped (its rows of out are unspecified, and where q_start is wrong those of no
- * request too); a page id outside the caches sets it too, and its positions are not attended. */
+ * NaN and infinities included; a row that attends such a key or value, or has scores beyond F32's range, is not finite
+ * or unspecified. Finite numbers may lie as far apart as F32 allows: each number of q and the caches counts as in F32
+ * products, with an error of up to 2^-21 of the largest of its group of four adjacent head dims; weights under 2^-100
+ * of a row's largest may count as 0. A q_start that does not rise or leaves [0, rows], a kv_len outside [0, max_pages
+ * * P] or a request of more than max_new tokens sets the error flag and the request is skipped (its rows of out are
+ * unspecified, and where q_start is wrong those of no request too); a page id outside the caches sets it too, and its
+ * positions are not attended. */
 pai_status pai_sdpa_paged(pai_ctx* ctx, const pai_tensor* q, const pai_tensor* k_cache, const pai_tensor* v_cache,
                           const pai_tensor* table, const pai_tensor* q_start, const pai_tensor* kv_len, float scale,
                           int32_t max_new, pai_tensor* out);

@@ -2,15 +2,27 @@
 // (attention_paged.cu) is good for, i.e. chunks of new tokens.
 //
 // Arithmetic. A product of fp32 numbers is taken as three fp16 products: with x = hi + lo, hi = fp16(x) and
-// lo = fp16(x - hi), x·y = hi·hi' + hi·lo' + lo·hi' up to 3·2^-22 relative, accumulated in fp32 by the tensor cores.
-// fp16 holds 2^-24 .. 65504, so operands are first scaled by powers of two (exact) that bring the largest magnitude of
-// a query row, or of a tile of 128 keys or values, to [2^13, 2^14); numbers far below that lose relative precision
-// only under 2^-39 of the largest. The scales come out again in a factor that the softmax and the sum over tiles
-// multiply by anyway. Weights exp(s - m) are taken against a reference m that follows the row maximum only when that has
-// risen by 2^9, so that sums need a rescale rarely, and carry a factor 2^6 in numerator and denominator: they stay under
-// 2^15, and their remainders lose nothing above 2^-31 of a typical largest one. This is half
-// the tensor time of three TF32 products and half the shared memory. Per tile of keys the product P·V goes to its own
-// accumulator and is added to fp32 registers, so the tensor cores' sums stay short (24 steps).
+// lo = fp16(x - hi), x·y = hi·hi' + hi·lo' + lo·hi' up to 3·2^-22 relative, accumulated in fp32 by the tensor cores. This
+// is half the tensor time of three TF32 products and half the shared memory, but fp16 holds only 2^-24 .. 65504. So
+//   q, K, V  are scaled by powers of two (exact) that bring the largest magnitude of a query row, or of a tile of 128 keys
+//            or values, to [2^13, 2^14). A number is then off by 2^-22 of itself or 2^-39 of the largest, whichever is
+//            more: the same for what lies within 2^16 of it. What a row does not attend shares the tile with what it does, so
+//            a single large number, anywhere in it, would take the precision of all others. A key (or value) fits a scale if
+//            none of its groups of four adjacent numbers is larger, and none that is not 0 is more than 2^16 below. Where some
+//            do not, the tile takes the scale that suits most, and the others are left out and added in fp32, straight from
+//            their pages. (Within groups of two, ordinary data with some channels a hundred times the others would leave
+//            keys out in one tile of ten; within four, in one of a million. A number is thus as good as in fp32 next to the
+//            largest of its four.) A row of q that does not fit, or scores that could pass some thousand, where rounding
+//            is a matter of whole powers of two, makes all keys of a tile fp32 work for the row's warp. V tiles under 2^-60
+//            are, too: the factors below would take them out of the normal numbers.
+//   weights  exp(s - t) are taken against t, the power of two above the row's largest score in the tile, and times 2^14:
+//            all they lose is 2^-38 of the tile's largest. (With t following the row's maximum only now and then, a tile of
+//            small weights and large values lost all of them.) The factor from there to the row's reference, which does follow
+//            only when the maximum has risen by 2^9, is an exact power of two and goes into the sums over tiles with the scale
+//            of V. There weights are at most 1, so that a sum of large values does not overflow before it is divided.
+// Per tile of keys the product P·V goes to its own accumulator and is added to fp32 registers, so the tensor cores' sums
+// stay short (24 steps). Four chunks of 2,000 tokens over 2,000 cached ones, 0.66 ms, take 1.1 ms with one large value per
+// request, 8.6 with one in each page of 16, 12.4 if all is fp32 work.
 //
 // One persistent CTA per SM works on an item: 256 query rows (two tiles of 128, row = token * g + head of the group) of
 // one (request, kv head) against a run of key tiles:
@@ -70,6 +82,7 @@ constexpr int kConvWarp = 2 * kSoftmaxWarps, kLoadWarp = kConvWarp + 2 * kConvWa
 constexpr int kWalkWarp = kIssueWarp + 2;
 constexpr int kTcThreads = 32 * (kWalkWarp + 1);  // seven warpgroups
 constexpr int kItems = 4;                         // items handed out ahead
+constexpr float kRise = 9.0f;                     // a row's reference follows its maximum when that is 2^kRise above it
 // Registers per thread of the softmax, conversion and loading/issuing warpgroups: 4·96 + 2·40 + 40 = 504, what the CTA is
 // launched with (7·72).
 constexpr int kLaunchRegs = 72, kSoftmaxRegs = 96, kConvRegs = 40, kMiscRegs = 40;
@@ -109,12 +122,17 @@ struct TcShared {
   Item items[kItems];
   int64_t tmp[2 * kTcThreads / 32];
   int64_t off;
-  alignas(16) uint32_t seen[2][kTcRing][4];  // [K, V]: keys of a tile that exist (bit per key)
+  alignas(16) uint32_t seen[2][kTcRing][4];  // [K, V]: keys of a tile that exist and that its scale suits (bit per key)
   float row_x[2][2][kTcRows];    // [query tile][half]: what the two threads of a row exchange
-  alignas(16) uint32_t max_bits[2][2][kConvWarps];  // converter warps' largest magnitudes; top bit: one is not finite
+  float row_top[2][2][2][kTcRows];  // [turn][query tile][half]: their largest scores of a key tile, two sets
+  alignas(16) uint32_t range[2][2][kConvWarps];  // converter warps' largest numbers and smallest pairs, as bf16 bits
+  uint32_t columns[2][kConvWarps];               // ... columns of groups of four that are not all 0
+  uint32_t keys[2][kTcKeys];                     // a key's (a value's) largest and smallest group
+  uint32_t small[kTcRing][4];                    // values left out of a tile that are smaller than the others
   float join_m[kTcRows], join_l[kTcRows];        // split items: the second group's maxima and sums
-  float scale[2][kTcRing];       // what a product with the tile is multiplied by to undo the tile's scale
-  int v_odd[kTcRing];            // a V tile held values that are not finite
+  // what a product with the tile is multiplied by to undo the tile's scale; negative: some keys of the tile are left to the
+  // fp32 path
+  float scale[2][kTcRing];
   int req;
   int unplaced;                  // a row range is invalid
   volatile int abort;
@@ -185,33 +203,37 @@ __device__ __forceinline__ void bar_named(int id, int threads) {
   __syncwarp();
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
-// ... and whether any of the threads says so.
-__device__ __forceinline__ bool bar_any(int id, int threads, bool mine) {
-  uint32_t r;
-  __syncwarp();
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 p, %3, 0;\n\t"
-      "bar.red.or.pred q, %1, %2, p;\n\t"
-      "selp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(r)
-      : "r"(id), "r"(threads), "r"((uint32_t)mine)
-      : "memory");
-  return r != 0;
-}
 __device__ __forceinline__ void bar_signal(int id, int threads) {
   __syncwarp();
   asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
+// A query row's scale times a key tile's, above which scores could be some thousand (numbers of the two up to 2^12 in product):
+// made once by the tensor cores and once in fp32 they could differ by more than 1, and weights of both kinds would no longer
+// go together, so all of the tile is fp32 work.
+constexpr float kMostScore = 1.52587890625e-5f;  // 2^-16
 // The power of two that brings a magnitude (bits of a finite fp32, sign cleared) to [2^13, 2^14), and its inverse.
 // Magnitudes under 2^-112 keep the largest scale.
 __device__ __forceinline__ void tile_scale(uint32_t bits, float& up, float& down) {
-  const int e = bits == 0 ? 140 : max(14, (int)(bits >> 23));  // biased exponent
+  const int e = max(14, (int)(bits >> 23));  // biased exponent
   up = __uint_as_float((uint32_t)(267 - e) << 23);
   down = __uint_as_float((uint32_t)(e - 13) << 23);
 }
 __device__ __forceinline__ bool finite_bits(uint32_t bits) { return bits < 0x7f800000u; }
+// Magnitudes as bf16 bits (16 bits, exponent in steps of kExp): one lies more than 2^16 below another.
+constexpr uint32_t kExp = 128, kApart = 16 * kExp;
+// 2^e x, for x a power of two; 0 below the normal numbers. e x is no larger than they are.
+__device__ __forceinline__ float times_pow2(float x, int e) {
+  const int field = (int)(__float_as_uint(x) >> 23) + e;
+  return field > 0 ? __uint_as_float((uint32_t)field << 23) : 0.0f;
+}
+
+constexpr uint32_t kInf = 255 * kExp, kTiny = 67 * kExp;  // infinity, 2^-60
+// max(|x|, |z|) and max(|y|, |w|) of four numbers, rounded to bf16; NaN counts as the largest.
+__device__ __forceinline__ __nv_bfloat162 max_abs4(float4 f) {
+  return __hmax2_nan(__habs2(__floats2bfloat162_rn(f.x, f.y)), __habs2(__floats2bfloat162_rn(f.z, f.w)));
+}
+__device__ __forceinline__ uint32_t bits2(__nv_bfloat162 x) { return *reinterpret_cast<const uint32_t*>(&x); }
 
 __device__ __forceinline__ uint32_t pack2(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 // Two fp32 numbers as fp16 hi parts and fp16 remainders (first number in the low half).
@@ -321,7 +343,8 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
     const int s = a.heads.div(r), h = it.kvh * a.g + (r - s * a.g);
     const int limit = live ? it.shift + s : -1;  // the last key this row attends
     const int first_limit = it.shift + a.heads.div(first);
-    float qdown;  // undoes the row's scale
+    // undoes the row's scale; the largest of the warp's rows, infinite where a row has its numbers too far apart for one scale
+    float qdown, q_most;
     {
       const float* p = a.q + (int64_t)(it.first + s) * a.q0 + (int64_t)h * a.q1;
       float x[32];
@@ -335,16 +358,28 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
         }
         x[d] = f.x; x[d + 1] = f.y; x[d + 2] = f.z; x[d + 3] = f.w;
       }
-      uint32_t big = 0;
+      uint32_t big = 0, small = 0xffffffffu;  // largest number, smallest group of four that is not 0 (less 1)
 #pragma unroll
-      for (int d = 0; d < 32; d++) {
-        x[d] = fmaf(x[d], a.scale_hi, x[d] * a.scale_lo);  // scores in powers of two
-        const uint32_t b = __float_as_uint(x[d]) & 0x7fffffffu;
-        if (finite_bits(b)) big = max(big, b);
+      for (int d = 0; d < 32; d += 4) {
+        uint32_t four = 0;
+#pragma unroll
+        for (int e = d; e < d + 4; e++) {
+          x[e] = fmaf(x[e], a.scale_hi, x[e] * a.scale_lo);  // scores in powers of two
+          const uint32_t b = __float_as_uint(x[e]) & 0x7fffffffu;
+          if (finite_bits(b)) four = max(four, b);
+        }
+        big = max(big, four);
+        small = min(small, four - 1);
       }
-      big = max(big, __float_as_uint(exchange(__uint_as_float(big))));
+      // both in one word, in 16 bits each: the scale needs no more than the exponent
+      const uint32_t theirs = __float_as_uint(exchange(__uint_as_float((big & 0xffff0000u) | (small >> 16))));
+      big = max(big, theirs & 0xffff0000u);
+      small = min(small >> 16, theirs & 0xffffu);
+      const bool odd = __any_sync(0xffffffffu, small + kApart < (big >> 16));
       float up;
       tile_scale(big, up, qdown);
+      q_most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(qdown)));
+      if (odd) q_most = INFINITY;  // no key for the tensor cores
 #pragma unroll
       for (int c = 0; c < 2; c++) {  // 16 elements: 8 columns of hi, 8 of lo
         float hi[8], lo[8];
@@ -366,7 +401,6 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
 #pragma unroll
     for (int d = 0; d < 16; d++) o[d] = make_float2(0.0f, 0.0f);
     float m = -INFINITY, l = 0.0f;  // reference and sum of the weights
-    int odd = 0;
 #pragma unroll 1
     for (int t = t0; t < end; t += step) {
       const int j = J + t - it.t0, slot = j % kTcRing, turn = (t - t0) / step;
@@ -374,13 +408,15 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
       if (tile == 0 ? turn > 0 && turn <= turns : turn < turns) bar_named(kBarTurn + tile, both);
       fence_after();
       // kept finite and above 0: a score of 0 or -inf times it stays one
-      const float c = fminf(fmaxf(qdown * sh.scale[0][slot], 1.1754944e-38f), 3.4028235e38f);
+      const float kdown = sh.scale[0][slot];
+      const float c = fminf(fmaxf(fabsf(qdown * kdown), 1.1754944e-38f), 3.4028235e38f);
+      const bool all_fp32 = q_most * fabsf(kdown) > kMostScore;
       const uint4 seen = *reinterpret_cast<const uint4*>(sh.seen[0][slot]);
-      if (t * kTcKeys + kTcKeys - 1 > first_limit || (seen.x & seen.y & seen.z & seen.w) != 0xffffffffu) {
+      if (t * kTcKeys + kTcKeys - 1 > first_limit || (seen.x & seen.y & seen.z & seen.w) != 0xffffffffu || all_fp32) {
         // scores of keys that do not exist or that the row does not attend become -inf in place
 #pragma unroll 1
         for (int g = 0; g < 4; g++) {
-          const int k0 = 64 * half + 16 * g, n = limit - (t * kTcKeys + k0) + 1;
+          const int k0 = 64 * half + 16 * g, n = all_fp32 ? 0 : limit - (t * kTcKeys + k0) + 1;
           const uint32_t vis = (sh.seen[0][slot][k0 >> 5] >> (k0 & 31)) & (n >= 16 ? 0xffffu : n <= 0 ? 0u : (1u << n) - 1u);
           float x[16];
           tc::tmem_ld16(cs + 16 * g, x);
@@ -402,14 +438,13 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
         }
         top = fmaxf(top, y);
       }
-      top *= c;
-      float old = m;
-      const bool rise = bar_any(pair, pair_threads, top > m + 9.0f);  // of any row of these warps; also from -inf, never on NaN
-      if (rise) {
-        top = fmaxf(top, exchange(top));
-        if (top > m + 9.0f) m = top;
-      }
-      const float ref = 6.0f - (m == -INFINITY ? 0.0f : m);
+      float* tops = sh.row_top[C & 1][tile][0];  // two sets: the one before may still be read
+      top *= c;  // a power of two
+      tops[half * kTcRows + row] = top;
+      bar_named(pair, pair_threads);
+      top = ceilf(fmaxf(top, tops[(half ^ 1) * kTcRows + row]));
+      // rounded down, so that no weight is above 2^14, however large the scores: fp16 holds none of 2^16
+      const float ref = __fsub_rd(14.0f, top == -INFINITY ? 0.0f : top);
       const float2 c2 = make_float2(c, c), ref2 = make_float2(ref, ref);
       float2 sum0 = make_float2(0.0f, 0.0f), sum1 = sum0;
 #pragma unroll 1
@@ -434,27 +469,114 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
       fence_before();
       bar_signal(kBarIssue + tile, 64 * quads + 32);
       if (turn < turns) bar_signal(kBarTurn + (tile ^ 1), both);
-      const float sum = (sum0.x + sum0.y) + (sum1.x + sum1.y);
-      if (rise) {
-        const float alpha = m == old ? 1.0f : ex2_sfu(old - m);
+      const bool rise = top > m + kRise;  // also from -inf, never on NaN
+      if (__any_sync(0xffffffffu, rise)) {
+        const float alpha = rise ? times_pow2(1.0f, (int)fmaxf(m - top, -1000.0f)) : 1.0f;
+        if (rise) m = top;
         const float2 al = make_float2(alpha, alpha);
-        l = l * alpha + sum;
+        l *= alpha;
 #pragma unroll
         for (int d = 0; d < 16; d++) o[d] = __fmul2_rn(o[d], al);
-      } else {
-        l += sum;
       }
+      // from the tile's weights, against -ref, to the row's, against m + kRise
+      const int shift = (int)fmaxf(top == -INFINITY ? -1000.0f : -ref - m, -1000.0f) - (int)kRise;
+      l = fmaf((sum0.x + sum0.y) + (sum1.x + sum1.y), times_pow2(1.0f, shift), l);
       if (ok && !warp_wait_bar(&sh.pv_full[tile], C & 1, &sh.abort)) ok = false;
       C++;
       fence_after();
-      const float2 f = make_float2(sh.scale[1][slot], sh.scale[1][slot]);
-      odd |= sh.v_odd[slot];
+      const float vdown = sh.scale[1][slot];
+      if (fminf(kdown, vdown) < 0.0f || all_fp32) {
+        // Keys that are left to fp32: those that sh.seen misses, or all where a row of q has its numbers too far apart. One at a
+        // time, and what can be made again is: registers are taken from the loop around (four prompt chunks of 2,000 653 us;
+        // with four keys at a time 746).
+        // pass 0: the largest score of keys whose values are small ones left out; pass 1: values left out; pass 2: keys left
+        // out. Where a small value has the largest weight of the tile, the others, taken against that, may have lost what
+        // counts beside it: then pass 1 takes all values of the tile, and P·V is not used.
+        int my_row = r, my_slot = slot, key0 = t * kTcKeys, my_half = half;
+        asm volatile("" : "+r"(my_row), "+r"(my_slot), "+r"(key0), "+r"(my_half));  // none of this is made ahead of the branch
+        const bool all = all_fp32, v_drops = !all && vdown < 0.0f;
+        bool near = false;
+#pragma unroll 1
+        for (int pass = !ok ? 3 : v_drops ? 0 : 2; pass < 3; pass++) {
+          if (pass == 1) near = __any_sync(0xffffffffu, near);
+          if (!all && !near && pass == (v_drops ? 1 : 2)) {
+            const float down = times_pow2(fabsf(vdown), shift);
 #pragma unroll
-      for (int c = 0; c < 2; c++) {
-        float x[16];
-        tc::tmem_ld16(cpv + 16 * c, x);
+            for (int d = 0; d < 16; d += 4) {
+              float x[8];
+              tc::tmem_ld8(cpv + 2 * d, x);
 #pragma unroll
-        for (int d = 0; d < 8; d++) o[8 * c + d] = __ffma2_rn(make_float2(x[2 * d], x[2 * d + 1]), f, o[8 * c + d]);
+              for (int e = 0; e < 4; e++)
+                o[d + e] = __ffma2_rn(make_float2(x[2 * e], x[2 * e + 1]), make_float2(down, down), o[d + e]);
+            }
+          }
+#pragma unroll 1
+          for (int k = 0; k < kTcKeys; k++) {
+            const uint32_t k_fits = sh.seen[0][my_slot][k >> 5];
+            uint32_t take = ~0u;
+            if (!all) {
+              if (pass == 0) take = k_fits & sh.small[my_slot][k >> 5];
+              else if (pass == 1) take = near ? k_fits : k_fits & ~sh.seen[1][my_slot][k >> 5];
+              else take = ~k_fits;
+            }
+            take >>= k & 31;
+            if (take == 0) k |= 31;  // none in the rest of the word
+            if (!(take & 1u)) continue;
+            const int pi = a.page.div(key0 + k);
+            int page;
+            if (key0 + k >= it.len) continue;
+            if (!integral(a.table[(int64_t)it.req * a.t0 + pi * a.t1], 0, a.pages - 1, page)) continue;
+            const int64_t at = (int64_t)page * a.c0 + (int64_t)it.kvh * a.c1 + (int64_t)(key0 + k - pi * a.page.size) * a.c2;
+            const int rr = min(my_row, it.rows - 1), sr = a.heads.div(rr);
+            const float* q = a.q + (int64_t)(it.first + sr) * a.q0 + (int64_t)(it.kvh * a.g + (rr - sr * a.g)) * a.q1;
+            const bool on = my_row < it.rows && key0 + k <= it.shift + sr;  // the row attends it
+            float x = 0.0f;
+#pragma unroll 1
+            for (int d = 0; d < a.D; d += 4) {
+              const float4 f = a.q_vec ? *reinterpret_cast<const float4*>(q + d)
+                                       : make_float4(q[d], q[d + 1], q[d + 2], q[d + 3]);
+              const float4 y = *reinterpret_cast<const float4*>(a.k + at + d);
+              x = fmaf(fmaf(f.x, a.scale_hi, f.x * a.scale_lo), y.x, x);
+              x = fmaf(fmaf(f.y, a.scale_hi, f.y * a.scale_lo), y.y, x);
+              x = fmaf(fmaf(f.z, a.scale_hi, f.z * a.scale_lo), y.z, x);
+              x = fmaf(fmaf(f.w, a.scale_hi, f.w * a.scale_lo), y.w, x);
+            }
+            if (pass == 0) {
+              near = near || (on && x > top - 1.0f);
+              continue;
+            }
+            if (pass == 2 && on && ceilf(x) > m + kRise) {
+              const float alpha = times_pow2(1.0f, (int)fmaxf(m - ceilf(x), -1000.0f));
+              m = ceilf(x);
+              l *= alpha;
+#pragma unroll
+              for (int d = 0; d < 16; d++) o[d] = __fmul2_rn(o[d], make_float2(alpha, alpha));
+            }
+            if (on) {  // a value that the row does not attend may be anything: it is left out, not multiplied by 0
+              const float w = ex2_sfu(x - (m == -INFINITY ? 0.0f : m) - kRise);  // m + kRise may round to m
+              if (pass == 2 && my_half == 0) l += w;  // the sums of both halves are joined
+              const float* v = a.v + at + 32 * my_half;
+#pragma unroll
+              for (int d = 0; d < 8; d++) {
+                if (32 * my_half + 4 * d >= a.D) break;
+                const float4 y = *reinterpret_cast<const float4*>(v + 4 * d);
+                o[2 * d] = __ffma2_rn(make_float2(y.x, y.y), make_float2(w, w), o[2 * d]);
+                o[2 * d + 1] = __ffma2_rn(make_float2(y.z, y.w), make_float2(w, w), o[2 * d + 1]);
+              }
+            }
+            __syncwarp();
+          }
+        }
+      } else {
+        const float down = times_pow2(vdown, shift);
+        const float2 f = make_float2(down, down);
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+          float x[16];
+          tc::tmem_ld16(cpv + 16 * c, x);
+#pragma unroll
+          for (int d = 0; d < 8; d++) o[8 * c + d] = __ffma2_rn(make_float2(x[2 * d], x[2 * d + 1]), f, o[8 * c + d]);
+        }
       }
     }
     if (tile == 0 && turns > 0 && mine == turns) bar_named(kBarTurn, both);
@@ -462,25 +584,6 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
     // Every warp has read the last scales before the issuing warp frees tiles that the ring's slots are reused for, and
     // none of this group, those without rows included, gets ahead to the next item's barriers.
     bar_named(end_bar, 256 + 32);
-    if (odd) {
-      // Values that are not finite were left out of the products: add those that this row attends.
-      const int k1 = min(it.t1 * kTcKeys, limit + 1);
-#pragma unroll 1
-      for (int j = it.t0 * kTcKeys; j < k1; j++) {
-        if (it.split && ((j / kTcKeys - it.t0) & 1) != tile) continue;
-        const int pi = a.page.div(j);
-        int page;
-        if (!integral(a.table[it.req * a.t0 + pi * a.t1], 0, a.pages - 1, page)) continue;
-        const float* v = a.v + (int64_t)page * a.c0 + (int64_t)it.kvh * a.c1 + (int64_t)(j - pi * a.page.size) * a.c2 + 32 * half;
-#pragma unroll
-        for (int d = 0; d < 16; d++) {
-          if (32 * half + 2 * d >= a.D) break;
-          const float2 f = *reinterpret_cast<const float2*>(v + 2 * d);
-          if (!finite_bits(__float_as_uint(f.x) & 0x7fffffffu)) o[d].x += f.x;
-          if (!finite_bits(__float_as_uint(f.y) & 0x7fffffffu)) o[d].y += f.y;
-        }
-      }
-    }
     J += it.t1 - it.t0;
     if (it.split) {
       // The second group's result goes to the first through the second's P·V columns (free until its next P).
@@ -571,6 +674,69 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
   }
 }
 
+// For a tile whose numbers lie far apart: the largest magnitude (in bf16 bits; 0 if there is none) under which most keys keep
+// their precision; kLeft is added when not all do. Those are taken out of sh.seen and become 0. A key keeps its precision if none
+// of its groups of four is larger and none further than 2^16 below; groups of 0 do not count in K, in V unless all keys have
+// them. `rows` is the lane's place in its warp's rows.
+constexpr uint32_t kLeft = 1u << 16;
+__device__ __forceinline__ uint32_t sort_keys(const AttnArgs& a, TcShared& sh, uint8_t* rows, int op, int slot, bool ok) {
+  int tid = threadIdx.x;
+  asm volatile("" : "+r"(tid), "+r"(op), "+r"(slot));  // nothing of this is computed ahead of the branch that leads here
+  const int warp = (tid >> 5) & 3, lane = tid & 31, tr = lane >> 4, tc4 = lane & 15;
+  uint32_t any = 0;
+#pragma unroll 1
+  for (int e = 0; e < 16 && 4 * tc4 < a.D; e++) any |= bits2(max_abs4(*reinterpret_cast<const float4*>(rows + e * 512)));
+  __syncwarp();
+  const uint32_t n = __ballot_sync(0xffffffffu, any != 0);
+  if (lane == 0) sh.columns[op][warp] = n | n >> 16;
+  bar_named(kBarConv + op, 32 * kConvWarps);
+  const uint32_t columns = sh.columns[op][0] | sh.columns[op][1] | sh.columns[op][2] | sh.columns[op][3];
+  const bool counts = (columns >> tc4) & 1u;
+  const uint32_t seen = ok ? sh.seen[op][slot][warp] : 0u;
+  uint32_t* keys = sh.keys[op];
+#pragma unroll 1
+  for (int e = 0; e < 16; e++) {
+    uint32_t hi = 0, lo = 0xffffu;
+    if (counts && ((seen >> (2 * e + tr)) & 1u)) {
+      const uint32_t m = bits2(max_abs4(*reinterpret_cast<const float4*>(rows + e * 512)));
+      hi = max(m & 0xffffu, m >> 16);
+      if (hi != 0 || op == 1) lo = hi;
+    }
+#pragma unroll 1
+    for (int o = 1; o < 16; o <<= 1) {
+      hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    }
+    if (tc4 == 0) keys[32 * warp + 2 * e + tr] = hi << 16 | lo;
+  }
+  bar_named(kBarConv + op, 32 * kConvWarps);
+  auto fits = [&](uint32_t key, uint32_t top) { return key >> 16 <= top && (key & 0xffffu) + kApart >= top; };
+  uint32_t best = 0;  // how many keys fit, and under which magnitude, one of the keys' own
+#pragma unroll 1
+  for (int c = lane; c < kTcKeys; c += 32) {
+    const uint32_t top = keys[c] >> 16;
+    if (top == 0 || top >= kInf || (op == 1 && top < kTiny)) continue;
+    uint32_t count = 0;
+#pragma unroll 1
+    for (int i = 0; i < kTcKeys; i++) count += fits(keys[i], top) ? 1u : 0u;
+    best = max(best, count << 16 | top);
+  }
+  __syncwarp();
+  best = __reduce_max_sync(0xffffffffu, best);
+  const uint32_t top = best & 0xffffu, key = keys[32 * warp + lane];
+  const uint32_t out = __ballot_sync(0xffffffffu, best == 0 || !fits(key, top)) & seen;
+  const uint32_t small = __ballot_sync(0xffffffffu, best == 0 || (key & 0xffffu) + kApart < top) & out;
+#pragma unroll 1
+  for (int e = 0; e < 16; e++)  // missing rows, too: they are copies of one that may be among these
+    if (!(((seen & ~out) >> (2 * e + tr)) & 1u)) *reinterpret_cast<float4*>(rows + e * 512) = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (lane == 0) {
+    if (out != 0) sh.seen[op][slot][warp] = seen & ~out;
+    if (op == 1) sh.small[slot][warp] = small;
+  }
+  __syncwarp();
+  return top + (best >> 16 < kTcKeys ? kLeft : 0u);
+}
+
 // Splits the raw K (op 0) or V (op 1) tiles in place. A warp has four of a tile's groups of eight rows; a first pass takes
 // the largest magnitude of the whole tile, a second splits group by group, so that few registers are held.
 __device__ __forceinline__ void convert_role(const AttnArgs& a, TcShared& sh, uint8_t* tiles, int op) {
@@ -580,6 +746,7 @@ __device__ __forceinline__ void convert_role(const AttnArgs& a, TcShared& sh, ui
   // eight is stored as chunk c ^ r
   const uint32_t from = 4 * warp * kGroup + tr * 256 + 16 * tc4;
   const uint32_t to = 4 * warp * kGroup + ((tr * 128 + ((tc4 >> 1) << 4) + ((tc4 & 1) << 3)) ^ (tr << 4));
+  const bool pad = 4 * tc4 >= a.D;
   bool ok = true;
   int J = 0, st = 0, parity = 0;
   const Item* p_it;
@@ -589,17 +756,23 @@ __device__ __forceinline__ void convert_role(const AttnArgs& a, TcShared& sh, ui
 #pragma unroll 1
     for (; n > 0; n--) {
       uint8_t* tile = tiles + (op * kTcStages + st) * kTile;
-      uint32_t big = 0;
+      uint32_t big = 0, small = 0xffffu;
       if (ok && !warp_wait_bar(&sh.raw[op][st], parity, &sh.abort)) ok = false;
       if (ok) {
         const uint32_t seen = sh.seen[op][J % kTcRing][warp];  // of the warp's 32 rows
-        if (seen != 0xffffffffu || a.D < kTcDim) {  // nothing was copied there
+        if (seen != 0xffffffffu || a.D < kTcDim) {
+          // Nothing was copied there. A missing row's weights are 0; it becomes one like the warp's first, so that it changes
+          // none of what is found out below.
+          float4 like = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (seen != 0xffffffffu && seen != 0 && !pad)
+            like = *reinterpret_cast<const float4*>(tile + 4 * warp * kGroup + (__ffs(seen) - 1) * 256 + 16 * tc4);
+          __syncwarp();
 #pragma unroll 1
           for (int e = 0; e < 16; e++)
-            if (4 * tc4 >= a.D || !((seen >> (2 * e + tr)) & 1u))
-              *reinterpret_cast<float4*>(tile + from + e * 512) = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (pad || !((seen >> (2 * e + tr)) & 1u)) *reinterpret_cast<float4*>(tile + from + e * 512) = like;
         }
-        __nv_bfloat162 big2 = __floats2bfloat162_rn(0.0f, 0.0f);  // in bf16: only its exponent counts
+        // The largest magnitude, and the smallest of pairs (of a group of four), in bf16: only exponents count.
+        __nv_bfloat162 most = __floats2bfloat162_rn(0.0f, 0.0f), least = __floats2bfloat162_rn(3e38f, 3e38f);
 #pragma unroll 1
         for (int g = 0; g < 4; g++) {
           float4 x[4];
@@ -607,40 +780,27 @@ __device__ __forceinline__ void convert_role(const AttnArgs& a, TcShared& sh, ui
           for (int e = 0; e < 4; e++) x[e] = *reinterpret_cast<const float4*>(tile + from + g * kGroup + e * 512);
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            big2 = __hmax2_nan(big2, __habs2(__floats2bfloat162_rn(x[e].x, x[e].y)));
-            big2 = __hmax2_nan(big2, __habs2(__floats2bfloat162_rn(x[e].z, x[e].w)));
+            const __nv_bfloat162 m = max_abs4(x[e]);
+            most = __hmax2_nan(most, m);
+            least = __hmin2(least, m);
           }
         }
-        const uint32_t b2 = *reinterpret_cast<const uint32_t*>(&big2);
-        big = max(b2 << 16, b2 & 0xffff0000u);
-        if (!finite_bits(big)) {  // the largest finite magnitude, and a mark
-          big = 0;
-#pragma unroll 1
-          for (int e = 0; e < 16; e++) {
-            float* v = reinterpret_cast<float*>(tile + from + e * 512);
-#pragma unroll 1
-            for (int c = 0; c < 4; c++) {
-              const uint32_t b = __float_as_uint(v[c]) & 0x7fffffffu;
-              if (finite_bits(b)) big = max(big, b);
-              else if (op == 1) v[c] = 0.0f;  // it would spoil the rows that do not attend it, too
-            }
-          }
-          big |= 0x80000000u;
-        }
+        big = max(bits2(most) & 0xffffu, bits2(most) >> 16);
+        if (!pad && seen != 0) small = min(bits2(least) & 0xffffu, bits2(least) >> 16);
       }
-      const uint32_t odd = __any_sync(0xffffffffu, (int)big < 0) ? 0x80000000u : 0u;
-      big = __reduce_max_sync(0xffffffffu, big & 0x7fffffffu) | odd;
-      uint32_t* maxima = sh.max_bits[op][J & 1];  // two sets: a warp may be a tile ahead of one that still reads
-      if (lane == 0) maxima[warp] = big;
+      const uint32_t mine = __reduce_max_sync(0xffffffffu, big) << 16 | __reduce_min_sync(0xffffffffu, small);
+      uint32_t* range = sh.range[op][J & 1];  // two sets: a warp may be a tile ahead of one that still reads
+      if (lane == 0) range[warp] = mine;
       bar_named(kBarConv + op, 32 * kConvWarps);
+      const uint4 all = *reinterpret_cast<const uint4*>(range);
+      uint32_t top = max(max(all.x, all.y), max(all.z, all.w)) >> 16;
+      const uint32_t low = min(min(all.x & 0xffffu, all.y & 0xffffu), min(all.z & 0xffffu, all.w & 0xffffu));
+      if (low + kApart < top || top >= kInf || (op == 1 && top != 0 && top < kTiny))
+        top = sort_keys(a, sh, tile + from, op, J % kTcRing, ok);
       if (ok) {
-        const uint4 all = *reinterpret_cast<const uint4*>(maxima);
         float up, down;
-        tile_scale(max(max(all.x & 0x7fffffffu, all.y & 0x7fffffffu), max(all.z & 0x7fffffffu, all.w & 0x7fffffffu)), up, down);
-        if (warp == 0 && lane == 0) {
-          sh.scale[op][J % kTcRing] = down;
-          if (op == 1) sh.v_odd[J % kTcRing] = (all.x | all.y | all.z | all.w) >> 31;
-        }
+        tile_scale(top << 16, up, down);
+        if (warp == 0 && lane == 0) sh.scale[op][J % kTcRing] = top >= kLeft ? -down : down;
         const float2 up2 = make_float2(up, up);
 #pragma unroll 1
         for (int g = 0; g < 4; g++) {

@@ -588,6 +588,168 @@ def test_attention_of_a_few_large_keys_among_small_ones(be, reqs):
     check_attention(ref, got, 64, 170, np.abs(vc).max(), most, rms)
 
 
+def attend_bound(q, kc, vc, table, q_start, kv_len, scale):
+    """float64 result and a bound of its error for each element. With w_j the weights of the row, a score's error is at
+    most (D + 16) u sum |q||k| scale (see above), which bends its weight by twice that, e_j, relatively, and the sums add
+    (L + 32) u: |error of o_d| <= sum_j w_j |v_jd| (e_j + (L + 32) u) + |o_d| sum_j w_j e_j. Keys of weight 0 count
+    for nothing, however large, and so does what other rows attend. A weight is not asked to be exact under 2^-100,
+    and its products not under fp32's smallest normal number."""
+    rows, h, d = q.shape
+    page, g = kc.shape[2], h // kc.shape[1]
+    out, tol = np.zeros((rows, h, d)), np.zeros((rows, h, d))
+    for i in range(len(kv_len)):
+        a, b, length = q_start[i], q_start[i + 1], kv_len[i]
+        ids = table[i, :ceil_div(length, page)]
+        k = kc[ids].transpose(1, 0, 2, 3).reshape(kc.shape[1], -1, d)[:, :length].astype(np.float64)
+        v = vc[ids].transpose(1, 0, 2, 3).reshape(kc.shape[1], -1, d)[:, :length].astype(np.float64)
+        for r in range(a, b):
+            n = length - (b - a) + (r - a) + 1
+            for j in range(h):
+                kk, vv, x = k[j // g, :n], v[j // g, :n], q[r, j].astype(np.float64)
+                s = kk @ x * scale
+                w = np.exp(s - s.max())
+                w /= w.sum()
+                e = 2 * (d + 16) * U * (np.abs(kk) @ np.abs(x)) * scale
+                out[r, j] = w @ vv
+                tol[r, j] = (w * (e + (n + 32) * U) + 2.0 ** -100) @ np.abs(vv) + np.abs(out[r, j]) * (w @ e) + 2.0 ** -126
+    return out, tol
+
+
+def check_bound(be, case, scale, max_new=0):
+    ref, tol = attend_bound(*case, scale)
+    got = attend(be, *case, scale, max_new).astype(np.float64)
+    assert np.isfinite(got).all()
+    worst = (np.abs(got - ref) / tol).max()
+    assert worst <= 1, f"error {worst:.3g} times its bound"
+    assert be.check_device_error() == 0
+
+
+WIDE = [([(9, 3)], 3, 64), ([(200, 70), (3, 1)], 70, 64), ([(40, 130)], 0, 64), ([(250, 24), (140, 24)], 24, 16)]
+
+
+def at_key(case, i, j):
+    """Page and offset of a request's position."""
+    page = case[1].shape[2]
+    return case[3][i, j // page], j % page
+
+
+@pytest.mark.parametrize("reqs,max_new,d", WIDE)
+@pytest.mark.parametrize("size", [1e6, 1e8, 1e12, 1e30, 3e38])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_a_large_number_that_a_row_does_not_attend_changes_nothing(be, reqs, max_new, d, size, which):
+    """One element of the last new token's key or value is large: the rows before it do not attend it."""
+    case = paged_case(89, 4, 2, d, 16, reqs, 0, stale=0.0)
+    p, o = at_key(case, 0, int(case[5][0]) - 1)
+    case[1 if which == "k" else 2][p, :, o, 5] = np.float32(size)
+    check_bound(be, case, d ** -0.5, max_new)
+
+
+@pytest.mark.parametrize("reqs,max_new,d", WIDE)
+@pytest.mark.parametrize("size", [1e3, 1e6, 1e12, 1e30])
+def test_large_keys_of_weight_zero_leave_the_other_scores(be, reqs, max_new, d, size):
+    """Keys far below the others in score: attended by every row, weight 0."""
+    case = paged_case(97, 4, 2, d, 16, reqs, 0, stale=0.0)
+    case[0][..., 5] = np.abs(case[0][..., 5]) + 0.5
+    for j in (1, 7):
+        p, o = at_key(case, 0, j)
+        case[1][p, :, o, 5] = np.float32(-size)
+    check_bound(be, case, d ** -0.5, max_new)
+
+
+@pytest.mark.parametrize("reqs,max_new,d", WIDE)
+@pytest.mark.parametrize("size,score", [(1e3, -3.0), (1e6, -12.0), (1e12, -25.0), (1e20, -30.0), (1e30, -60.0), (3e38, -60.0)])
+def test_large_values_of_small_weight(be, reqs, max_new, d, size, score):
+    """A value that its weight brings down to the size of the others, or above: the weight keeps its precision."""
+    case = paged_case(101, 4, 2, d, 16, reqs, 0, stale=0.0)
+    case[0][..., 5] = 1.0
+    p, o = at_key(case, 0, 3)
+    case[1][p, :, o, 5] = np.float32(score * d ** 0.5)
+    case[2][p, :, o] *= np.float32(size) / np.abs(case[2][p, :, o]).max()
+    check_bound(be, case, d ** -0.5, max_new)
+
+
+@pytest.mark.parametrize("size,score", [(1e4, -12.0), (1e10, -25.0), (1e16, -30.0), (1e30, -60.0), (1e-10, 20.0), (1e-30, 60.0)])
+@pytest.mark.parametrize("reqs,max_new,d", [([(380, 70)], 70, 64), ([(300, 3)], 3, 64), ([(270, 200), (300, 1)], 0, 16)])
+def test_stretches_of_large_values_of_small_weight(be, reqs, max_new, d, size, score):
+    """Positions 100 to 300 hold values of another size than the rest and scores as far the other way."""
+    case = paged_case(103, 4, 2, d, 16, reqs, 0, stale=0.0)
+    case[0][..., 5] = 1.0
+    for j in range(100, 300):
+        p, o = at_key(case, 0, j)
+        case[1][p, :, o, 5] = np.float32(score * d ** 0.5)
+        case[2][p, :, o] *= np.float32(size)
+    check_bound(be, case, d ** -0.5, max_new)
+
+
+@pytest.mark.parametrize("reqs,max_new,d", WIDE)
+@pytest.mark.parametrize("size", [1e7, 1e10, 1e30])
+@pytest.mark.parametrize("j", [128, 160])
+def test_large_values_in_front_of_a_stretch_that_ends_inside_a_tile(be, reqs, max_new, d, size, j):
+    """The first position of 32, with positions that do not exist behind it in the same 32."""
+    case = paged_case(109, 4, 2, d, 16, reqs, 0)
+    for i in range(len(reqs)):
+        if j < case[5][i]:
+            p, o = at_key(case, i, j)
+            case[2][p, :, o, 5] = np.float32(size)
+            case[1][p, :, o, 6] = np.float32(-size)
+    check_bound(be, case, d ** -0.5, max_new)
+
+
+@pytest.mark.parametrize("reqs,max_new,d", WIDE)
+@pytest.mark.parametrize("size", [1e5, 1e7, 1e9, 1e11, 1e14, 1e20])
+def test_scores_of_any_size(be, reqs, max_new, d, size):
+    """Scores whose steps in fp32 are whole powers of two: the largest keeps its weight, with a large value in the tile as well."""
+    for big in (False, True):
+        q, kc, vc, *rest = paged_case(113, 4, 2, d, 16, reqs, 0, stale=0.0)
+        case = [q * np.float32(size), kc, vc, *rest]
+        if big:
+            p, o = at_key(case, 0, 3)
+            vc[p, :, o, 5] = 1e7
+        got = attend(be, *case, d ** -0.5, max_new).astype(np.float64)
+        assert np.isfinite(got).all()
+        ref, tol = attend_bound(*case, d ** -0.5)
+        # scores this large are off by more than 1: all a row must do is stay within the values it attends, and follow a key that
+        # leads by more than the error
+        h = q.shape[1] // kc.shape[1]
+        for r in range(len(q)):
+            i = int(np.searchsorted(rest[1], r, "right")) - 1
+            n = int(rest[2][i] - (rest[1][i + 1] - rest[1][i]) + r - rest[1][i]) + 1
+            at = np.arange(n)
+            for j in range(q.shape[1]):
+                k = kc[rest[0][i, at // 16], j // h, at % 16].astype(np.float64)
+                v = vc[rest[0][i, at // 16], j // h, at % 16].astype(np.float64)
+                s = k @ case[0][r, j].astype(np.float64) * d ** -0.5
+                off = 2 * (d + 16) * U * (np.abs(k) @ np.abs(case[0][r, j]).astype(np.float64)).max() * d ** -0.5
+                near = s > s.max() - 2 * off - 100  # beyond that, less than 2^-100
+                lo, hi = v[near].min(0), v[near].max(0)
+                slack = (n + 32) * U * np.abs(v[near]).max(0) + 2.0 ** -90 * np.abs(v).max(0)
+                assert (got[r, j] >= lo - slack).all() and (got[r, j] <= hi + slack).all()
+        assert be.check_device_error() == 0
+
+
+@pytest.mark.parametrize("reqs,max_new,d", WIDE)
+@pytest.mark.parametrize("what", ["k 1e8, q 1e-8", "q 1e8, k 1e-8", "q 1e12, k 0", "v 1e8", "v 1e20", "v zeros of the weightiest key", "v column of zeros",
+                                  "v 1e36", "v 1e-36", "k zeros", "rows of q far apart"])
+def test_channels_of_sizes_far_apart(be, reqs, max_new, d, what):
+    q, kc, vc, *rest = paged_case(107, 4, 2, d, 16, reqs, 0, stale=0.0)
+    case = [q, kc, vc, *rest]
+    if what.startswith("k 1e8"): kc[..., 5] *= np.float32(1e8); q[..., 5] *= np.float32(1e-8)
+    if what.startswith("q 1e8"): q[..., 5] *= np.float32(1e8); kc[..., 5] *= np.float32(1e-8)
+    if what.startswith("q 1e12"): q[..., 5] *= np.float32(1e12); kc[..., 5] = 0
+    if what == "v 1e8": vc[..., 5] *= np.float32(1e8)
+    if what == "v 1e20": vc[..., 5] *= np.float32(1e20)
+    if what == "v column of zeros": vc[..., 4:8] = 0
+    if what == "v 1e36": vc *= np.float32(1e36)
+    if what == "v 1e-36": vc *= np.float32(1e-36)
+    if what == "k zeros": kc[rest[0][0, 0], :, 3:9] = 0; kc[..., 8:12] = 0
+    if what == "rows of q far apart": q *= np.float32(2.0) ** -np.arange(len(q), dtype=np.float32)[:, None, None].clip(0, 60)
+    if what.startswith("v zeros"):
+        q[..., 5] = 1.0
+        p, o = at_key(case, 0, 2)
+        kc[p, :, o, 5], vc[p, :, o] = np.float32(40 * d ** 0.5), 0
+    check_bound(be, case, d ** -0.5, max_new)
+
+
 @pytest.mark.parametrize("reqs", [[(40, 1), (3, 1)], [(70, 100), (20, 3)]])
 @pytest.mark.parametrize("shift", [0, 1])
 def test_attention_of_strided_views(be, reqs, shift):
