@@ -77,9 +77,10 @@ struct Scatter {
 // lanes by Scatter, which leaves each lane one (row, key) score to exponentiate; the probabilities go back to the
 // group's lanes by shuffles for P V. Keys and values come through a ring in shared memory, which each lane fills by
 // asynchronous copies two steps ahead with what it reads itself, so the ring needs no barrier and the keys on their way
-// (128 KB per SM) no registers. Weights are taken against a reference that follows the row maximum only when that rises
-// by 2^8 (fp32 holds such weights as well), so the sums are hardly ever rescaled. Steps of keys that every row attends
-// have no masks, and where pages hold whole groups a group's page is looked up once.
+// (128 KB per SM) no registers. Weights are taken against 2^8 above a reference that follows the row maximum only when
+// that rises by 2^8, so the sums are hardly ever rescaled, and no weight is above 1: a large value, weighted, does not
+// overflow. Steps of keys that every row attends have no masks, and where pages hold whole groups a group's page is looked
+// up once.
 //
 // Work split: every (request, kv head, group of R rows) is ceil(len / 64) units; the units of all of them, in order,
 // are divided evenly over the blocks, so lengths need not be alike. A block's share is a run of segments, listed in
@@ -338,7 +339,7 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsPerSm) k_paged_rows(const A
           acc[y][2 * h] = acc[y][2 * h + 1] = make_float2(0.f, 0.f);
         }
       if (x + 1 < ns) read_q(s_seg[x + 1]);
-      float m[kOwn], ref[kOwn], l[kOwn];  // reference, the same or 0 while there is none, sum
+      float m[kOwn], ref[kOwn], l[kOwn];  // reference; kRise above it, or 0 while there is none; sum
       int limit[kOwn];                    // the last key that each kept score's row attends
 #pragma unroll
       for (int o = 0; o < kOwn; o++) {
@@ -396,7 +397,8 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsPerSm) k_paged_rows(const A
             for (int sh = kRep; sh < kRep * kRowLanes; sh <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, sh));
             if (mx > m[o] + kRise) {
               alpha[o] = ex2_sfu(m[o] - mx);
-              m[o] = ref[o] = mx;
+              m[o] = mx;
+              ref[o] = mx + kRise;
               l[o] *= alpha[o];
             } else {
               alpha[o] = 1.0f;

@@ -727,6 +727,19 @@ def test_scores_of_any_size(be, reqs, max_new, d, size):
         assert be.check_device_error() == 0
 
 
+@pytest.mark.parametrize("reqs,max_new,d", WIDE + [([(1500, 1)] * 30, 1, 64), ([(1500, 2)] * 30, 2, 128)])
+@pytest.mark.parametrize("score", [0.0, 2.0, 5.0])
+def test_the_largest_value_of_the_type_does_not_overflow(be, reqs, max_new, d, score):
+    """A weight of less than 1 times 3.4e38, its score above those before it: finite, as the sum divided is."""
+    case = paged_case(127, 4, 2, d, 16, reqs, 0, stale=0.0)
+    case[0][..., 5] = 1.0
+    for i, (cached, _) in enumerate(reqs):
+        p, o = at_key(case, i, min(200, cached) - 3)
+        case[1][p, :, o, 5] = np.float32(score * d ** 0.5)
+        case[2][p, :, o, 5] = np.float32(3.4e38)
+    check_bound(be, case, d ** -0.5, max_new)
+
+
 @pytest.mark.parametrize("reqs,max_new,d", WIDE)
 @pytest.mark.parametrize("what", ["k 1e8, q 1e-8", "q 1e8, k 1e-8", "q 1e12, k 0", "v 1e8", "v 1e20", "v zeros of the weightiest key", "v column of zeros",
                                   "v 1e36", "v 1e-36", "k zeros", "rows of q far apart"])
