@@ -361,7 +361,8 @@ pai_status pai_dataset_batch(pai_ctx* ctx, const int64_t* indices, int32_t count
 pai_status pai_dataset_close(pai_ctx* ctx);
 
 /* ==== Diagnostics (no counterpart in the reference; used by the benchmark and tests) ==== */
-/* Reads and clears the device flag that bounded waits inside kernels set on a timeout (PAI_ERR_TIMEOUT if set). */
+/* Reads and clears the device flag that bounded waits inside kernels set on a timeout (PAI_ERR_TIMEOUT if set). After one, what
+ * the paged attention computed until this call is invalid, too: its split work counts arrivals that may be missing. */
 pai_status pai_check_device_error(pai_ctx* ctx, int32_t* code);
 /* Device time between two points of the compute stream, from CUDA events recorded on that stream. stop blocks. */
 pai_status pai_timer_start(pai_ctx* ctx);

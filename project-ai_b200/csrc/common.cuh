@@ -79,7 +79,8 @@ struct pai_ctx {
   // device flag the kernels with bounded waits report into (0 = ok)
   int* d_error_flag = nullptr;
   // arrival counters of the paged attention's split work (attention_paged.cu): zero between launches, which reset what
-  // they used; launches of one context run one after another on its stream, replayed graphs' included
+  // they used; launches of one context run one after another on its stream, replayed graphs' included. After a wait that gave
+  // up they may not be, and are cleared with the error flag
   unsigned* d_tickets = nullptr;
   pai::NcclState* nccl = nullptr;
   pai::IoState* io = nullptr;  // checkpoint streaming and the open packed dataset (io.cu)

@@ -451,6 +451,24 @@ PAI_API pai_status pai_sync(pai_ctx* ctx) {
   return PAI_OK;
 }
 
+// Reads and clears the device error flag that bounded waits in the kernels report into. With it go the arrival counters of split
+// work: a CTA that gave up a wait may not have arrived everywhere.
+PAI_API pai_status pai_check_device_error(pai_ctx* ctx, int32_t* code) {
+  PAI_TRY(enter(ctx));
+  int v = 0;
+  PAI_CUDA(cudaMemcpyAsync(&v, ctx->d_error_flag, 4, cudaMemcpyDeviceToHost, ctx->stream));
+  PAI_CUDA(cudaStreamSynchronize(ctx->stream));
+  if (v) {
+    PAI_CUDA(cudaMemsetAsync(ctx->d_error_flag, 0, 4, ctx->stream));
+    PAI_CUDA(cudaMemsetAsync(ctx->d_tickets, 0, kTickets * sizeof(unsigned), ctx->stream));
+  }
+  if (code) *code = v;
+  if (v)
+    return set_error(PAI_ERR_TIMEOUT, "a kernel wait timed out (site %d); results of the affected launch, and of paged attention "
+                     "since, are invalid", v);
+  return PAI_OK;
+}
+
 PAI_API pai_status pai_device_name(pai_ctx* ctx, char* buf, int32_t n) {
   if (!ctx || !buf || n <= 0) return set_error(PAI_ERR_ARGUMENT, "bad arguments");
   snprintf(buf, (size_t)n, "%s", ctx->name);

@@ -933,15 +933,3 @@ PAI_API pai_status pai_matmul(pai_ctx* ctx, const pai_tensor* a, const pai_tenso
   *out = r;
   return PAI_OK;
 }
-
-// Reads and clears the device error flag that bounded waits in the kernels report into.
-PAI_API pai_status pai_check_device_error(pai_ctx* ctx, int32_t* code) {
-  PAI_TRY(enter(ctx));
-  int v = 0;
-  PAI_CUDA(cudaMemcpyAsync(&v, ctx->d_error_flag, 4, cudaMemcpyDeviceToHost, ctx->stream));
-  PAI_CUDA(cudaStreamSynchronize(ctx->stream));
-  if (v) PAI_CUDA(cudaMemsetAsync(ctx->d_error_flag, 0, 4, ctx->stream));
-  if (code) *code = v;
-  if (v) return set_error(PAI_ERR_TIMEOUT, "a kernel wait timed out (site %d); results of the affected launch are invalid", v);
-  return PAI_OK;
-}

@@ -1,0 +1,58 @@
+"""Host code of the paged KV cache entry points where the GPU cannot be made to fail: the library's own objects, linked with a
+CUDA runtime whose device memory is host memory (fake_cudart.cpp). No GPU is used, and no kernel runs."""
+import ctypes
+import subprocess
+from pathlib import Path
+
+import numpy as np
+import pytest
+
+import projectai_b200
+from projectai_b200 import build
+from projectai_b200.cabi import DeviceTimeoutError, NativeBackend, NativeLibrary
+
+HERE = Path(__file__).resolve().parent
+OBJECTS = ("context", "paged", "attention_paged", "attention_paged_tc")
+TICKETS = 4 * 4096  # bytes of the arrival counters
+
+
+@pytest.fixture(scope="session")
+def fake(tmp_path_factory):
+    build.build_cuda()
+    out = tmp_path_factory.mktemp("fake") / "libfake.so"
+    cuda = Path(build.NVCC).resolve().parents[1]
+    subprocess.run([build.CXX, "-shared", "-fPIC", "-std=c++17", "-O1", f"-I{cuda}/include", "-o", str(out), str(HERE / "fake_cudart.cpp"),
+                    *[str(build.BUILD / f"{name}.o") for name in OBJECTS], "-Wl,--no-undefined,-Bsymbolic", "-lpthread"], check=True)  # its own runtime, not one that is loaded already
+    lib = NativeLibrary(out, "pai_")
+    lib.lib.fake_block.argtypes, lib.lib.fake_block.restype = [ctypes.c_size_t], ctypes.c_void_p
+    lib.lib.fake_fail_after.argtypes = [ctypes.c_long]
+    lib.lib.fake_log.restype = ctypes.c_char_p
+    lib.lib.fake_launches.restype = ctypes.c_long
+    return lib
+
+
+@pytest.fixture()
+def be(fake):
+    b = NativeBackend(fake)
+    yield b
+    fake.lib.fake_fail_after(-1)
+    b.close()
+
+
+def device(fake, nbytes, dtype):
+    """A block of "device" memory of the newest context, by its size."""
+    p = fake.lib.fake_block(nbytes)
+    return np.frombuffer((ctypes.c_char * nbytes).from_address(p), dtype=dtype)
+
+
+def test_an_error_of_the_device_clears_the_arrival_counters(fake, be):
+    """A wait that gave up may leave a split item without its last arrival: the counters must not carry that into later
+    launches once the error has been read."""
+    flag, tickets = device(fake, 64, np.int32), device(fake, TICKETS, np.uint32)
+    assert not flag.any() and not tickets.any()  # as created
+    for code in (76, 80, 1):
+        flag[0], tickets[3], tickets[4095] = code, 2, 1
+        with pytest.raises(DeviceTimeoutError):
+            be.check_device_error()
+        assert flag[0] == 0 and not tickets.any()
+    assert be.check_device_error() == 0
