@@ -596,8 +596,8 @@ PAI_API pai_status pai_sdpa_paged(pai_ctx* ctx, const pai_tensor* q, const pai_t
   const char* names[6] = {"q", "k_cache", "v_cache", "table", "q_start", "kv_len"};
   for (int i = 0; i < 6; i++) PAI_TRY(check_view(ctx, ins[i], names[i]));
   PAI_TRY(pai_paged::check_sdpa(set_error, q, k_cache, v_cache, table, q_start, kv_len, max_new));
-  pai_tensor r;
-  PAI_TRY(alloc_tensor(ctx, 3, q->dims, PAI_F32, false, &r));
+  Results<1> r(ctx);
+  PAI_TRY(r.add(3, q->dims));
   paged::AttnArgs a{};
   a.q = fptr(*q); a.q0 = q->strides[0]; a.q1 = q->strides[1];
   a.k = fptr(*k_cache); a.v = fptr(*v_cache);
@@ -605,7 +605,7 @@ PAI_API pai_status pai_sdpa_paged(pai_ctx* ctx, const pai_tensor* q, const pai_t
   a.table = fptr(*table); a.t0 = table->strides[0]; a.t1 = table->strides[1];
   a.start = fptr(*q_start); a.start_s = q_start->strides[0];
   a.len = fptr(*kv_len); a.len_s = kv_len->strides[0];
-  a.out = fptr(r);
+  a.out = fptr(r.t[0]);
   a.n = table->dims[0]; a.rows = q->dims[0]; a.H = q->dims[1]; a.D = q->dims[2];
   a.KVH = k_cache->dims[1]; a.g = a.H / a.KVH; a.heads = paged::page_div(a.g);
   a.pages = k_cache->dims[0]; a.max_pages = table->dims[1];
@@ -616,7 +616,7 @@ PAI_API pai_status pai_sdpa_paged(pai_ctx* ctx, const pai_tensor* q, const pai_t
   a.scale_lo = (float)(scale2 - (double)a.scale_hi);
   a.tickets = ctx->d_tickets;
   a.error_flag = ctx->d_error_flag;
-  if (numel(r) > 0) {
+  if (numel(r.t[0]) > 0) {
     auto aligned = [](const pai_tensor& t) {
       if (reinterpret_cast<uintptr_t>(fptr(t)) % 16) return false;
       for (int i = 0; i + 1 < t.rank; i++)
@@ -652,6 +652,6 @@ PAI_API pai_status pai_sdpa_paged(pai_ctx* ctx, const pai_tensor* q, const pai_t
       PAI_PDL_LAUNCH(e, "paged attention");
     }
   }
-  *out = r;
+  *out = r.take(0);
   return PAI_OK;
 }

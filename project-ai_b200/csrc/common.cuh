@@ -146,6 +146,29 @@ void raw_free(pai_ctx* ctx, void* p);
 
 // Allocates a contiguous tensor registered in the innermost scope. zero != 0 clears it on the stream.
 pai_status alloc_tensor(pai_ctx* ctx, int rank, const int32_t* dims, int dtype, bool zero, pai_tensor* out);
+// Result tensors of a call: released when it returns early, handed out by take().
+template <int N>
+struct Results {
+  pai_ctx* ctx;
+  pai_tensor t[N] = {};
+  int made = 0;
+  explicit Results(pai_ctx* c) : ctx(c) {}
+  Results(const Results&) = delete;
+  pai_status add(int rank, const int32_t* dims) {
+    PAI_TRY(alloc_tensor(ctx, rank, dims, PAI_F32, false, &t[made]));
+    made++;
+    return PAI_OK;
+  }
+  pai_tensor take(int i) {
+    const pai_tensor r = t[i];
+    t[i].base = nullptr;
+    return r;
+  }
+  ~Results() {
+    for (int i = 0; i < made; i++)
+      if (t[i].base) pai_release(ctx, t[i].base);
+  }
+};
 // A scratch buffer that is not a tensor: freed by the caller with raw_free (stream-ordered).
 struct Scratch {
   pai_ctx* ctx = nullptr;

@@ -277,8 +277,8 @@ PAI_API pai_status pai_paged_plan(pai_ctx* ctx, const pai_tensor* lengths, const
   const int n = lengths->dims[0];
   const int32_t d1 = n + 1, dn = n, dr = rows, d2 = 2;
   const int32_t* dims[5] = {&d1, &dn, &dr, &dr, &d2};
-  pai_tensor r[5];
-  for (int i = 0; i < 5; i++) PAI_TRY(alloc_tensor(ctx, 1, dims[i], PAI_F32, false, &r[i]));
+  Results<5> r(ctx);
+  for (int i = 0; i < 5; i++) PAI_TRY(r.add(1, dims[i]));
   paged::PlanArgs a{};
   a.len = fptr(*lengths); a.len_s = lengths->strides[0];
   a.add = fptr(*new_tokens); a.add_s = new_tokens->strides[0];
@@ -288,12 +288,12 @@ PAI_API pai_status pai_paged_plan(pai_ctx* ctx, const pai_tensor* lengths, const
   a.n = n; a.max_pages = table->dims[1]; a.pages = ring->dims[0]; a.rows = rows;
   a.per = (n + paged::kPlanThreads - 1) / paged::kPlanThreads;
   a.page = paged::page_div(page_size);
-  a.q_start = fptr(r[0]); a.kv_len = fptr(r[1]); a.slots = fptr(r[2]); a.positions = fptr(r[3]); a.next_state = fptr(r[4]);
+  a.q_start = fptr(r.t[0]); a.kv_len = fptr(r.t[1]); a.slots = fptr(r.t[2]); a.positions = fptr(r.t[3]); a.next_state = fptr(r.t[4]);
   a.error_flag = ctx->d_error_flag;
   PAI_PDL_LAUNCH(launch_pdl(paged::k_paged_plan, dim3(grid_for(ctx, rows, paged::kPlanThreads, 1, 2)),
                             dim3(paged::kPlanThreads), 0, ctx->stream, a),
                  "paged plan");
-  *q_start = r[0]; *kv_len = r[1]; *slots = r[2]; *positions = r[3]; *next_state = r[4];
+  *q_start = r.take(0); *kv_len = r.take(1); *slots = r.take(2); *positions = r.take(3); *next_state = r.take(4);
   return PAI_OK;
 }
 
@@ -307,8 +307,8 @@ PAI_API pai_status pai_paged_rope_append(pai_ctx* ctx, const pai_tensor* q, cons
   const char* names[9] = {"q", "k", "v", "cos", "sin", "positions", "slots", "k_cache", "v_cache"};
   for (int i = 0; i < 9; i++) PAI_TRY(check_view(ctx, ins[i], names[i]));
   PAI_TRY(pai_paged::check_append(set_error, q, k, v, cos_table, sin_table, positions, slots, k_cache, v_cache));
-  pai_tensor r;
-  PAI_TRY(alloc_tensor(ctx, 3, q->dims, PAI_F32, false, &r));
+  Results<1> r(ctx);
+  PAI_TRY(r.add(3, q->dims));
   paged::AppendArgs a{};
   a.q = fptr(*q); a.q0 = q->strides[0]; a.q1 = q->strides[1];
   a.k = fptr(*k); a.k0 = k->strides[0]; a.k1 = k->strides[1];
@@ -318,7 +318,7 @@ PAI_API pai_status pai_paged_rope_append(pai_ctx* ctx, const pai_tensor* q, cons
   a.slot = fptr(*slots); a.slot_s = slots->strides[0];
   a.kc = fptr(*k_cache); a.vc = fptr(*v_cache);
   a.c0 = k_cache->strides[0]; a.c1 = k_cache->strides[1]; a.c2 = k_cache->strides[2];
-  a.q_out = fptr(r);
+  a.q_out = fptr(r.t[0]);
   a.rows = q->dims[0]; a.H = q->dims[1]; a.KVH = k->dims[1]; a.D = q->dims[2];
   a.tab_rows = cos_table->dims[0]; a.slots = k_cache->dims[0] * k_cache->dims[2];
   a.page = paged::page_div(k_cache->dims[2]);
@@ -342,6 +342,6 @@ PAI_API pai_status pai_paged_rope_append(pai_ctx* ctx, const pai_tensor* q, cons
                        : launch_pdl(paged::k_paged_rope_append<false>, grid, dim3(256), 0, ctx->stream, a),
                    "paged rope append");
   }
-  *q_out = r;
+  *q_out = r.take(0);
   return PAI_OK;
 }

@@ -56,3 +56,49 @@ def test_an_error_of_the_device_clears_the_arrival_counters(fake, be):
             be.check_device_error()
         assert flag[0] == 0 and not tickets.any()
     assert be.check_device_error() == 0
+
+
+def in_use(be):
+    n = ctypes.c_int64()
+    be._c("memory_stats", ctypes.byref(n), None, None)
+    return n.value
+
+
+def plan_args(be):
+    return [be.allocate(s) for s in ((300,), (300,), (300, 2), (700,), (2,))] + [16, 70_000]
+
+
+def append_args(be):
+    q, k, v = be.allocate((700, 8, 64)), be.allocate((700, 2, 64)), be.allocate((700, 2, 64))
+    return [q, k, v, be.allocate((9, 64)), be.allocate((9, 64)), be.allocate((700,)), be.allocate((700,)), be.allocate((50, 2, 16, 64)), be.allocate((50, 2, 16, 64))]
+
+
+def attend_args(be):
+    return [be.allocate((700, 8, 64)), be.allocate((50, 2, 16, 64)), be.allocate((50, 2, 16, 64)), be.allocate((3, 9)), be.allocate((4,)),
+            be.allocate((3,)), 0.125]
+
+
+@pytest.mark.parametrize("op,args,allocations", [("paged_plan", plan_args, 5), ("paged_rope_append", append_args, 1), ("sdpa_paged", attend_args, 2)])
+def test_a_call_that_runs_out_of_memory_keeps_nothing(fake, be, op, args, allocations):
+    args = args(be)
+    held, launches = in_use(be), fake.lib.fake_launches()
+    for n in range(allocations):  # the allocation that fails
+        for scope in (False, True):
+            fake.lib.fake_fail_after(0)
+            with pytest.raises(MemoryError):  # gives cached blocks back: the next ones are new
+                be.allocate((1 << 22,))
+            fake.lib.fake_fail_after(n)
+            if scope:
+                be._c("scope_begin")
+            with pytest.raises(MemoryError):
+                getattr(be, op)(*args)
+            assert in_use(be) == held
+            if scope:
+                be._c("scope_end")
+    assert fake.lib.fake_launches() == launches
+    fake.lib.fake_fail_after(-1)
+    got = getattr(be, op)(*args)
+    assert fake.lib.fake_launches() == launches + 1 and in_use(be) > held
+    for t in got if isinstance(got, tuple) else (got,):
+        be.release(t)
+    assert in_use(be) == held
