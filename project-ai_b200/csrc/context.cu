@@ -402,14 +402,20 @@ PAI_API pai_status pai_ctx_create(int device, pai_ctx** out) {
   cudaError_t e2 = cudaStreamCreateWithFlags(&c->comm_stream, cudaStreamNonBlocking);
   cudaError_t e3 = cudaMalloc(&c->d_error_flag, 64);
   cudaError_t e4 = cudaMalloc(&c->d_tickets, kTickets * sizeof(unsigned));
-  if (e1 != cudaSuccess || e2 != cudaSuccess || e3 != cudaSuccess || e4 != cudaSuccess) {
+  bool ok = e1 == cudaSuccess && e2 == cudaSuccess && e3 == cudaSuccess && e4 == cudaSuccess;
+  // Cleared and waited for on the context's own stream: the default stream and the device may be in use by a graph capture of
+  // another context, which such a wait would end.
+  ok = ok && cudaMemsetAsync(c->d_error_flag, 0, 64, c->stream) == cudaSuccess &&
+       cudaMemsetAsync(c->d_tickets, 0, kTickets * sizeof(unsigned), c->stream) == cudaSuccess &&
+       cudaStreamSynchronize(c->stream) == cudaSuccess;
+  if (!ok) {
+    cudaFree(c->d_error_flag);
+    cudaFree(c->d_tickets);
+    if (c->stream) cudaStreamDestroy(c->stream);
+    if (c->comm_stream) cudaStreamDestroy(c->comm_stream);
     delete c;
     return set_error(PAI_ERR_CUDA, "failed to create streams for device %d", device);
   }
-  // both clears are ordered before the first kernel: the compute stream does not wait for the default stream by itself
-  cudaMemset(c->d_error_flag, 0, 64);
-  cudaMemset(c->d_tickets, 0, kTickets * sizeof(unsigned));
-  cudaDeviceSynchronize();
   *out = c;
   return PAI_OK;
 }

@@ -527,6 +527,24 @@ def test_two_captured_calls_and_eager_ones_share_the_context(cuda):
         cuda.graph_destroy(graph)
 
 
+@pytest.mark.gpu
+def test_a_context_can_be_created_while_another_captures(cuda, cuda_lib):
+    case = paged_case(131, 8, 2, 64, 16, [(300, 1), (9, 1)])
+    held = [cuda.from_host(x) for x in case]
+    ref, most, rms = attend_ref(*case, 0.125)
+    cuda.sdpa_paged(*held, 0.125, 1)
+    cuda.graph_begin()
+    out = cuda.sdpa_paged(*held, 0.125, 1)
+    other = cabi.NativeBackend(cuda_lib, 0)
+    graph = cuda.graph_end()
+    cuda.graph_launch(graph)
+    check_attention(ref, cuda.to_host(out), 64, 301, np.nanmax(np.abs(case[2])), most, rms)
+    check_attention(ref, attend(other, *case, 0.125, 1), 64, 301, np.nanmax(np.abs(case[2])), most, rms)
+    assert cuda.check_device_error() == 0 and other.check_device_error() == 0
+    cuda.graph_destroy(graph)
+    other.close()
+
+
 @pytest.mark.parametrize("new", [2, 90])
 def test_rows_without_keys_and_rows_of_no_request_are_zero(be, new):
     q, kc, vc, table, q_start, kv_len = paged_case(19, 4, 2, 64, 16, [(0, new), (5, 1)], 2)

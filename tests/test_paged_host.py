@@ -9,7 +9,7 @@ import pytest
 
 import projectai_b200
 from projectai_b200 import build
-from projectai_b200.cabi import DeviceTimeoutError, NativeBackend, NativeLibrary
+from projectai_b200.cabi import BackendError, DeviceTimeoutError, NativeBackend, NativeLibrary
 
 HERE = Path(__file__).resolve().parent
 OBJECTS = ("context", "paged", "attention_paged", "attention_paged_tc")
@@ -27,7 +27,7 @@ def fake(tmp_path_factory):
     lib.lib.fake_block.argtypes, lib.lib.fake_block.restype = [ctypes.c_size_t], ctypes.c_void_p
     lib.lib.fake_fail_after.argtypes = [ctypes.c_long]
     lib.lib.fake_log.restype = ctypes.c_char_p
-    lib.lib.fake_launches.restype = ctypes.c_long
+    lib.lib.fake_launches.restype = lib.lib.fake_blocks.restype = ctypes.c_long
     return lib
 
 
@@ -102,3 +102,22 @@ def test_a_call_that_runs_out_of_memory_keeps_nothing(fake, be, op, args, alloca
     for t in got if isinstance(got, tuple) else (got,):
         be.release(t)
     assert in_use(be) == held
+
+
+def test_creating_a_context_waits_for_nothing_but_its_own_stream(fake):
+    """Whatever else the device does, a graph capture of another context included."""
+    fake.lib.fake_log_clear()
+    b = NativeBackend(fake)
+    assert fake.lib.fake_log() == b""
+    assert not device(fake, 64, np.int32).any() and not device(fake, TICKETS, np.uint32).any()
+    b.close()
+
+
+def test_a_context_that_runs_out_of_memory_keeps_nothing(fake):
+    held = fake.lib.fake_blocks()
+    for n in range(2):
+        fake.lib.fake_fail_after(n)
+        with pytest.raises(BackendError):
+            NativeBackend(fake)
+        assert fake.lib.fake_blocks() == held
+    fake.lib.fake_fail_after(-1)
