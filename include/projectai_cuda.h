@@ -271,7 +271,7 @@ pai_status pai_paged_plan(pai_ctx* ctx, const pai_tensor* lengths, const pai_ten
  * [-1, pages * P) sets the error flag and writes nothing; a position outside the tables too, and its row of q_out is
  * 0. The tables have 2^24 rows at most. Slots other than -1 must differ from one another (pai_paged_plan's do): of two
  * rows with one slot, each element that the cache ends up with is one of theirs. q, k and v rows may be strided (unit
- * head-dim stride). */
+ * head-dim stride). The caches must not overlap one another or another operand. */
 pai_status pai_paged_rope_append(pai_ctx* ctx, const pai_tensor* q, const pai_tensor* k, const pai_tensor* v,
                                  const pai_tensor* cos_table, const pai_tensor* sin_table, const pai_tensor* positions,
                                  const pai_tensor* slots, const pai_tensor* k_cache, const pai_tensor* v_cache,

@@ -24,7 +24,60 @@ inline bool writable(const pai_tensor& t) {
   return true;
 }
 
-inline const float* first(const pai_tensor& t) { return static_cast<const float*>(t.base) + t.offset; }
+// Whether two views have an element in common: whether sum i_k s_k - sum j_k t_k = the distance of their first elements has a
+// solution within their dims. The terms are tried from the widest on, as far as those left can reach the rest, which for
+// nested and interleaved layouts are one or two at each; views whose search takes longer count as apart.
+class Overlap {
+  int64_t coef_[2 * PAI_MAX_RANK], most_[2 * PAI_MAX_RANK], reach_[2 * PAI_MAX_RANK + 1];
+  int terms_ = 0, budget_ = 4096;
+  bool search(int k, int64_t rest) {
+    if (rest < 0 || rest > reach_[k]) return false;
+    if (k == terms_) return rest == 0;
+    const int64_t hi = rest / coef_[k] < most_[k] ? rest / coef_[k] : most_[k];
+    const int64_t need = rest - reach_[k + 1];
+    for (int64_t i = need > 0 ? (need + coef_[k] - 1) / coef_[k] : 0; i <= hi; i++) {
+      if (budget_-- <= 0) return false;
+      if (search(k + 1, rest - i * coef_[k])) return true;
+    }
+    return false;
+  }
+  bool add(const pai_tensor& t, int64_t sign, int64_t* rest) {  // false: the view is empty
+    for (int i = 0; i < t.rank; i++) {
+      if (t.dims[i] == 0) return false;
+      int64_t c = sign * t.strides[i];
+      const int64_t n = t.dims[i] - 1;
+      if (n == 0 || c == 0) continue;
+      if (c < 0) {  // counted from the other end
+        *rest -= c * n;
+        c = -c;
+      }
+      int at = 0;
+      while (at < terms_ && coef_[at] > c) at++;
+      if (at < terms_ && coef_[at] == c) {
+        most_[at] += n;
+        continue;
+      }
+      for (int k = terms_++; k > at; k--) {
+        coef_[k] = coef_[k - 1];
+        most_[k] = most_[k - 1];
+      }
+      coef_[at] = c;
+      most_[at] = n;
+    }
+    return true;
+  }
+
+ public:
+  static bool of(const pai_tensor& a, const pai_tensor& b) {
+    if (a.base != b.base) return false;
+    Overlap o;
+    int64_t rest = b.offset - a.offset;
+    if (!o.add(a, 1, &rest) || !o.add(b, -1, &rest)) return false;
+    o.reach_[o.terms_] = 0;
+    for (int k = o.terms_ - 1; k >= 0; k--) o.reach_[k] = o.reach_[k + 1] + o.coef_[k] * o.most_[k];
+    return o.search(0, rest);
+  }
+};
 
 inline pai_status check_plan(Fail fail, const pai_tensor* lengths, const pai_tensor* new_tokens, const pai_tensor* table,
                              const pai_tensor* ring, const pai_tensor* state, int32_t page_size, int32_t rows) {
@@ -45,7 +98,7 @@ inline pai_status check_plan(Fail fail, const pai_tensor* lengths, const pai_ten
   const pai_tensor* all[5] = {lengths, new_tokens, table, ring, state};
   for (int w = 2; w < 4; w++)
     for (int i = 0; i < 5; i++)
-      if (i != w && all[i]->base == all[w]->base && first(*all[i]) == first(*all[w]) && n > 0)
+      if (i != w && Overlap::of(*all[i], *all[w]))
         return fail(PAI_ERR_ARGUMENT, "PagedPlan: table and ring are written in place and cannot share elements with another operand");
   return PAI_OK;
 }
@@ -95,8 +148,11 @@ inline pai_status check_append(Fail fail, const pai_tensor* q, const pai_tensor*
     return fail(PAI_ERR_UNSUPPORTED, "PagedRopeAppend: rows must be contiguous and the tables share one layout");
   if (!writable(*k_cache) || !writable(*v_cache))
     return fail(PAI_ERR_ARGUMENT, "PagedRopeAppend: the caches are written in place and cannot be broadcast views");
-  if (k_cache->base == v_cache->base && k_cache->offset == v_cache->offset && k_cache->dims[0] > 0)
-    return fail(PAI_ERR_ARGUMENT, "PagedRopeAppend: the k and v caches are the same elements");
+  const pai_tensor* others[7] = {q, k, v, cos_table, sin_table, positions, slots};
+  bool shared = Overlap::of(*k_cache, *v_cache);
+  for (int i = 0; i < 7; i++) shared = shared || Overlap::of(*others[i], *k_cache) || Overlap::of(*others[i], *v_cache);
+  if (shared)
+    return fail(PAI_ERR_ARGUMENT, "PagedRopeAppend: the caches are written in place and cannot share elements with one another or another operand");
   return PAI_OK;
 }
 

@@ -347,6 +347,55 @@ def test_append_refuses_tables_whose_rows_f32_cannot_name(be):
     assert be.check_device_error() == 0
 
 
+def view(t, offset, dims, strides):
+    r = t.copy_desc()
+    r.rank, r.offset = len(dims), offset
+    for i, (n, s) in enumerate(zip(dims, strides)):
+        r.dims[i], r.strides[i] = n, s
+    return r
+
+
+def test_plan_refuses_operands_that_share_elements(be):
+    """One buffer of [N, 2 + max_pages + ...]: columns of their own are fine, shared ones are not."""
+    n, pages = 3, 4
+    big = be.from_host(np.zeros(200, np.float32))
+    packed = [view(big, 0, (n,), (6,)), view(big, 1, (n,), (6,)), view(big, 2, (n, pages), (6, 1)), view(big, 100, (9,), (2,)), view(big, 101, (2,), (2,))]
+    be.paged_plan(*packed, 4, 2)  # lengths, new_tokens and table interleaved, ring and state too
+    assert be.check_device_error() == 0
+    for i, wrong in ((0, view(big, 2, (n,), (6,))), (1, view(big, 5, (n,), (6,))), (1, view(big, 17, (n,), (-6,))), (2, view(big, 98, (n, pages), (6, 1))),
+                     (3, view(big, 13, (9,), (1,))), (4, view(big, 100, (2,), (2,))), (4, view(big, 102, (2,), (1,)))):
+        args = list(packed)
+        args[i] = wrong
+        with pytest.raises(ArgumentError):
+            be.paged_plan(*args, 4, 2)
+
+
+def test_append_refuses_caches_that_share_elements(be):
+    d, page, pages, kvh = 16, 4, 5, 2
+    cos, sin = tables(8, d)
+    both = be.from_host(np.zeros((pages, 2, kvh, page, d), np.float32))  # keys and values of a page side by side
+    step, at = (2 * kvh * page * d, page * d, d, 1), kvh * page * d
+    kc, vc = view(both, 0, (pages, kvh, page, d), step), view(both, at, (pages, kvh, page, d), step)
+    q, k, v = be.from_host(rnd(1, 3, 4, d)), be.from_host(rnd(2, 3, kvh, d)), be.from_host(rnd(3, 3, kvh, d))
+    rest = [be.from_host(np.asarray(x, np.float32)) for x in (cos, sin, [0, 1, 2], [0, 1, 2])]
+    be.paged_rope_append(q, k, v, *rest, kc, vc)
+    assert be.check_device_error() == 0
+    for a, b in ((kc, view(both, at - d, (pages, kvh, page, d), step)), (kc, view(both, 2 * at, (pages - 1, kvh, page, d), step)),
+                 (view(both, 8, (pages - 1, kvh, page, d), step), vc)):
+        p = min(a.dims[0], b.dims[0])
+        with pytest.raises(ArgumentError):
+            be.paged_rope_append(q, k, v, *rest, *(view(x, x.offset, (p, kvh, page, d), step) for x in (a, b)))
+    inside = view(both, at, (3, kvh, d), (page * d, d, 1))  # rows of the value cache
+    for args in ((q, inside, v), (q, k, inside), (view(both, 0, (3, 4, d), (4 * d, d, 1)), k, v)):
+        with pytest.raises(ArgumentError):
+            be.paged_rope_append(*args, *rest, kc, vc)
+    for i in range(4):
+        wrong = list(rest)
+        wrong[i] = view(both, 3, tuple(rest[i].dims[:rest[i].rank]), tuple(rest[i].strides[:rest[i].rank]))
+        with pytest.raises(ArgumentError):
+            be.paged_rope_append(q, k, v, *wrong, kc, vc)
+
+
 # ---------------------------------------------------------------- attention
 def attend_ref(q, kc, vc, table, q_start, kv_len, scale):
     """float64, row by row; also max and root mean square of sum |q||k| scale for the tolerance."""
