@@ -67,9 +67,7 @@ class Overlap {
     return true;
   }
 
- public:
-  static bool of(const pai_tensor& a, const pai_tensor& b) {
-    if (a.base != b.base) return false;
+  static bool in_one_block(const pai_tensor& a, const pai_tensor& b) {
     Overlap o;
     int64_t rest = b.offset - a.offset;
     if (!o.add(a, 1, &rest) || !o.add(b, -1, &rest)) return false;
@@ -77,6 +75,9 @@ class Overlap {
     for (int k = o.terms_ - 1; k >= 0; k--) o.reach_[k] = o.reach_[k + 1] + o.coef_[k] * o.most_[k];
     return o.search(0, rest);
   }
+
+ public:
+  static bool of(const pai_tensor& a, const pai_tensor& b) { return a.base == b.base && in_one_block(a, b); }
 };
 
 inline pai_status check_plan(Fail fail, const pai_tensor* lengths, const pai_tensor* new_tokens, const pai_tensor* table,
