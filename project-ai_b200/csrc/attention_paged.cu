@@ -76,8 +76,8 @@ struct Scatter {
 // 32 / LPK such groups with KH consecutive keys each. The KH * R partial dot products of a group are summed over its
 // lanes by Scatter, which leaves each lane one (row, key) score to exponentiate; the probabilities go back to the
 // group's lanes by shuffles for P V. Keys and values come through a ring in shared memory, which each lane fills by
-// asynchronous copies two steps ahead with what it reads itself, so the ring needs no barrier and the keys on their way
-// (128 KB per SM) no registers. Weights are taken against 2^8 above a reference that follows the row maximum only when
+// asynchronous copies two steps ahead (five with one float4 per lane) with what it reads itself, so the ring needs no barrier
+// and the keys on their way (128 KB per SM, 160) no registers. Weights are taken against 2^8 above a reference that follows the row maximum only when
 // that rises by 2^8, so the sums are hardly ever rescaled, and no weight is above 1: a large value, weighted, does not
 // overflow. Steps of keys that every row attends have no masks, and where pages hold whole groups a group's page is looked
 // up once.
@@ -617,19 +617,13 @@ PAI_API pai_status pai_sdpa_paged(pai_ctx* ctx, const pai_tensor* q, const pai_t
   a.tickets = ctx->d_tickets;
   a.error_flag = ctx->d_error_flag;
   if (numel(r.t[0]) > 0) {
-    auto aligned = [](const pai_tensor& t) {
-      if (reinterpret_cast<uintptr_t>(fptr(t)) % 16) return false;
-      for (int i = 0; i + 1 < t.rank; i++)
-        if (t.dims[i] > 1 && t.strides[i] % 4) return false;
-      return true;
-    };
-    a.vec = a.D % 4 == 0 && aligned(*k_cache) && aligned(*v_cache);
-    a.q_vec = a.D % 4 == 0 && aligned(*q);
+    a.vec = a.D % 4 == 0 && paged::aligned(*k_cache) && paged::aligned(*v_cache);
+    a.q_vec = a.D % 4 == 0 && paged::aligned(*q);
     a.whole_groups = a.vec && a.page.size % paged::kGroupKeys == 0 && a.pages > 0;
     // Rows of one kv head: up to 8 the fp32 kernel reads each key once for all of them. Above, it would read keys again
     // for every 8 rows and its multiply-adds bound it; the tensor-core kernel's time hardly depends on the rows up to 128.
-    // Measured, 16 requests of about 1,900 keys, 8 kv heads of 64, us (fp32, tensor cores): 4 rows 45, 65; 8 rows 59, 65;
-    // 12 rows 85, 66; 24 rows 113, 67; 32 rows 143, 68; 12 kv heads, 8 rows 73, 81; 16 rows 112, 81.
+    // Measured by replayed graphs, 16 requests of about 1,900 keys, 8 kv heads of 64, us (fp32, tensor cores): 4 rows 37, 56;
+    // 8 rows 49, 56; 12 rows 75, 56; 24 rows 103, 57; 32 rows 133, 58; 12 kv heads, 8 rows 64, 74; 16 rows 104, 76.
     const int64_t most = (int64_t)a.max_new * a.g;
     const bool tc = most > 8 && paged::tc_fits(a);
     const int R = most <= 1 ? 1 : most <= 2 ? 2 : most <= 4 ? 4 : 8;

@@ -21,8 +21,8 @@
 //            only when the maximum has risen by 2^9, is an exact power of two and goes into the sums over tiles with the scale
 //            of V. There weights are at most 1, so that a sum of large values does not overflow before it is divided.
 // Per tile of keys the product P·V goes to its own accumulator and is added to fp32 registers, so the tensor cores' sums
-// stay short (24 steps). Four chunks of 2,000 tokens over 2,000 cached ones, 0.66 ms, take 1.1 ms with one large value per
-// request, 8.6 with one in each page of 16, 12.4 if all is fp32 work.
+// stay short (24 steps). Four chunks of 2,000 tokens over 2,000 cached ones, 0.66 ms, take 1.1 ms with a large value in
+// each of four pages, 8.6 with one in every page of 16, 12.4 if all is fp32 work.
 //
 // One persistent CTA per SM works on an item: 256 query rows (two tiles of 128, row = token * g + head of the group) of
 // one (request, kv head) against a run of key tiles:
@@ -38,13 +38,13 @@
 //   warp 27         walks the CTA's share of the work, hands the items to the others, and copies V as warp 24 does K.
 // Both query tiles use each converted K and V tile, which halves conversion and shared-memory writes per product. Up to
 // 128 rows there is one query tile: both softmax groups then work on it, each on every second key tile; the second hands
-// its result to the first through TMEM (six new tokens of 16 requests: 68 us, with one group 80; chunks among decoding
-// requests 135 and 155).
+// its result to the first through TMEM (six new tokens of 16 requests: 60 us, with one group 71; chunks among decoding
+// requests 129 and 148).
 //
-// Measured, 32 query heads over 8 kv heads of 64: four chunks of 2,000 tokens over 2,000 cached ones 0.66 to 0.70 ms, 227
-// to 240 TFLOP/s of results (158 GFLOP), i.e. 680 to 720 of fp16 products. A key tile takes 8,300 cycles there: the chain of
-// a query tile (scores 770 of tensor work, softmax 4,000, P·V 1,000, the waits between) with the other query tile's in the
-// gaps, and half of the issue slots.
+// Measured, 32 query heads over 8 kv heads of 64 (times in this file are those of a replayed graph of the call): four chunks
+// of 2,000 tokens over 2,000 cached ones 0.66 ms, 240 TFLOP/s of results (158 GFLOP), i.e. 720 of fp16 products. A key tile
+// takes 8,400 cycles there: the chain of a query tile (scores 770 of tensor work, softmax 4,100, P·V 1,000, the waits
+// between) with the other query tile's in the gaps, and half of the issue slots.
 //
 // Work split: as in k_paged_rows, the (item, key tile) units of all requests in one line, divided evenly over the CTAs;
 // an item that crosses CTAs leaves fp32 partial results that the last of them to finish joins in CTA order.
@@ -245,9 +245,9 @@ __device__ __forceinline__ void split2(float2 x, uint32_t& hi, uint32_t& lo) {
 }
 
 // A request's units: per kv head, groups of 256 rows, each with the key tiles that its last row attends. A tile counts as
-// many units as it takes time, about 8,300 cycles for two query tiles, 5,300 for one (chunks among decoding requests 135 us, 151
-// when all count alike), unless there are so few that a CTA has no more than two: then each counts alike, so that more
-// CTAs have one (small heads, 131 new tokens of 5 requests: 34 us, 40 with weights).
+// many units as it takes time, about 8,400 cycles for two query tiles, 5,300 for one (chunks among decoding requests 129 us,
+// 145 when all count alike), unless there are so few that a CTA has no more than two: then each counts alike, so that more
+// CTAs have one (small heads, 131 new tokens of 5 requests: 26.8 us, 28.2 with weights).
 struct Weights {
   int one, two;  // units of a key tile of a group of one, of two query tiles
   __device__ __forceinline__ int of(int rows, int group) const { return rows - group * 2 * kTcRows > kTcRows ? two : one; }
@@ -845,7 +845,7 @@ __device__ __forceinline__ void copies_hold(uint64_t* bar) {
 
 // Copies the raw K (op 0) or V (op 1) tiles of an item out of their pages, the CTA's tiles J and on: a page's rows with one
 // bulk copy where they make 1 KB or more (a bulk copy takes some 100 cycles to issue), else 16 bytes at a time, a lane per
-// row: six new tokens of 16 requests, pages of 16 or 8 positions 67 us, of 4 69; 16 bytes at a time 76. False if a wait gave up.
+// row: six new tokens of 16 requests, pages of 16 positions 58 us, of 4 62; 16 bytes at a time 69 and 72. False if a wait gave up.
 __device__ __forceinline__ bool load_item(const AttnArgs& a, TcShared& sh, uint8_t* tiles, int op, const Item& it, int& J,
                                           bool& bad) {
   const int lane = threadIdx.x & 31;

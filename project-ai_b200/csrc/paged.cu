@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const PlanArgs a) {
 // y[j] = x[j] cos[j] - x[j+h] sin[j], y[j+h] = x[j+h] cos[j+h] + x[j] sin[j+h] (h = D / 2), rounded as k_rope_append
 // rounds it (RotaryEmbedding, CpuComputeBackend.cs:397-420). Bound by HBM: each element is read once and written once.
 // A thread takes elements j.. and j+h.. (4 of each with VEC) of several heads of one row, so the row's table entries,
-// position and slot are read once for them; heads are q's, then k's, then v's. 8,000 rows of 32 + 2 8 heads of 64: 61 us,
+// position and slot are read once for them; heads are q's, then k's, then v's. 13,657 rows of 32 + 2·8 heads of 64: 61 us,
 // 5.5 TB/s.
 struct AppendArgs {
   const float* q; int64_t q0, q1;
@@ -252,13 +252,6 @@ __global__ void __launch_bounds__(256) k_paged_rope_append(const AppendArgs a) {
   }
 }
 
-static bool aligned(const pai_tensor& t) {  // 16-byte rows: every index but the last moves by whole float4
-  if (reinterpret_cast<uintptr_t>(fptr(t)) % 16) return false;
-  for (int i = 0; i + 1 < t.rank; i++)
-    if (t.dims[i] > 1 && t.strides[i] % 4) return false;
-  return true;
-}
-
 }  // namespace paged
 }  // namespace pai
 
@@ -330,8 +323,8 @@ PAI_API pai_status pai_paged_rope_append(pai_ctx* ctx, const pai_tensor* q, cons
                      paged::aligned(*v_cache);
     const int lanes = a.D / 2 / (vec ? 4 : 1);
     // One head per thread until the grid fills the GPU, then up to 8, which share one read of the tables, position and
-    // slot: 32 rows of 48 heads of 64, 10 us with one head (call included), 11 with four, 13 with eight; 8,000 rows 83, 69
-    // and 69 us.
+    // slot: 32 rows of 48 heads of 64, 4.2 us with one head (replayed graph), 4.3 with four, 6.3 with eight; 13,657 rows 77, 62
+    // and 63 us.
     const int64_t threads = (int64_t)a.rows * heads * lanes;
     int64_t share = threads / ((int64_t)ctx->sm_count * 2048);
     share = share < 1 ? 1 : share > 8 ? 8 : share;

@@ -29,6 +29,13 @@ inline PageDiv page_div(int size) {
   return PageDiv{size, (unsigned)(((1ull << (31 + l)) + d - 1) / d), 31 + l};
 }
 
+inline bool aligned(const pai_tensor& t) {  // 16-byte rows: every index but the last moves by whole float4
+  if (reinterpret_cast<uintptr_t>(fptr(t)) % 16) return false;
+  for (int i = 0; i + 1 < t.rank; i++)
+    if (t.dims[i] > 1 && t.strides[i] % 4) return false;
+  return true;
+}
+
 // Exclusive prefix sums of N values per thread over the block, in thread order; totals in every thread. `tmp` holds N values
 // per warp.
 template <int THREADS, int N>
