@@ -12,9 +12,9 @@
 //            do not, the tile takes the scale that suits most, and the others are left out and added in fp32, straight from
 //            their pages. (Within groups of two, ordinary data with some channels a hundred times the others would leave
 //            keys out in one tile of ten; within four, in one of a million. A number is thus as good as in fp32 next to the
-//            largest of its four.) A row of q that does not fit, or scores that could pass some thousand, where rounding
-//            is a matter of whole powers of two, makes all keys of a tile fp32 work for the row's warp. V tiles under 2^-60
-//            are, too: the factors below would take them out of the normal numbers.
+//            largest of its four.) A row of q that does not fit makes all keys fp32 work for its warp; so do scores that
+//            could pass some thousand, where rounding is a matter of whole powers of two, in tiles with values left out. V tiles
+//            under 2^-60 are left out, too: the factors below would take them out of the normal numbers.
 //   weights  exp(s - t) are taken against t, the power of two above the row's largest score in the tile, and times 2^14:
 //            all they lose is 2^-38 of the tile's largest. (With t following the row's maximum only now and then, a tile of
 //            small weights and large values lost all of them.) The factor from there to the row's reference, which does follow
@@ -209,8 +209,8 @@ __device__ __forceinline__ void bar_signal(int id, int threads) {
 }
 
 // A query row's scale times a key tile's, above which scores could be some thousand (numbers of the two up to 2^12 in product):
-// made once by the tensor cores and once in fp32 they could differ by more than 1, and weights of both kinds would no longer
-// go together, so all of the tile is fp32 work.
+// made once by the tensor cores and once in fp32 they could differ by more than 1. Weights of both kinds would no longer go
+// together for a value that is left out, so all of such a tile is fp32 work then.
 constexpr float kMostScore = 1.52587890625e-5f;  // 2^-16
 // The power of two that brings a magnitude (bits of a finite fp32, sign cleared) to [2^13, 2^14), and its inverse.
 // Magnitudes under 2^-112 keep the largest scale.
@@ -410,7 +410,11 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
       // kept finite and above 0: a score of 0 or -inf times it stays one
       const float kdown = sh.scale[0][slot];
       const float c = fminf(fmaxf(fabsf(qdown * kdown), 1.1754944e-38f), 3.4028235e38f);
-      const bool all_fp32 = q_most * fabsf(kdown) > kMostScore;
+      bool all_fp32 = q_most * fabsf(kdown) > kMostScore;
+      if (all_fp32 && q_most != INFINITY) {  // only where values are left out: their tile is not to be split again before this P
+        if (ok && !warp_wait_bar(&sh.conv[1][j % kTcStages], (j / kTcStages) & 1, &sh.abort)) ok = false;
+        all_fp32 = sh.scale[1][slot] < 0.0f;
+      }
       const uint4 seen = *reinterpret_cast<const uint4*>(sh.seen[0][slot]);
       if (t * kTcKeys + kTcKeys - 1 > first_limit || (seen.x & seen.y & seen.z & seen.w) != 0xffffffffu || all_fp32) {
         // scores of keys that do not exist or that the row does not attend become -inf in place
