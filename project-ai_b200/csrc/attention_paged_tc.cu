@@ -7,22 +7,23 @@
 //   q, K, V  are scaled by powers of two (exact) that bring the largest magnitude of a query row, or of a tile of 128 keys
 //            or values, to [2^13, 2^14). A number is then off by 2^-22 of itself or 2^-39 of the largest, whichever is
 //            more: the same for what lies within 2^16 of it. What a row does not attend shares the tile with what it does, so
-//            a single large number, anywhere in it, would take the precision of all others. A key (or value) fits a scale if
-//            none of its groups of four adjacent numbers is larger, and none that is not 0 is more than 2^16 below. Where some
-//            do not, the tile takes the scale that suits most, and the others are left out and added in fp32, straight from
-//            their pages. (Within groups of two, ordinary data with some channels a hundred times the others would leave
-//            keys out in one tile of ten; within four, in one of a million. A number is thus as good as in fp32 next to the
-//            largest of its four.) A row of q that does not fit makes all keys fp32 work for its warp; so do scores that
-//            could pass some thousand, where rounding is a matter of whole powers of two, in tiles with values left out. V tiles
-//            under 2^-60 are left out, too: the factors below would take them out of the normal numbers.
+//            a single large number, anywhere in it, would take the precision of all others. A tile of which some pair of
+//            numbers (of a group of four adjacent ones) is more than 2^16 below the largest is therefore sorted: it takes the
+//            scale that suits most keys (V, one for each head dim), and keys that do not fit are left out and added in fp32,
+//            straight from their pages. Numbers thus count as in fp32 next to the largest of their group of four, which is
+//            what the choice of keys goes by: single numbers of ordinary data are 2^16 below others often enough.
+//            A row of q of which half of the groups or more are far below the largest makes keys fp32 work for its warp (all,
+//            or those of uneven tiles); so do scores that could pass some thousand, where rounding is a matter of whole
+//            powers of two, in tiles with values left out.
 //   weights  exp(s - t) are taken against t, the power of two above the row's largest score in the tile, and times 2^14:
 //            all they lose is 2^-38 of the tile's largest. (With t following the row's maximum only now and then, a tile of
 //            small weights and large values lost all of them.) The factor from there to the row's reference, which does follow
 //            only when the maximum has risen by 2^9, is an exact power of two and goes into the sums over tiles with the scale
 //            of V. There weights are at most 1, so that a sum of large values does not overflow before it is divided.
 // Per tile of keys the product P·V goes to its own accumulator and is added to fp32 registers, so the tensor cores' sums
-// stay short (24 steps). Four chunks of 2,000 tokens over 2,000 cached ones, 0.66 ms, take 1.1 ms with a large value in
-// each of four pages, 8.6 with one in every page of 16, 12.4 if all is fp32 work.
+// stay short (24 steps). Four chunks of 2,000 tokens over 2,000 cached ones, 0.66 ms, take 1.9 ms where all tiles are sorted
+// (head dims of q, K and V that are always small), 1.1 with a large value in each of four pages, 4.4 with one in an eighth
+// of the pages of 16, 8.6 in all; 107 if everything is fp32 work (one head dim of q or K 2^17 above all others).
 //
 // One persistent CTA per SM works on an item: 256 query rows (two tiles of 128, row = token * g + head of the group) of
 // one (request, kv head) against a run of key tiles:
@@ -126,12 +127,13 @@ struct TcShared {
   float row_x[2][2][kTcRows];    // [query tile][half]: what the two threads of a row exchange
   float row_top[2][2][2][kTcRows];  // [turn][query tile][half]: their largest scores of a key tile, two sets
   alignas(16) uint32_t range[2][2][kConvWarps];  // converter warps' largest numbers and smallest pairs, as bf16 bits
-  uint32_t columns[2][kConvWarps];               // ... columns of groups of four that are not all 0
-  uint32_t keys[2][kTcKeys];                     // a key's (a value's) largest and smallest group
+  uint2 columns[2][kConvWarps][16];              // ... largest number of each head dim, four to a group
+  uint32_t keys[2][kTcKeys];                     // a key's (a value's) largest group, and kSound
   uint32_t small[kTcRing][4];                    // values left out of a tile that are smaller than the others
+  alignas(16) float v_scale[kTcRing][kTcDim];    // of a sorted V tile: `scale` for each head dim
   float join_m[kTcRows], join_l[kTcRows];        // split items: the second group's maxima and sums
-  // what a product with the tile is multiplied by to undo the tile's scale; negative: some keys of the tile are left to the
-  // fp32 path
+  // what a product with the tile is multiplied by to undo the tile's scale; negative: the tile was sorted, and keys may be left
+  // to the fp32 path
   float scale[2][kTcRing];
   int req;
   int unplaced;                  // a row range is invalid
@@ -220,15 +222,15 @@ __device__ __forceinline__ void tile_scale(uint32_t bits, float& up, float& down
   down = __uint_as_float((uint32_t)(e - 13) << 23);
 }
 __device__ __forceinline__ bool finite_bits(uint32_t bits) { return bits < 0x7f800000u; }
-// Magnitudes as bf16 bits (16 bits, exponent in steps of kExp): one lies more than 2^16 below another.
-constexpr uint32_t kExp = 128, kApart = 16 * kExp;
+// Magnitudes as bf16 bits (16 bits, exponent in steps of kExp): one lies more than 2^kApartExp below another.
+constexpr uint32_t kExp = 128, kApartExp = 16, kApart = kApartExp * kExp;
 // 2^e x, for x a power of two; 0 below the normal numbers. e x is no larger than they are.
 __device__ __forceinline__ float times_pow2(float x, int e) {
   const int field = (int)(__float_as_uint(x) >> 23) + e;
   return field > 0 ? __uint_as_float((uint32_t)field << 23) : 0.0f;
 }
 
-constexpr uint32_t kInf = 255 * kExp, kTiny = 67 * kExp;  // infinity, 2^-60
+constexpr uint32_t kInf = 255 * kExp, kTiny = 67 * kExp, kUnit = 140 * kExp;  // infinity, 2^-60, what has a scale of 1
 // max(|x|, |z|) and max(|y|, |w|) of four numbers, rounded to bf16; NaN counts as the largest.
 __device__ __forceinline__ __nv_bfloat162 max_abs4(float4 f) {
   return __hmax2_nan(__habs2(__floats2bfloat162_rn(f.x, f.y)), __habs2(__floats2bfloat162_rn(f.z, f.w)));
@@ -285,6 +287,23 @@ __device__ __forceinline__ void free_item(TcShared& sh, int i) {
 }
 
 // ---------------------------------------------------------------- roles
+// Of a row's groups of four: how many are within 2^16 of its largest number (in bf16 bits), in the upper half, and how many
+// further below but not 0. A call that reads the row again, as what it holds would be taken from all of the softmax.
+__device__ __noinline__ uint32_t row_groups(const float* q, int dims, float scale_hi, float scale_lo, uint32_t largest) {
+  uint32_t near = 0, far = 0;
+#pragma unroll 1
+  for (int d = 0; d < dims; d += 4) {
+    uint32_t four = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const uint32_t b = __float_as_uint(fmaf(q[d + e], scale_hi, q[d + e] * scale_lo)) & 0x7fffffffu;
+      if (finite_bits(b)) four = max(four, b);
+    }
+    if (four != 0) ((four >> 16) + kApart >= largest ? near : far)++;
+  }
+  return near << 16 | far;
+}
+
 // Softmax of query tile `tile`. After a timed-out wait `ok` stays false: no further TMEM or barrier-object work, but the
 // named barriers are met.
 __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, uint32_t tmem) {
@@ -343,8 +362,11 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
     const int s = a.heads.div(r), h = it.kvh * a.g + (r - s * a.g);
     const int limit = live ? it.shift + s : -1;  // the last key this row attends
     const int first_limit = it.shift + a.heads.div(first);
-    // undoes the row's scale; the largest of the warp's rows, infinite where a row has its numbers too far apart for one scale
-    float qdown, q_most;
+    // What undoes the row's scale; and K's scales (plain, of a sorted tile) above which a tile may be fp32 work for the warp.
+    // They are 0 if it is, because numbers of a row lie too far apart: where more than half of its groups are far below the
+    // largest, whatever the keys; where half are or are 0, with keys of a sorted tile, of which also half of the groups count.
+    // (Where fewer are, row and key share groups that count, and products of the others are small beside those.)
+    float qdown, k_most, k_least;
     {
       const float* p = a.q + (int64_t)(it.first + s) * a.q0 + (int64_t)h * a.q1;
       float x[32];
@@ -358,7 +380,7 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
         }
         x[d] = f.x; x[d + 1] = f.y; x[d + 2] = f.z; x[d + 3] = f.w;
       }
-      uint32_t big = 0, small = 0xffffffffu;  // largest number, smallest group of four that is not 0 (less 1)
+      uint32_t big = 0, least = 0xffffffffu;  // largest number, smallest of the groups of four
 #pragma unroll
       for (int d = 0; d < 32; d += 4) {
         uint32_t four = 0;
@@ -369,17 +391,21 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
           if (finite_bits(b)) four = max(four, b);
         }
         big = max(big, four);
-        small = min(small, four - 1);
+        if (32 * half + d < a.D) least = min(least, four);
       }
       // both in one word, in 16 bits each: the scale needs no more than the exponent
-      const uint32_t theirs = __float_as_uint(exchange(__uint_as_float((big & 0xffff0000u) | (small >> 16))));
+      const uint32_t theirs = __float_as_uint(exchange(__uint_as_float((big & 0xffff0000u) | (least >> 16))));
       big = max(big, theirs & 0xffff0000u);
-      small = min(small >> 16, theirs & 0xffffu);
-      const bool odd = __any_sync(0xffffffffu, small + kApart < (big >> 16));
+      least = min(least >> 16, theirs & 0xffffu);
       float up;
       tile_scale(big, up, qdown);
-      q_most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(qdown)));
-      if (odd) q_most = INFINITY;  // no key for the tensor cores
+      k_most = k_least = kMostScore / __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(qdown)));
+      if (__any_sync(0xffffffffu, least + kApart < (big >> 16))) {
+        const uint32_t groups = row_groups(p, live ? a.D : 0, a.scale_hi, a.scale_lo, big >> 16);
+        __syncwarp();
+        if (__any_sync(0xffffffffu, big != 0 && 8 * (groups >> 16) <= (uint32_t)a.D)) k_least = 0.0f;
+        if (__any_sync(0xffffffffu, 8 * (groups & 0xffffu) > (uint32_t)a.D)) k_most = 0.0f;
+      }
 #pragma unroll
       for (int c = 0; c < 2; c++) {  // 16 elements: 8 columns of hi, 8 of lo
         float hi[8], lo[8];
@@ -410,13 +436,14 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
       // kept finite and above 0: a score of 0 or -inf times it stays one
       const float kdown = sh.scale[0][slot];
       const float c = fminf(fmaxf(fabsf(qdown * kdown), 1.1754944e-38f), 3.4028235e38f);
-      bool all_fp32 = q_most * fabsf(kdown) > kMostScore;
-      if (all_fp32 && q_most != INFINITY) {  // only where values are left out: their tile is not to be split again before this P
-        if (ok && !warp_wait_bar(&sh.conv[1][j % kTcStages], (j / kTcStages) & 1, &sh.abort)) ok = false;
-        all_fp32 = sh.scale[1][slot] < 0.0f;
-      }
+      bool all_fp32 = kdown > k_most || -kdown > k_least;
       const uint4 seen = *reinterpret_cast<const uint4*>(sh.seen[0][slot]);
       if (t * kTcKeys + kTcKeys - 1 > first_limit || (seen.x & seen.y & seen.z & seen.w) != 0xffffffffu || all_fp32) {
+        if (all_fp32 && (kdown > 0.0f ? k_most : k_least) > 0.0f) {  // only where values are left out
+          // V cannot be split anew before this P
+          if (ok && !warp_wait_bar(&sh.conv[1][j % kTcStages], (j / kTcStages) & 1, &sh.abort)) ok = false;
+          all_fp32 = sh.scale[1][slot] < 0.0f;
+        }
         // scores of keys that do not exist or that the row does not attend become -inf in place
 #pragma unroll 1
         for (int g = 0; g < 4; g++) {
@@ -504,14 +531,17 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
         for (int pass = !ok ? 3 : v_drops ? 0 : 2; pass < 3; pass++) {
           if (pass == 1) near = __any_sync(0xffffffffu, near);
           if (!all && !near && pass == (v_drops ? 1 : 2)) {
-            const float down = times_pow2(fabsf(vdown), shift);
+            const float f = times_pow2(1.0f, shift);
 #pragma unroll
             for (int d = 0; d < 16; d += 4) {
               float x[8];
               tc::tmem_ld8(cpv + 2 * d, x);
 #pragma unroll
-              for (int e = 0; e < 4; e++)
-                o[d + e] = __ffma2_rn(make_float2(x[2 * e], x[2 * e + 1]), make_float2(down, down), o[d + e]);
+              for (int e = 0; e < 4; e++) {
+                float2 down = make_float2(vdown, vdown);
+                if (vdown < 0.0f) down = *reinterpret_cast<const float2*>(&sh.v_scale[my_slot][32 * my_half + 2 * (d + e)]);
+                o[d + e] = __ffma2_rn(__fmul2_rn(make_float2(x[2 * e], x[2 * e + 1]), make_float2(f, f)), down, o[d + e]);
+              }
             }
           }
 #pragma unroll 1
@@ -678,67 +708,124 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
   }
 }
 
-// For a tile whose numbers lie far apart: the largest magnitude (in bf16 bits; 0 if there is none) under which most keys keep
-// their precision; kLeft is added when not all do. Those are taken out of sh.seen and become 0. A key keeps its precision if none
-// of its groups of four is larger and none further than 2^16 below; groups of 0 do not count in K, in V unless all keys have
-// them. `rows` is the lane's place in its warp's rows.
-constexpr uint32_t kLeft = 1u << 16;
-__device__ __forceinline__ uint32_t sort_keys(const AttnArgs& a, TcShared& sh, uint8_t* rows, int op, int slot, bool ok) {
-  int tid = threadIdx.x;
-  asm volatile("" : "+r"(tid), "+r"(op), "+r"(slot));  // nothing of this is computed ahead of the branch that leads here
-  const int warp = (tid >> 5) & 3, lane = tid & 31, tr = lane >> 4, tc4 = lane & 15;
-  uint32_t any = 0;
-#pragma unroll 1
-  for (int e = 0; e < 16 && 4 * tc4 < a.D; e++) any |= bits2(max_abs4(*reinterpret_cast<const float4*>(rows + e * 512)));
-  __syncwarp();
-  const uint32_t n = __ballot_sync(0xffffffffu, any != 0);
-  if (lane == 0) sh.columns[op][warp] = n | n >> 16;
-  bar_named(kBarConv + op, 32 * kConvWarps);
-  const uint32_t columns = sh.columns[op][0] | sh.columns[op][1] | sh.columns[op][2] | sh.columns[op][3];
-  const bool counts = (columns >> tc4) & 1u;
+// For a tile whose numbers lie far apart: finds the scale that suits most keys, takes the others out of sh.seen and makes them
+// 0. Returns the magnitude (in bf16 bits; 0 if there is none) that bounds the tile's numbers. V has a scale for each head dim, as
+// a product's columns may be scaled as one likes, and is multiplied here. `rows` is the lane's place in its warp's rows.
+//   K: a key fits if it is no larger than that, and no more than 2^16 smaller, nor are half of its groups (a few head dims that
+//      are always small cost nothing; one that is always large would cost the others their precision);
+//   V: a value fits if its largest number is, and if then none of its groups is all 2^16 below the others that fit: weights are
+//      taken against the largest, which may be its own, and lose what is further below.
+// A call: in place it costs the loop around it 2% (six new tokens of 16 requests).
+constexpr uint32_t kNeutral = 1u << 31;  // the key does not count
+__device__ __noinline__ uint32_t sort_keys(TcShared& sh, uint8_t* rows, int dims, int op, int slot, bool ok) {
+  const int warp = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31, tr = lane >> 4, tc4 = lane & 15;
   const uint32_t seen = ok ? sh.seen[op][slot][warp] : 0u;
   uint32_t* keys = sh.keys[op];
+  auto group = [&](int e) {  // the lane's four numbers of row 2 e + tr
+    const float4 f = *reinterpret_cast<const float4*>(rows + e * 512);
+    const __nv_bfloat162 a = __floats2bfloat162_rn(f.x, f.y), b = __floats2bfloat162_rn(f.z, f.w);
+    return make_uint2(bits2(a) & 0x7fff7fffu, bits2(b) & 0x7fff7fffu);
+  };
+  auto most = [](uint2 g) { return max(max(g.x & 0xffffu, g.x >> 16), max(g.y & 0xffffu, g.y >> 16)); };
+  auto larger = [](uint2 a, uint2 b) { return make_uint2(__vmaxu2(a.x, b.x), __vmaxu2(a.y, b.y)); };
+  // the largest of the lane's head dims in those of the warp's rows, and then of all rows
+  auto column = [&](uint32_t of) {
+    uint2 m = make_uint2(0, 0);
+#pragma unroll 1
+    for (int e = 0; e < 16; e++)
+      if ((of >> (2 * e + tr)) & 1u) m = larger(m, group(e));
+    __syncwarp();
+    m = larger(m, make_uint2(__shfl_xor_sync(0xffffffffu, m.x, 16), __shfl_xor_sync(0xffffffffu, m.y, 16)));
+    if (tr == 0) sh.columns[op][warp][tc4] = 4 * tc4 < dims ? m : make_uint2(0, 0);
+    bar_named(kBarConv + op, 32 * kConvWarps);
+    m = make_uint2(0, 0);
+#pragma unroll 1
+    for (int w = 0; w < kConvWarps; w++) m = larger(m, sh.columns[op][w][tc4]);
+    return m;
+  };
+  uint2 largest = column(seen);
+  const bool counts = (largest.x | largest.y) != 0;
+  const int half = (dims / 4 + 1) / 2;  // of the groups
 #pragma unroll 1
   for (int e = 0; e < 16; e++) {
-    uint32_t hi = 0, lo = 0xffffu;
-    if (counts && ((seen >> (2 * e + tr)) & 1u)) {
-      const uint32_t m = bits2(max_abs4(*reinterpret_cast<const float4*>(rows + e * 512)));
-      hi = max(m & 0xffffu, m >> 16);
-      if (hi != 0 || op == 1) lo = hi;
-    }
+    const bool exists = (seen >> (2 * e + tr)) & 1u;
+    uint32_t hi = exists && counts ? most(group(e)) : 0;
 #pragma unroll 1
-    for (int o = 1; o < 16; o <<= 1) {
-      hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-      lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    }
-    if (tc4 == 0) keys[32 * warp + 2 * e + tr] = hi << 16 | lo;
+    for (int o = 1; o < 16; o <<= 1) hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    if (tc4 == 0) keys[32 * warp + 2 * e + tr] = !exists || (op == 0 && hi == 0) ? kNeutral : hi;
   }
   bar_named(kBarConv + op, 32 * kConvWarps);
-  auto fits = [&](uint32_t key, uint32_t top) { return key >> 16 <= top && (key & 0xffffu) + kApart >= top; };
-  uint32_t best = 0;  // how many keys fit, and under which magnitude, one of the keys' own
+  auto fits = [&](uint32_t key, uint32_t top) { return key == kNeutral || (key <= top && key + kApart >= top); };
+  // how many keys fit, and under which magnitude, one of the keys' own: the largest if all do
+  uint32_t best = 0, count = 0;
 #pragma unroll 1
-  for (int c = lane; c < kTcKeys; c += 32) {
-    const uint32_t top = keys[c] >> 16;
-    if (top == 0 || top >= kInf || (op == 1 && top < kTiny)) continue;
-    uint32_t count = 0;
-#pragma unroll 1
-    for (int i = 0; i < kTcKeys; i++) count += fits(keys[i], top) ? 1u : 0u;
-    best = max(best, count << 16 | top);
-  }
+  for (int c = lane; c < kTcKeys; c += 32)
+    if (keys[c] < kInf) best = max(best, keys[c]);
   __syncwarp();
   best = __reduce_max_sync(0xffffffffu, best);
-  const uint32_t top = best & 0xffffu, key = keys[32 * warp + lane];
-  const uint32_t out = __ballot_sync(0xffffffffu, best == 0 || !fits(key, top)) & seen;
-  const uint32_t small = __ballot_sync(0xffffffffu, best == 0 || (key & 0xffffu) + kApart < top) & out;
 #pragma unroll 1
-  for (int e = 0; e < 16; e++)  // missing rows, too: they are copies of one that may be among these
-    if (!(((seen & ~out) >> (2 * e + tr)) & 1u)) *reinterpret_cast<float4*>(rows + e * 512) = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int c = lane; c < kTcKeys; c += 32) count += fits(keys[c], best) ? 1u : 0u;
+  __syncwarp();
+  count = __reduce_add_sync(0xffffffffu, count);
+  if (count < kTcKeys) {
+    best = 0;
+#pragma unroll 1
+    for (int c = lane; c < kTcKeys; c += 32) {
+      const uint32_t top = keys[c];
+      if (top == 0 || top >= kInf) continue;
+      count = 0;
+#pragma unroll 1
+      for (int i = 0; i < kTcKeys; i++) count += fits(keys[i], top) ? 1u : 0u;
+      best = max(best, count << 16 | top);
+    }
+    __syncwarp();
+    best = __reduce_max_sync(0xffffffffu, best) & 0xffffu;
+  }
+  const uint32_t key = keys[32 * warp + lane];
+  uint32_t fit = __ballot_sync(0xffffffffu, best != 0 && fits(key, best)) & seen;
+  uint32_t small = __ballot_sync(0xffffffffu, best == 0 || key + kApart < best) & seen & ~fit, uneven = 0;
+  largest = op == 1 ? column(fit) : make_uint2(best | best << 16, best | best << 16);
+#pragma unroll 1
+  for (int e = 0; e < 16; e++) {
+    const uint2 g = group(e);
+    auto near = [&](uint32_t m, uint32_t of) { return (of != 0 && m != 0 && m + kApart >= of); };
+    const bool any = near(g.x & 0xffffu, largest.x & 0xffffu) || near(g.x >> 16, largest.x >> 16) ||
+                     near(g.y & 0xffffu, largest.y & 0xffffu) || near(g.y >> 16, largest.y >> 16);
+    const uint32_t n = __ballot_sync(0xffffffffu, op == 1 ? (largest.x | largest.y) != 0 && !any : any);
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+      const int of = __popc((n >> (16 * r)) & 0xffffu);
+      if (op == 1 ? of > 0 : of < half && keys[32 * warp + 2 * e + r] != kNeutral) uneven |= 1u << (2 * e + r);
+    }
+  }
+  uneven &= fit;
+  fit &= ~uneven;
+  small |= uneven;
+  float4 up = make_float4(1.f, 1.f, 1.f, 1.f);
+  if (op == 1) {
+    float4 down;
+    tile_scale(largest.x << 16, up.x, down.x);
+    tile_scale(largest.x & 0xffff0000u, up.y, down.y);
+    tile_scale(largest.y << 16, up.z, down.z);
+    tile_scale(largest.y & 0xffff0000u, up.w, down.w);
+    if (warp == 0 && lane < 16) *reinterpret_cast<float4*>(&sh.v_scale[slot][4 * lane]) = down;
+  }
+#pragma unroll 1
+  for (int e = 0; e < 16; e++) {  // missing rows, too: they are copies of one that may be left out
+    float4* row = reinterpret_cast<float4*>(rows + e * 512);
+    float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+    if ((fit >> (2 * e + tr)) & 1u) {
+      f = *row;
+      f = make_float4(f.x * up.x, f.y * up.y, f.z * up.z, f.w * up.w);
+    }
+    *row = f;
+  }
   if (lane == 0) {
-    if (out != 0) sh.seen[op][slot][warp] = seen & ~out;
+    if (fit != seen) sh.seen[op][slot][warp] = fit;
     if (op == 1) sh.small[slot][warp] = small;
   }
   __syncwarp();
-  return top + (best >> 16 < kTcKeys ? kLeft : 0u);
+  return op == 1 ? kUnit : best;
 }
 
 // Splits the raw K (op 0) or V (op 1) tiles in place. A warp has four of a tile's groups of eight rows; a first pass takes
@@ -799,12 +886,12 @@ __device__ __forceinline__ void convert_role(const AttnArgs& a, TcShared& sh, ui
       const uint4 all = *reinterpret_cast<const uint4*>(range);
       uint32_t top = max(max(all.x, all.y), max(all.z, all.w)) >> 16;
       const uint32_t low = min(min(all.x & 0xffffu, all.y & 0xffffu), min(all.z & 0xffffu, all.w & 0xffffu));
-      if (low + kApart < top || top >= kInf || (op == 1 && top != 0 && top < kTiny))
-        top = sort_keys(a, sh, tile + from, op, J % kTcRing, ok);
+      const bool sort = low + kApart < top || top >= kInf || (op == 1 && top != 0 && top < kTiny);
+      if (sort) top = sort_keys(sh, tile + from, a.D, op, J % kTcRing, ok);
       if (ok) {
         float up, down;
         tile_scale(top << 16, up, down);
-        if (warp == 0 && lane == 0) sh.scale[op][J % kTcRing] = top >= kLeft ? -down : down;
+        if (warp == 0 && lane == 0) sh.scale[op][J % kTcRing] = sort ? -down : down;
         const float2 up2 = make_float2(up, up);
 #pragma unroll 1
         for (int g = 0; g < 4; g++) {

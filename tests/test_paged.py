@@ -655,15 +655,21 @@ def test_attention_of_a_few_large_keys_among_small_ones(be, reqs):
     check_attention(ref, got, 64, 170, np.abs(vc).max(), most, rms)
 
 
-def attend_bound(q, kc, vc, table, q_start, kv_len, scale):
+def fours(x):
+    """Each number replaced by the largest of its group of four adjacent ones."""
+    g = np.abs(x.astype(np.float64)).reshape(*x.shape[:-1], -1, 4).max(-1, keepdims=True)
+    return np.broadcast_to(g, (*g.shape[:-1], 4)).reshape(x.shape)
+
+
+def attend_bound(q, kc, vc, table, q_start, kv_len, scale, size=np.abs):
     """float64 result and a bound of its error for each element. With w_j the weights of the row, a score's error is at
     most (D + 16) u sum |q||k| scale (see above), which bends its weight by twice that, e_j, relatively, and the sums add
     (L + 32) u: |error of o_d| <= sum_j w_j |v_jd| (e_j + (L + 32) u) + |o_d| sum_j w_j e_j. Keys of weight 0 count
     for nothing, however large, and so does what other rows attend. A weight is not asked to be exact under 2^-100,
-    and its products not under fp32's smallest normal number."""
+    and its products not under fp32's smallest normal number. `size` is what counts for |x|: abs, or fours."""
     rows, h, d = q.shape
     page, g = kc.shape[2], h // kc.shape[1]
-    out, tol = np.zeros((rows, h, d)), np.zeros((rows, h, d))
+    out, tol = np.zeros((rows, h, d)), np.full((rows, h, d), 2.0 ** -126)  # rows of no request are 0
     for i in range(len(kv_len)):
         a, b, length = q_start[i], q_start[i + 1], kv_len[i]
         ids = table[i, :ceil_div(length, page)]
@@ -676,14 +682,14 @@ def attend_bound(q, kc, vc, table, q_start, kv_len, scale):
                 s = kk @ x * scale
                 w = np.exp(s - s.max())
                 w /= w.sum()
-                e = 2 * (d + 16) * U * (np.abs(kk) @ np.abs(x)) * scale
+                e = 2 * (d + 16) * U * (size(kk) @ size(x)) * scale
                 out[r, j] = w @ vv
-                tol[r, j] = (w * (e + (n + 32) * U) + 2.0 ** -100) @ np.abs(vv) + np.abs(out[r, j]) * (w @ e) + 2.0 ** -126
+                tol[r, j] = (w * (e + (n + 32) * U) + 2.0 ** -100) @ size(vv) + np.abs(out[r, j]) * (w @ e) + 2.0 ** -126
     return out, tol
 
 
-def check_bound(be, case, scale, max_new=0):
-    ref, tol = attend_bound(*case, scale)
+def check_bound(be, case, scale, max_new=0, size=np.abs):
+    ref, tol = attend_bound(*case, scale, size)
     got = attend(be, *case, scale, max_new).astype(np.float64)
     assert np.isfinite(got).all()
     worst = (np.abs(got - ref) / tol).max()
@@ -807,9 +813,49 @@ def test_the_largest_value_of_the_type_does_not_overflow(be, reqs, max_new, d, s
     check_bound(be, case, d ** -0.5, max_new)
 
 
+def sizes(rng, shape, kind, decades):
+    """Factors up to 10^decades either way: none; some positions; some channels; some numbers; zero positions; zero numbers; one for all."""
+    n, d = shape[0], shape[-1]
+    some = lambda size, part: np.where(rng.random(size) < part, rng.uniform(-decades, decades, size), 0.0)  # noqa: E731
+    f = {0: np.zeros(1), 1: some(n, rng.choice([0.02, 0.2, 0.6])).reshape(-1, *[1] * (len(shape) - 1)), 2: some(d, rng.choice([0.03, 0.3, 0.7])),
+         3: some(shape, rng.choice([0.001, 0.01, 0.3])), 6: rng.uniform(-decades, decades, 1)}
+    if kind == 4: return (rng.random(n) < 0.8).astype(np.float64).reshape(-1, *[1] * (len(shape) - 1))
+    if kind == 5: return (rng.random(shape) < 0.5).astype(np.float64)
+    return 10.0 ** f[kind]
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_numbers_far_apart_at_random(be, seed):
+    """Groups of four adjacent head dims count as their largest number, which is what the tensor-core kernel promises."""
+    rng = np.random.default_rng(1000 + seed)
+    done = 0
+    while done < 4:
+        d, kvh, g, page = int(rng.choice([4, 8, 16, 20, 48, 64, 64])), int(rng.choice([1, 2])), int(rng.choice([1, 2, 4, 8])), int(rng.choice([1, 4, 5, 16]))
+        reqs = [(int(rng.integers(0, 300)), int(rng.choice([1, 3, 20, 70]))) for _ in range(int(rng.integers(1, 3)))]
+        q, kc, vc, table, q_start, kv_len = paged_case(int(rng.integers(1 << 30)), g * kvh, kvh, d, page, reqs, 1, stale=float(rng.choice([0.0, np.nan, 3e38])))
+        decades, scale = float(rng.choice([3, 6, 12, 25])), float(rng.choice([d ** -0.5, 1.0, 0.01]))
+        kinds = rng.integers(0, 7, 3)
+        q = (q * sizes(rng, q.shape, int(kinds[0]), decades)).astype(np.float32)
+        largest = 0.0
+        for x, kind in ((kc, int(kinds[1])), (vc, int(kinds[2]))):
+            for i, n in enumerate(kv_len):
+                at = np.arange(n)
+                part = x[table[i, at // page], :, at % page]
+                part = np.clip(part * sizes(rng, part.shape, kind, decades), -3e38, 3e38).astype(np.float32)
+                x[table[i, at // page], :, at % page] = part
+                if x is kc: largest = max(largest, float(np.abs(part).max()))
+        case = [q, kc, vc, table, q_start, kv_len]
+        with np.errstate(over="ignore"):
+            if float(np.abs(q).max()) * largest * d * max(1.5 * scale, 1.0) > 1e37 or np.abs(attend_bound(*case, scale)[0]).max() > 1e36:
+                continue  # scores or sums that F32 does not hold
+        done += 1
+        check_bound(be, case, scale, max(x for _, x in reqs), fours)
+
+
 @pytest.mark.parametrize("reqs,max_new,d", WIDE)
 @pytest.mark.parametrize("what", ["k 1e8, q 1e-8", "q 1e8, k 1e-8", "q 1e12, k 0", "v 1e8", "v 1e20", "v zeros of the weightiest key", "v column of zeros",
-                                  "v 1e36", "v 1e-36", "k zeros", "rows of q far apart"])
+                                  "v 1e36", "v 1e-36", "k zeros", "rows of q far apart", "four of k 1e-7", "four of v 1e-7", "four of q 1e-7",
+                                  "four of all 1e-7", "half of v 1e-20", "half of q and k 1e-9", "zeros at the end", "v tiny and large"])
 def test_channels_of_sizes_far_apart(be, reqs, max_new, d, what):
     q, kc, vc, *rest = paged_case(107, 4, 2, d, 16, reqs, 0, stale=0.0)
     case = [q, kc, vc, *rest]
@@ -822,6 +868,13 @@ def test_channels_of_sizes_far_apart(be, reqs, max_new, d, what):
     if what == "v 1e36": vc *= np.float32(1e36)
     if what == "v 1e-36": vc *= np.float32(1e-36)
     if what == "k zeros": kc[rest[0][0, 0], :, 3:9] = 0; kc[..., 8:12] = 0
+    if what.startswith("four of"):
+        for x, name in ((q, "q"), (kc, "k"), (vc, "v")):
+            if name in what[8:] or "all" in what: x[..., 4:8] *= np.float32(1e-7)
+    if what == "half of v 1e-20": vc[..., ::2] *= np.float32(1e-20)
+    if what == "half of q and k 1e-9": q[..., d // 2:] *= np.float32(1e-9); kc[..., : d // 2] *= np.float32(1e-9)
+    if what == "zeros at the end": q[..., -d // 4:] = 0; kc[..., -d // 4:] = 0; vc[..., -d // 4:] = 0
+    if what == "v tiny and large": vc *= np.float32(10.0) ** np.linspace(-34, 30, d).astype(np.float32)
     if what == "rows of q far apart": q *= np.float32(2.0) ** -np.arange(len(q), dtype=np.float32)[:, None, None].clip(0, 60)
     if what.startswith("v zeros"):
         q[..., 5] = 1.0
