@@ -130,6 +130,7 @@ struct TcShared {
   uint2 columns[2][kConvWarps][16];              // ... largest number of each head dim, four to a group
   uint32_t keys[2][kTcKeys];                     // a key's (a value's) largest group, and kSound
   uint32_t small[kTcRing][4];                    // values left out of a tile that are smaller than the others
+  float k_sorted[2 * kSoftmaxWarps];             // of a softmax warp: K's scale above which a sorted tile may be fp32 work
   alignas(16) float v_scale[kTcRing][kTcDim];    // of a sorted V tile: `scale` for each head dim
   float join_m[kTcRows], join_l[kTcRows];        // split items: the second group's maxima and sums
   // what a product with the tile is multiplied by to undo the tile's scale; negative: the tile was sorted, and keys may be left
@@ -362,11 +363,11 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
     const int s = a.heads.div(r), h = it.kvh * a.g + (r - s * a.g);
     const int limit = live ? it.shift + s : -1;  // the last key this row attends
     const int first_limit = it.shift + a.heads.div(first);
-    // What undoes the row's scale; and K's scales (plain, of a sorted tile) above which a tile may be fp32 work for the warp.
+    // What undoes the row's scale; and K's scale above which a tile may be fp32 work for the warp, for sorted tiles in sh.k_sorted.
     // They are 0 if it is, because numbers of a row lie too far apart: where more than half of its groups are far below the
     // largest, whatever the keys; where half are or are 0, with keys of a sorted tile, of which also half of the groups count.
     // (Where fewer are, row and key share groups that count, and products of the others are small beside those.)
-    float qdown, k_most, k_least;
+    float qdown, k_most;
     {
       const float* p = a.q + (int64_t)(it.first + s) * a.q0 + (int64_t)h * a.q1;
       float x[32];
@@ -399,13 +400,8 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
       least = min(least >> 16, theirs & 0xffffu);
       float up;
       tile_scale(big, up, qdown);
-      k_most = k_least = kMostScore / __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(qdown)));
-      if (__any_sync(0xffffffffu, least + kApart < (big >> 16))) {
-        const uint32_t groups = row_groups(p, live ? a.D : 0, a.scale_hi, a.scale_lo, big >> 16);
-        __syncwarp();
-        if (__any_sync(0xffffffffu, big != 0 && 8 * (groups >> 16) <= (uint32_t)a.D)) k_least = 0.0f;
-        if (__any_sync(0xffffffffu, 8 * (groups & 0xffffu) > (uint32_t)a.D)) k_most = 0.0f;
-      }
+      k_most = kMostScore / __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(qdown)));
+      const bool uneven = __any_sync(0xffffffffu, least + kApart < (big >> 16));
 #pragma unroll
       for (int c = 0; c < 2; c++) {  // 16 elements: 8 columns of hi, 8 of lo
         float hi[8], lo[8];
@@ -422,6 +418,15 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
       tmem_st_wait();
       fence_before();
       bar_signal(kBarIssue + tile, 64 * quads + 32);
+      float k_sorted = k_most;
+      if (uneven) {
+        const uint32_t groups = row_groups(p, live ? a.D : 0, a.scale_hi, a.scale_lo, big >> 16);
+        __syncwarp();
+        if (__any_sync(0xffffffffu, big != 0 && 8 * (groups >> 16) <= (uint32_t)a.D)) k_sorted = 0.0f;
+        if (__any_sync(0xffffffffu, 8 * (groups & 0xffffu) > (uint32_t)a.D)) k_most = 0.0f;
+      }
+      if (lane == 0) sh.k_sorted[warp] = k_sorted;
+      __syncwarp();
     }
     float2 o[16];
 #pragma unroll
@@ -436,13 +441,16 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, TcShared& sh, ui
       // kept finite and above 0: a score of 0 or -inf times it stays one
       const float kdown = sh.scale[0][slot];
       const float c = fminf(fmaxf(fabsf(qdown * kdown), 1.1754944e-38f), 3.4028235e38f);
-      bool all_fp32 = kdown > k_most || -kdown > k_least;
+      bool all_fp32 = __float_as_uint(kdown) > __float_as_uint(k_most);  // or the tile is sorted
       const uint4 seen = *reinterpret_cast<const uint4*>(sh.seen[0][slot]);
       if (t * kTcKeys + kTcKeys - 1 > first_limit || (seen.x & seen.y & seen.z & seen.w) != 0xffffffffu || all_fp32) {
-        if (all_fp32 && (kdown > 0.0f ? k_most : k_least) > 0.0f) {  // only where values are left out
-          // V cannot be split anew before this P
-          if (ok && !warp_wait_bar(&sh.conv[1][j % kTcStages], (j / kTcStages) & 1, &sh.abort)) ok = false;
-          all_fp32 = sh.scale[1][slot] < 0.0f;
+        if (all_fp32) {
+          const float least = kdown > 0.0f ? k_most : sh.k_sorted[warp];
+          all_fp32 = fabsf(kdown) > least;
+          if (all_fp32 && least > 0.0f) {  // only where values are left out; V cannot be split anew before this P
+            if (ok && !warp_wait_bar(&sh.conv[1][j % kTcStages], (j / kTcStages) & 1, &sh.abort)) ok = false;
+            all_fp32 = sh.scale[1][slot] < 0.0f;
+          }
         }
         // scores of keys that do not exist or that the row does not attend become -inf in place
 #pragma unroll 1
