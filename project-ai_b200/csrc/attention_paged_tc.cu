@@ -21,8 +21,8 @@
 //            only when the maximum has risen by 2^9, is an exact power of two and goes into the sums over tiles with the scale
 //            of V. There weights are at most 1, so that a sum of large values does not overflow before it is divided.
 // Per tile of keys the product P·V goes to its own accumulator and is added to fp32 registers, so the tensor cores' sums
-// stay short (24 steps). Four chunks of 2,000 tokens over 2,000 cached ones, 0.66 ms, take 1.9 ms where all tiles are sorted
-// (head dims of q, K and V that are always small), 1.1 with a large value in each of four pages, 4.4 with one in an eighth
+// stay short (24 steps). Four chunks of 2,000 tokens over 2,000 cached ones, 0.66 ms, take 1.8 to 2.2 ms where all tiles are
+// sorted (head dims of K or V that are always small), 1.1 with a large value in each of four pages, 4.4 with one in an eighth
 // of the pages of 16, 8.6 in all; 107 if everything is fp32 work (one head dim of q or K 2^17 above all others).
 //
 // One persistent CTA per SM works on an item: 256 query rows (two tiles of 128, row = token * g + head of the group) of
